@@ -488,6 +488,65 @@ int moe_ep_p2p_experts(const moe_ep_p2p *p, const uint16_t *gate_up, const uint1
                        size_t workspace_bytes, void *const *kernel_events, void *stream);
 int moe_ep_p2p_finish(const moe_ep_p2p *p, void *stream);
 
+/* ---------------------------------------------------------------- FP8 ----
+ * The MoE layer on e4m3 values with FP32 scales.  Activations carry one scale
+ * per row and 128 columns ([T, ceil(n / 128)], row-major), weights one per
+ * 128 x 128 block ([.., ceil(N / 128), ceil(K / 128)], row-major; blocks are
+ * cut at the matrix's edges).  A group of values v_i is held as
+ *   a = max(max |v_i|, 1e-10),  q_i = e4m3(v_i * 448 / a),  scale = a / 448
+ * and read back as q_i * scale.  A group that holds a NaN or an infinity is
+ * NaN throughout, and so is what is computed from it; other rows are not
+ * touched by it.
+ *
+ * The reference keeps its experts in BF16 (edge35b/expert_stream.py:356); these
+ * entry points stand beside the BF16 ones for weights that ship, or are
+ * brought, to FP8.
+ */
+
+/* The residual addition, RMS norm and e4m3 form of rows:
+ *   r = bf16(x + residual)          (r = x without a residual)
+ *   y = r * rsqrt(mean(r^2) + eps) * (weight_offset + weight)
+ * q [T, H] and scales [T, ceil(H / 128)] hold y (before any rounding to BF16),
+ * normed [T, H] BF16 (may be NULL) its rounding, residual_out [T, H] BF16 (may
+ * be NULL) r.  weight_offset is 1 for norms whose weight is stored around zero.
+ * weight NULL: no norm, q and scales hold x itself (residual, normed and
+ * residual_out must be NULL).  x and residual rows lie x_stride and
+ * residual_stride elements apart; the outputs are dense.  residual_out may be
+ * residual and normed may be x (same address and dense rows); no other
+ * overlap. */
+int moe_rmsnorm_fp8(const uint16_t *x, int64_t x_stride, const uint16_t *residual, int64_t residual_stride,
+                    const uint16_t *weight, float weight_offset, float eps, int tokens, int hidden, uint8_t *q,
+                    float *scales, uint16_t *normed, uint16_t *residual_out, void *stream);
+
+/* BF16 weights [banks, rows, cols] to e4m3 q of the same shape and scales
+ * [banks, ceil(rows / 128), ceil(cols / 128)]. */
+int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, uint8_t *q, float *scales,
+                            void *stream);
+
+/* out[T, rows] (BF16, or FP32 with out_f32 = 1) = x . w^T on the values that x
+ * [T, cols] and w [rows, cols] stand for, products summed in FP32.  cols must
+ * be a multiple of 16; x, w and out are 16-byte aligned.  The workspace query
+ * may return 0: workspace may then be NULL. */
+size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols);
+int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
+                   int rows, int cols, void *out, int out_f32, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
+/* The routed experts (the Qwen3_5MoeExperts.forward contract of
+ * moe_layer_forward with route_in) on e4m3 banks gate_up [E, 2I, H] and down
+ * [E, H, I]: for each route (t, k) of expert e = idx[t, k]
+ *   h = silu(gate . x_t) * (up . x_t)  in FP32, brought to e4m3 per 128 values
+ *   out[t] += weights[t, k] * (down . h)
+ * with FP32 sums and one rounding to BF16 at the end on the smallest batches;
+ * larger ones keep each route's row as BF16 before the weighted sum.  Ids
+ * outside [0, E) contribute nothing (a token with none left is 0).  hidden is
+ * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024. */
+size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner);
+int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up, const float *gate_up_scales,
+                    const uint8_t *down, const float *down_scales, const int64_t *idx, const uint16_t *weights,
+                    int tokens, int experts, int top_k, int hidden, int inner, uint16_t *out, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,91 @@
+// Shared pieces of the FP8 operators: e4m3 values with one FP32 scale per row
+// and 128 columns (activations) or per 128 x 128 block (weights).
+//
+// A group of 128 values x_i is held as q_i = e4m3(x_i * 448 / a), s = a / 448,
+// with a = max(max |x_i|, 1e-10); x_i is read back as q_i * s.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace lrb {
+namespace fp8 {
+
+constexpr int kGroup = 128;       // values that share a scale
+constexpr float kTop = 448.0f;    // the largest e4m3 value
+constexpr float kTiny = 1e-10f;   // a group's maximum counts as at least this
+
+__host__ __device__ constexpr int groups(int n) { return (n + kGroup - 1) / kGroup; }
+
+// The larger of two magnitudes, NaN if either is: a group that holds a NaN
+// must not come out as numbers.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// One group's divisor.  q = x * 448 / a is computed as (1.75 x 2^-8) / (a 2^-16):
+// both factors of 1.75 = 7/4 and the powers of two are exact for a BF16 x, and
+// neither side can overflow.  The quotient starts as t * (1 / d) and takes one
+// residual step, q + (t - q d) / d with the residual exact in an FMA.  A value
+// that lies on a border of two e4m3 values is representable, so the step makes
+// it exact and the tie rounds to even as it would after an exact division; any
+// other quotient of BF16 x and a is at least 2^-13 away from a border, far more
+// than the last error.  Three instructions a value instead of a full division.
+// A NaN maximum gives NaN; an infinite one gives 1/d = 0 and a NaN residual, so
+// a group that holds an infinity is NaN throughout as well.
+struct Divisor {
+    float d, r;
+    __device__ __forceinline__ explicit Divisor(float a) : d(a * 0x1p-16f), r(1.0f / (a * 0x1p-16f)) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        const float t = x * (1.75f * 0x1p-8f);
+        const float q = t * r;
+        return fmaf(fmaf(-q, d, t), r, q);
+    }
+};
+
+__device__ __forceinline__ float scale_of(float a) { return __fdiv_rn(a, kTop); }
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t pack4(const Divisor &f, float a, float b, float c, float d) {
+    return pack2(f(a), f(b)) | (pack2(f(c), f(d)) << 16);
+}
+
+// Two e4m3 values (the low 16 bits) as FP32; exact.
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+__device__ __forceinline__ void unpack16(uint4 v, float (&f)[16]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = unpack2(w[i] & 0xffff), b = unpack2(w[i] >> 16);
+        f[4 * i] = a.x;
+        f[4 * i + 1] = a.y;
+        f[4 * i + 2] = b.x;
+        f[4 * i + 3] = b.y;
+    }
+}
+// dot(16 e4m3 weights, 16 FP32 activations) in FP32.
+__device__ __forceinline__ float dot16(uint4 w, const float (&x)[16]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 lo = unpack2(u[i] & 0xffff), hi = unpack2(u[i] >> 16);
+        a = fmaf(lo.x, x[4 * i], a);
+        b = fmaf(lo.y, x[4 * i + 1], b);
+        a = fmaf(hi.x, x[4 * i + 2], a);
+        b = fmaf(hi.y, x[4 * i + 3], b);
+    }
+    return a + b;
+}
+
+}  // namespace fp8
+}  // namespace lrb

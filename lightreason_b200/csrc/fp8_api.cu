@@ -1,0 +1,76 @@
+// C entry points of the FP8 products: argument checks, workspaces and the
+// choice of kernel by size.
+#include "fp8_kernels.cuh"
+
+namespace lrb {
+namespace {
+
+size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+int check_experts(int tokens, int experts, int top_k, int hidden, int inner) {
+    LRB_REQUIRE(tokens >= 0 && experts >= 1 && experts <= 1024, "moe_experts_fp8: bad tokens %d / experts %d", tokens,
+                experts);
+    LRB_REQUIRE(top_k >= 1 && top_k <= 32, "moe_experts_fp8: top_k %d outside [1, 32]", top_k);
+    LRB_REQUIRE(hidden >= 16 && hidden % 16 == 0 && hidden <= 65536,
+                "moe_experts_fp8: hidden %d must be a multiple of 16 in [16, 65536]", hidden);
+    LRB_REQUIRE(inner >= 128 && inner % 128 == 0 && inner <= 16384,
+                "moe_experts_fp8: inner %d must be a multiple of 128 in [128, 16384]", inner);
+    LRB_REQUIRE(static_cast<int64_t>(tokens) * top_k < (1 << 30), "moe_experts_fp8: too many routes");
+    return MOE_OK;
+}
+
+}  // namespace
+}  // namespace lrb
+
+using namespace lrb;
+
+extern "C" size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols) {
+    (void)tokens, (void)rows, (void)cols;
+    return 0;
+}
+
+extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales,
+                              int tokens, int rows, int cols, void *out, int out_f32, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    LRB_REQUIRE(tokens >= 0 && rows >= 1, "moe_linear_fp8: bad tokens %d / rows %d", tokens, rows);
+    LRB_REQUIRE(cols >= 16 && cols % 16 == 0, "moe_linear_fp8: cols %d must be a positive multiple of 16", cols);
+    LRB_REQUIRE(out_f32 == 0 || out_f32 == 1, "moe_linear_fp8: out_f32 must be 0 or 1");
+    if (tokens == 0) return MOE_OK;
+    LRB_REQUIRE(x && x_scales && w && w_scales && out, "moe_linear_fp8: null tensor");
+    LRB_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scales, 4) && aligned(w_scales, 4) && aligned(out, 16),
+                "moe_linear_fp8: x, w and out must be 16-byte aligned");
+    const size_t need = moe_linear_fp8_workspace_bytes(tokens, rows, cols);
+    LRB_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need),
+                "moe_linear_fp8: workspace of %zu bytes (256-byte aligned) required", need);
+    if (int rc = require_sm100()) return rc;
+    const LinearFp8 a{x, x_scales, w, w_scales, tokens, rows, cols, out, out_f32};
+    return launch_linear_fp8_gemv(a, as_stream(stream));
+}
+
+extern "C" size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner) {
+    if (check_experts(tokens, experts, top_k, hidden, inner) != MOE_OK) return 0;
+    return align256(static_cast<size_t>(tokens) * top_k * inner * 4);
+}
+
+extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up,
+                               const float *gate_up_scales, const uint8_t *down, const float *down_scales,
+                               const int64_t *idx, const uint16_t *weights, int tokens, int experts, int top_k,
+                               int hidden, int inner, uint16_t *out, void *workspace, size_t workspace_bytes,
+                               void *stream) {
+    if (int rc = check_experts(tokens, experts, top_k, hidden, inner)) return rc;
+    if (tokens == 0) return MOE_OK;
+    LRB_REQUIRE(x && x_scales && gate_up && gate_up_scales && down && down_scales && idx && weights && out,
+                "moe_experts_fp8: null tensor");
+    LRB_REQUIRE(aligned(x, 16) && aligned(gate_up, 16) && aligned(down, 16) && aligned(x_scales, 4) &&
+                    aligned(gate_up_scales, 4) && aligned(down_scales, 4) && aligned(out, 16),
+                "moe_experts_fp8: x, the banks and out must be 16-byte aligned");
+    const size_t need = moe_experts_fp8_workspace_bytes(tokens, experts, top_k, hidden, inner);
+    LRB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need,
+                "moe_experts_fp8: workspace of %zu bytes (256-byte aligned) required", need);
+    if (int rc = require_sm100()) return rc;
+    const ExpertsFp8 a{x, x_scales, gate_up, down, gate_up_scales, down_scales, idx, weights, tokens, experts, top_k,
+                       hidden, inner, out};
+    return launch_experts_fp8_gemv(a, static_cast<float *>(workspace), as_stream(stream));
+}

@@ -1,0 +1,37 @@
+// Internal launchers of the FP8 products (fp8_gemv.cu, fp8_tc.cu, fp8_api.cu).
+#pragma once
+
+#include "fp8.cuh"
+#include "kernels.cuh"
+
+namespace lrb {
+
+// out[m, n] = sum over 128-column groups of xs[m, g] * ws[n / 128, g] * (x . w over the group)
+struct LinearFp8 {
+    const uint8_t *x;        // [tokens, cols] e4m3
+    const float *x_scales;   // [tokens, ceil(cols / 128)]
+    const uint8_t *w;        // [rows, cols] e4m3
+    const float *w_scales;   // [ceil(rows / 128), ceil(cols / 128)]
+    int tokens, rows, cols;
+    void *out;               // [tokens, rows] BF16 or FP32
+    int out_f32;
+};
+
+struct ExpertsFp8 {
+    const uint8_t *x;                 // [T, H]
+    const float *x_scales;            // [T, ceil(H / 128)]
+    const uint8_t *gate_up, *down;    // [E, 2I, H], [E, H, I]
+    const float *gate_up_scales;      // [E, 2I / 128, ceil(H / 128)]
+    const float *down_scales;         // [E, ceil(H / 128), I / 128]
+    const int64_t *idx;               // [T, K]; outside [0, E): dropped
+    const uint16_t *weights;          // [T, K] BF16
+    int tokens, experts, top_k, hidden, inner;
+    uint16_t *out;                    // [T, H] BF16
+};
+
+constexpr int kGemvTokens = 4;  // tokens per pass of the linear GEMV
+int launch_linear_fp8_gemv(const LinearFp8 &a, cudaStream_t stream);
+// h: FP32 [T * K, I] scratch
+int launch_experts_fp8_gemv(const ExpertsFp8 &a, float *h, cudaStream_t stream);
+
+}  // namespace lrb

@@ -1,0 +1,113 @@
+"""Refusals of the FP8 entry points before any device use (CPU only)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from lightreason_b200 import build, fp8, native
+
+E4M3 = torch.float8_e4m3fn
+P = ctypes.c_void_p
+
+
+@pytest.fixture(scope="module")
+def so():
+    build.build()
+    return native.lib()
+
+
+def refused(so, rc, text):
+    assert rc == native.MOE_EINVAL
+    assert text.encode() in so.moe_last_error(), so.moe_last_error()
+
+
+def test_rows_refusals(so):
+    ok = P(1 << 20)
+
+    def call(x=ok, xs=256, res=None, rs=256, w=ok, eps=1e-6, tokens=4, hidden=256, q=ok, s=ok, normed=None, r=None):
+        return so.moe_rmsnorm_fp8(x, xs, res, rs, w, 1.0, eps, tokens, hidden, q, s, normed, r, None)
+
+    refused(so, call(hidden=0), "bad tokens")
+    refused(so, call(tokens=-1), "bad tokens")
+    refused(so, call(xs=255), "row strides")
+    refused(so, call(res=ok, rs=8), "row strides")
+    refused(so, call(r=ok), "residual_out without residual")
+    refused(so, call(w=None, res=ok), "without a norm weight")
+    refused(so, call(w=None, normed=ok), "without a norm weight")
+    refused(so, call(q=None), "null tensor")
+    refused(so, call(eps=-1.0), "eps")
+    refused(so, call(eps=float("nan")), "eps")
+    assert call(tokens=0, x=None, q=None, s=None) == native.MOE_OK
+
+
+def test_blocks_refusals(so):
+    ok = P(1 << 20)
+    refused(so, so.moe_quantize_fp8_blocks(ok, 1, 0, 4, ok, ok, None), "bad shape")
+    refused(so, so.moe_quantize_fp8_blocks(ok, -1, 4, 4, ok, ok, None), "bad shape")
+    refused(so, so.moe_quantize_fp8_blocks(None, 1, 4, 4, ok, ok, None), "null tensor")
+    refused(so, so.moe_quantize_fp8_blocks(ok, 1 << 30, 1024, 1024, ok, ok, None), "too many blocks")
+    assert so.moe_quantize_fp8_blocks(None, 0, 4, 4, None, None, None) == native.MOE_OK
+
+
+def test_linear_refusals(so):
+    ok, bad = P(1 << 20), P((1 << 20) + 8)
+    ws = so.moe_linear_fp8_workspace_bytes
+
+    def call(x=ok, w=ok, tokens=3, rows=64, cols=256, out=ok, f32=0, work=ok, nbytes=1 << 30):
+        return so.moe_linear_fp8(x, ok, w, ok, tokens, rows, cols, out, f32, work, nbytes, None)
+
+    refused(so, call(cols=24), "multiple of 16")
+    refused(so, call(cols=0), "multiple of 16")
+    refused(so, call(rows=0), "bad tokens")
+    refused(so, call(tokens=-1), "bad tokens")
+    refused(so, call(f32=2), "out_f32")
+    refused(so, call(x=None), "null tensor")
+    for k in ("x", "w", "out"):
+        refused(so, call(**{k: bad}), "16-byte aligned")
+    for shape in ((64, 1024, 2048), (8, 512, 4096)):
+        if ws(*shape):
+            refused(so, call(tokens=shape[0], rows=shape[1], cols=shape[2], nbytes=ws(*shape) - 1), "workspace")
+    assert call(tokens=0, x=None, out=None) == native.MOE_OK
+
+
+def test_experts_refusals(so):
+    ok, bad = P(1 << 20), P((1 << 20) + 8)
+    need = so.moe_experts_fp8_workspace_bytes(3, 8, 2, 256, 128)
+    assert need > 0
+
+    def call(x=ok, gu=ok, dn=ok, idx=ok, tokens=3, experts=8, top_k=2, hidden=256, inner=128, out=ok, work=ok,
+             nbytes=need):
+        return so.moe_experts_fp8(x, ok, gu, ok, dn, ok, idx, ok, tokens, experts, top_k, hidden, inner, out, work,
+                                  nbytes, None)
+
+    refused(so, call(hidden=250), "hidden")
+    refused(so, call(inner=192), "inner")
+    refused(so, call(top_k=0), "top_k")
+    refused(so, call(top_k=33), "top_k")
+    refused(so, call(experts=0), "experts")
+    refused(so, call(experts=1025), "experts")
+    refused(so, call(tokens=-1), "tokens")
+    refused(so, call(tokens=1 << 29, top_k=8), "too many routes")
+    refused(so, call(idx=None), "null tensor")
+    for k in ("x", "gu", "dn", "out"):
+        refused(so, call(**{k: bad}), "16-byte aligned")
+    refused(so, call(nbytes=need - 1), "workspace")
+    refused(so, call(work=None), "workspace")
+    refused(so, call(work=bad), "workspace")
+    assert call(tokens=0, x=None, idx=None, out=None, work=None, nbytes=0) == native.MOE_OK
+    assert so.moe_experts_fp8_workspace_bytes(3, 8, 2, 250, 128) == 0
+
+
+def test_python_refuses_cpu_tensors_and_wrong_types():
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    q, s = torch.zeros(4, 256).to(E4M3), torch.zeros(4, 2)
+    w, ws = torch.zeros(128, 256).to(E4M3), torch.zeros(1, 2)
+    for call in (lambda: fp8.quantize_rows(x), lambda: fp8.rmsnorm_quantize(x, x[0]), lambda: fp8.quantize_blocks(x),
+                 lambda: fp8.linear(q, s, w, ws),
+                 lambda: fp8.experts(q, s, w[None], ws[None], w[None], ws[None], torch.zeros(4, 1).long(),
+                                     torch.zeros(4, 1).bfloat16())):
+        with pytest.raises(ValueError):
+            call()

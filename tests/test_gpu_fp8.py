@@ -1,0 +1,426 @@
+"""The FP8 operators on the GPU against 64-bit forms (tests/fp8_reference.py),
+elementwise, at the sizes, strides, routes and values where they can go wrong."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lightreason_b200 import build, fp8, native
+from tests import fp8_reference as R
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def dev():
+    build.build()
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    native.device_check(0)
+    return torch.device("cuda", 0)
+
+
+def gen(seed, dev):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=g.device)
+
+
+def same_e4m3(q, want, what):
+    """Equal as values (+0 and -0 alike)."""
+    bad = q.double() != want
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} e4m3 values differ"
+
+
+def within(got, want, bound, what):
+    err = (got.double() - want).abs()
+    assert torch.isfinite(got.double()).all(), f"{what}: non-finite values"
+    bad = err > bound
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside their bound; worst "
+                           f"{float((err / bound.clamp(min=1e-300)).max()):.2f} x")
+
+
+# -------------------------------------------------------------------- rows ---
+
+ROW_SHAPES = [(1, 1), (1, 7), (3, 127), (2, 128), (5, 129), (1, 2048), (4, 2048), (333, 1000), (2, 1001), (300, 256),
+              (700, 512), (200, 4096), (3, 8192), (2, 16384), (2, 16392), (1, 40000)]
+
+
+@pytest.mark.parametrize("tokens,hidden", ROW_SHAPES)
+def test_quantize_rows_is_the_exact_rounding(dev, tokens, hidden):
+    """For BF16 input every e4m3 value is the nearest one with ties to even,
+    and the scale is the FP32 value nearest to the quotient."""
+    g = gen(tokens * 7919 + hidden, dev)
+    x = (randn(g, tokens, hidden) * torch.exp(2 * randn(g, hidden))).to(torch.bfloat16)
+    q, s = fp8.quantize_rows(x)
+    _, want, scale = R.rows(x.double())
+    same_e4m3(q, want, "q")
+    assert torch.equal(s, scale.float()) and s.shape == (tokens, R.groups(hidden))
+
+
+def test_quantize_rows_ties_zeros_and_extremes(dev):
+    """Every BF16 magnitude against maxima of several exponents and mantissas:
+    zero rows, subnormals, the largest finite values, ties."""
+    every = torch.arange(0, 0x7F80, dtype=torch.int32, device=dev).to(torch.int16).view(torch.bfloat16)
+    x = torch.zeros(0x7F80 // 64 + 1, 128, dtype=torch.bfloat16, device=dev)
+    n = every.numel() // 64 * 64
+    x[:n // 64, :64] = every[:n].view(-1, 64)
+    x[:n // 64, 64:] = -every[:n].view(-1, 64)
+    # and against fixed maxima: all mantissas of one binade
+    top = torch.arange(0x3F80, 0x4000, dtype=torch.int32, device=dev).to(torch.int16).view(torch.bfloat16)
+    y = every[0x3000:0x3F80].view(-1, 31).repeat_interleave(8, 0)[:, :31]
+    z = torch.zeros(y.shape[0] * 4, 128, dtype=torch.bfloat16, device=dev)
+    z[:, :31] = y.repeat(4, 1)
+    z[:, 127] = top[torch.arange(z.shape[0], device=dev) % 128]
+    for v in (x, z):
+        q, s = fp8.quantize_rows(v)
+        _, want, scale = R.rows(v.double())
+        same_e4m3(q, want, "q")
+        assert torch.equal(s, scale.float())
+
+
+def test_quantize_rows_strided_and_unaligned(dev):
+    """Rows of a wider tensor, starting anywhere: vector and scalar paths."""
+    g = gen(3, dev)
+    wide = randn(g, 40, 700).to(torch.bfloat16)
+    for first, hidden in ((0, 512), (8, 512), (3, 512), (1, 300), (16, 320)):
+        x = wide[:, first:first + hidden]
+        q, s = fp8.quantize_rows(x)
+        qc, sc = fp8.quantize_rows(x.contiguous())
+        assert torch.equal(q.view(torch.uint8), qc.view(torch.uint8)) and torch.equal(s, sc)
+    x = wide[::3, :512]
+    assert torch.equal(fp8.quantize_rows(x)[0].view(torch.uint8),
+                       fp8.quantize_rows(x.contiguous())[0].view(torch.uint8))
+
+
+def norm_reference(x, weight, residual, eps, offset):
+    r = (x.double() + residual.double()).to(torch.bfloat16) if residual is not None else x
+    rd = r.double()
+    y = rd * torch.rsqrt(rd.square().mean(-1, keepdim=True) + eps) * (offset + weight.double())
+    return r, y
+
+
+# FP32 relative error of y: the sum of squares adds at most 8 + 5 + 64 positive
+# terms in sequence (a vector's, the warp's, the blocks of a row of 16384; the
+# scalar kernel's longest chain is 40000 / 32 / 8 + 13 = 170), halved by the
+# square root, plus eight roundings: below 128 of 2^-24; 256 allows twice that
+NORM_REL = 256 * R.F32
+
+
+def check_norm(got, x, weight, residual, eps=1e-6, offset=1.0):
+    q, s, normed, total = got
+    r, y = norm_reference(x, weight, residual, eps, offset)
+    if residual is not None:
+        assert torch.equal(total.view(torch.int16), r.view(torch.int16)), "residual_out"
+    within(normed, y, (R.BF + NORM_REL) * y.abs() + 2.0 ** -134, "normed")
+    a = R.tops(y)
+    within(s, a / R.TOP, 2 * NORM_REL * a / R.TOP, "scales")
+    v, _, _ = R.rows(y)
+    within(q, v, 0.5 * R.step(v) * (1 + 4 * NORM_REL) + 4 * NORM_REL * v.abs(), "q")
+
+
+@pytest.mark.parametrize("tokens,hidden", ROW_SHAPES)
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_rmsnorm_quantize(dev, tokens, hidden, with_residual):
+    g = gen(tokens * 31 + hidden, dev)
+    x = (3 * randn(g, tokens, hidden)).to(torch.bfloat16)
+    w = (0.5 * randn(g, hidden)).to(torch.bfloat16)
+    res = randn(g, tokens, hidden).to(torch.bfloat16) if with_residual else None
+    check_norm(fp8.rmsnorm_quantize(x, w, res), x, w, res)
+    got = fp8.rmsnorm_quantize(x, w, res, eps=1e-3, weight_offset=0.0)
+    check_norm(got, x, w, res, eps=1e-3, offset=0.0)
+
+
+def test_rmsnorm_quantize_in_place_strided_and_optional(dev):
+    """residual_out over residual and normed over x, as a model's residual
+    stream does; strided inputs; without the BF16 output."""
+    g = gen(11, dev)
+    for hidden in (2048, 1001):
+        wide = randn(g, 9, 2 * hidden + 16).to(torch.bfloat16)
+        x, res = wide[:, 8:8 + hidden], wide[:, hidden + 16:2 * hidden + 16]
+        w = randn(g, hidden).to(torch.bfloat16)
+        want = fp8.rmsnorm_quantize(x.contiguous(), w, res.contiguous())
+        got = fp8.rmsnorm_quantize(x, w, res)
+        xc, rc = x.contiguous(), res.contiguous()
+        q, s = torch.empty_like(want[0]), torch.empty_like(want[1])
+        placed = fp8.rmsnorm_quantize(xc, w, rc, out=(q, s, xc, rc))
+        bare = fp8.rmsnorm_quantize(x, w, res, normed=False)
+        assert bare[2] is None
+        for a in (got, placed):
+            for u, v in zip(a, want):
+                assert torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+        assert torch.equal(bare[0].view(torch.uint8), want[0].view(torch.uint8))
+
+
+def test_rows_with_nan_or_infinity_keep_to_themselves(dev):
+    """A group with a NaN or an infinity reads back as NaN; with the norm its
+    whole row does; other groups and rows are as without it."""
+    g = gen(12, dev)
+    for hidden in (512, 515):
+        x = randn(g, 6, hidden).to(torch.bfloat16)
+        w = randn(g, hidden).to(torch.bfloat16)
+        bad = x.clone()
+        bad[1, 130], bad[4, 3] = float("nan"), float("inf")
+        q0, s0 = fp8.quantize_rows(x)
+        q, s = fp8.quantize_rows(bad)
+        back, clean = R.widen_rows(q, s), R.widen_rows(q0, s0)
+        assert back[1, 128:256].isnan().all() and back[4, :128].isnan().all()
+        back[1, 128:256], back[4, :128] = clean[1, 128:256], clean[4, :128]
+        assert torch.equal(back, clean)
+        q0, s0, y0, _ = fp8.rmsnorm_quantize(x, w)
+        q, s, y, _ = fp8.rmsnorm_quantize(bad, w)
+        assert R.widen_rows(q, s)[1].isnan().all() and y[1].isnan().all()
+        # r / inf is 0 for the finite values of a row with an infinity, NaN at it
+        assert y[4, 3].isnan() and R.widen_rows(q, s)[4, :128].isnan().all()
+        keep = [0, 2, 3, 5]
+        assert torch.equal(y[keep], y0[keep]) and torch.equal(s[keep], s0[keep])
+        assert torch.equal(q[keep].view(torch.uint8), q0[keep].view(torch.uint8))
+
+
+def test_rows_past_32_bit_offsets(dev):
+    """More than 2^31 values: the last rows come out as they do alone."""
+    tokens, hidden = (1 << 31) // 2048 + 5, 2048
+    x = torch.zeros(tokens, hidden, dtype=torch.bfloat16, device=dev)
+    x[-3:] = randn(gen(5, dev), 3, hidden).to(torch.bfloat16)
+    w = torch.zeros(hidden, dtype=torch.bfloat16, device=dev)
+    q, s = fp8.quantize_rows(x)
+    qa, sa = fp8.quantize_rows(x[-3:].clone())
+    assert torch.equal(q[-3:].view(torch.uint8), qa.view(torch.uint8)) and torch.equal(s[-3:], sa)
+    q, s, y, _ = fp8.rmsnorm_quantize(x, w)
+    qa, sa, ya, _ = fp8.rmsnorm_quantize(x[-3:].clone(), w)
+    assert torch.equal(q[-3:].float(), qa.float()) and torch.equal(y[-3:], ya)
+    del x, q, s, y
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ blocks ---
+
+@pytest.mark.parametrize("shape", [(1, 1), (128, 128), (129, 127), (1000, 2000), (64, 72), (3, 260, 392), (2, 257, 100),
+                                   (5, 1, 3), (4, 256, 512)])
+def test_quantize_blocks_is_the_exact_rounding(dev, shape):
+    g = gen(sum(shape), dev)
+    w = (0.02 * randn(g, *shape)).to(torch.bfloat16)
+    q, s = fp8.quantize_blocks(w)
+    want, scale = R.blocks(w.double())
+    same_e4m3(q, want, "q")
+    assert s.shape == scale.shape and torch.equal(s, scale.float())
+
+
+def test_quantize_blocks_past_32_bit_offsets(dev):
+    w = torch.zeros(1025, 1024, 2048, dtype=torch.bfloat16, device=dev)
+    w[-1] = randn(gen(6, dev), 1024, 2048).to(torch.bfloat16)
+    q, s = fp8.quantize_blocks(w)
+    qa, sa = fp8.quantize_blocks(w[-1].clone())
+    assert torch.equal(q[-1].view(torch.uint8), qa.view(torch.uint8)) and torch.equal(s[-1], sa)
+    del w, q, s
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ linear ---
+
+def linear_case(dev, tokens, rows, cols, seed=0):
+    g = gen(seed + tokens * 131 + rows * 17 + cols, dev)
+    x, xs = fp8.quantize_rows(randn(g, tokens, cols).to(torch.bfloat16))
+    w, ws = fp8.quantize_blocks((0.05 * randn(g, rows, cols)).to(torch.bfloat16))
+    return x, xs, w, ws
+
+
+LINEAR_SHAPES = [(1, 1, 16), (1, 1024, 2048), (2, 100, 144), (3, 130, 2064), (4, 128, 128), (5, 257, 272),
+                 (7, 1000, 1040), (16, 512, 512), (17, 2048, 512), (33, 129, 4096), (64, 1024, 2048), (77, 1000, 1040),
+                 (127, 384, 640), (128, 256, 128), (129, 640, 256), (200, 2050, 336), (256, 8192, 256),
+                 (300, 72, 1024), (513, 1024, 1168), (1000, 511, 2048), (2048, 2048, 512), (1, 8200, 16),
+                 (300, 3, 48), (6, 20000, 128)]
+
+
+@pytest.mark.parametrize("tokens,rows,cols", LINEAR_SHAPES)
+def test_linear(dev, tokens, rows, cols):
+    x, xs, w, ws = linear_case(dev, tokens, rows, cols)
+    want, bound = R.linear(x, xs, w, ws)
+    within(fp8.linear(x, xs, w, ws, out_dtype=torch.float32), want, bound + R.F32 * want.abs(), "f32")
+    within(fp8.linear(x, xs, w, ws), want, bound + R.BF * (want.abs() + bound), "bf16")
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 40, 300])
+def test_linear_rows_and_outside_are_left_alone(dev, tokens):
+    """Rows around the output stay as they were; a row with NaN stays alone."""
+    x, xs, w, ws = linear_case(dev, tokens, 264, 400)
+    store = torch.full((tokens + 2, 264), 7.0, dtype=torch.bfloat16, device=dev)
+    fp8.linear(x, xs, w, ws, out=store[1:-1])
+    want = fp8.linear(x, xs, w, ws)
+    assert torch.equal(store[1:-1], want) and (store[0] == 7).all() and (store[-1] == 7).all()
+    xs = xs.clone()
+    xs[tokens // 2, 1] = float("nan")
+    got = fp8.linear(x, xs, w, ws)
+    assert got[tokens // 2].isnan().all()
+    keep = torch.arange(tokens, device=dev) != tokens // 2
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_linear_is_deterministic(dev):
+    for shape in ((64, 1024, 2048), (9, 512, 4096), (700, 1024, 1024)):
+        x, xs, w, ws = linear_case(dev, *shape)
+        first = fp8.linear(x, xs, w, ws, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(fp8.linear(x, xs, w, ws, out_dtype=torch.float32), first)
+
+
+# ----------------------------------------------------------------- experts ---
+
+def experts_case(dev, tokens, count, top_k, hidden, inner, seed=0, routes="random"):
+    g = gen(seed + tokens * 3 + count * 5 + hidden, dev)
+    x, xs = fp8.quantize_rows(randn(g, tokens, hidden).to(torch.bfloat16))
+    gu, gus = fp8.quantize_blocks((0.05 * randn(g, count, 2 * inner, hidden)).to(torch.bfloat16))
+    dn, dns = fp8.quantize_blocks((0.05 * randn(g, count, hidden, inner)).to(torch.bfloat16))
+    if routes == "random":
+        idx = torch.rand(tokens, count, generator=g, device=dev).topk(top_k, -1)[1]
+    elif routes == "same":        # every route of every token: one expert
+        idx = torch.full((tokens, top_k), count - 1, device=dev)
+    else:                         # "dropped": ids on every side of the range, whole tokens without a route
+        idx = torch.randint(-2, count + 2, (tokens, top_k), generator=g, device=dev)
+        idx[::3] = torch.tensor([-1, count, 1 << 40, -(1 << 40)], device=dev)[torch.arange(top_k, device=dev) % 4]
+    weights = torch.softmax(randn(g, tokens, top_k), -1).to(torch.bfloat16)
+    return x, xs, gu, gus, dn, dns, idx.contiguous(), weights
+
+
+EXPERT_SHAPES = [(1, 8, 2, 256, 128), (1, 32, 8, 2048, 512), (2, 4, 4, 144, 128), (3, 16, 5, 400, 256),
+                 (5, 64, 8, 2048, 512), (16, 32, 8, 1024, 256), (17, 16, 8, 2048, 512), (33, 4, 2, 16, 128),
+                 (64, 1, 1, 128, 128), (65, 3, 3, 2064, 384), (130, 8, 2, 272, 256), (300, 6, 4, 1104, 128),
+                 (700, 5, 2, 512, 640), (1500, 12, 8, 512, 256), (12, 40, 12, 640, 128), (1, 40, 32, 256, 256)]
+
+
+@pytest.mark.parametrize("tokens,count,top_k,hidden,inner", EXPERT_SHAPES)
+def test_experts(dev, tokens, count, top_k, hidden, inner):
+    c = experts_case(dev, tokens, count, top_k, hidden, inner)
+    want, bound = R.experts(*c)
+    within(fp8.experts(*c), want, bound, "out")
+
+
+@pytest.mark.parametrize("tokens,count,top_k,hidden,inner", [(1, 4, 8, 256, 128), (7, 4, 6, 272, 256),
+                                                             (40, 8, 8, 512, 128), (400, 20, 8, 528, 256)])
+@pytest.mark.parametrize("routes", ["same", "dropped"])
+def test_experts_skewed_and_dropped_routes(dev, tokens, count, top_k, hidden, inner, routes):
+    """All routes on one expert (the same id several times in a token), and
+    ids outside the bank, tokens with none left among them: those are zero."""
+    c = experts_case(dev, tokens, count, top_k, hidden, inner, routes=routes)
+    want, bound = R.experts(*c)
+    got = fp8.experts(*c)
+    within(got, want, bound, "out")
+    if routes == "dropped":
+        assert (got[::3] == 0).all()
+        nothing = torch.full_like(c[6], -1)
+        assert (fp8.experts(*c[:6], nothing, c[7]) == 0).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 90, 600])
+def test_experts_nan_row_keeps_to_itself(dev, tokens):
+    c = list(experts_case(dev, tokens, 8, 3, 512, 256))
+    store = torch.full((tokens + 2, 512), 7.0, dtype=torch.bfloat16, device=dev)
+    want = fp8.experts(*c)
+    fp8.experts(*c, out=store[1:-1])
+    assert torch.equal(store[1:-1], want) and (store[0] == 7).all() and (store[-1] == 7).all()
+    xs = c[1].clone()
+    xs[tokens // 2, 0] = float("inf")
+    got = fp8.experts(c[0], xs, *c[2:])
+    assert not torch.isfinite(got[tokens // 2]).any()
+    keep = torch.arange(tokens, device=dev) != tokens // 2
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_experts_bank_past_32_bit_offsets(dev):
+    """Banks of more than 2^32 bytes: the last experts as in banks of their own."""
+    count, inner, hidden = 700, 1536, 2048
+    c = experts_case(dev, 24, 2, 2, hidden, inner)
+    gu = torch.zeros(count, 2 * inner, hidden, dtype=torch.uint8, device=dev).view(E4M3)
+    dn = torch.zeros(count, hidden, inner, dtype=torch.uint8, device=dev).view(E4M3)
+    gus, dns = (torch.zeros(count, *s.shape[1:], device=dev) for s in (c[3], c[5]))
+    for big, small in ((gu.view(torch.uint8), c[2].view(torch.uint8)), (gus, c[3]),
+                       (dn.view(torch.uint8), c[4].view(torch.uint8)), (dns, c[5])):
+        big[-2:] = small
+    for tokens in (1, 24):
+        x, xs, idx, wt = c[0][:tokens], c[1][:tokens], c[6][:tokens], c[7][:tokens]
+        want = fp8.experts(x, xs, c[2], c[3], c[4], c[5], idx, wt)
+        got = fp8.experts(x, xs, gu, gus, dn, dns, idx + count - 2, wt)
+        assert torch.equal(got, want)
+    del gu, dn
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------ how it is run ---
+
+def test_empty_batch(dev):
+    x = torch.empty(0, 256, dtype=torch.bfloat16, device=dev)
+    q, s = fp8.quantize_rows(x)
+    assert q.shape == (0, 256) and s.shape == (0, 2)
+    assert fp8.rmsnorm_quantize(x, torch.zeros(256, dtype=torch.bfloat16, device=dev), x)[3].shape == (0, 256)
+    c = experts_case(dev, 2, 4, 2, 256, 128)
+    assert fp8.linear(q, s, c[2][0], c[3][0]).shape == (0, 256)
+    assert fp8.experts(q, s, *c[2:6], c[6][:0], c[7][:0]).shape == (0, 256)
+
+
+def chain_of_calls(x, res, w, c):
+    """Norm, router-independent linear and experts as a layer would use them."""
+    q, s, y, r = fp8.rmsnorm_quantize(x, w, res)
+    lin = fp8.linear(q, s, c[2][0], c[3][0])
+    return q, s, y, r, lin, fp8.experts(q, s, *c[2:])
+
+
+@pytest.mark.parametrize("tokens", [1, 48, 400])
+def test_streams_and_graphs(dev, tokens):
+    """The chain on a side stream, and in two captured graphs that live (and
+    replay) together on changing inputs, equals the eager calls."""
+    c = experts_case(dev, tokens, 8, 4, 512, 256)
+    g = gen(tokens, dev)
+    w = randn(g, 512).to(torch.bfloat16)
+    ins = [(randn(g, tokens, 512).to(torch.bfloat16), randn(g, tokens, 512).to(torch.bfloat16)) for _ in range(4)]
+    want = [chain_of_calls(*i, w, c) for i in ins]
+    same = lambda a, b: all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(a, b))  # noqa: E731
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        got = [chain_of_calls(*i, w, c) for i in ins]
+    torch.cuda.current_stream(dev).wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(same(a, b) for a, b in zip(got, want))
+    graphs = []
+    for k in range(2):
+        x, r = ins[k][0].clone(), ins[k][1].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = chain_of_calls(x, r, w, c)
+        graphs.append((graph, x, r, out))
+    for first in (0, 2):
+        for k, (graph, x, r, _) in enumerate(graphs):
+            x.copy_(ins[first + k][0])
+            r.copy_(ins[first + k][1])
+        s1, s2 = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+        for s, (graph, *_) in zip((s1, s2), graphs):
+            s.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for k, (_, _, _, out) in enumerate(graphs):
+            assert same(out, want[first + k])
+
+
+def test_back_to_back_calls_with_new_weights(dev):
+    """A product right behind the kernel that writes its weights, again and
+    again into the same memory: each sees its own weights."""
+    g = gen(77, dev)
+    ws = [(0.05 * randn(g, 512, 1024)).to(torch.bfloat16) for _ in range(6)]
+    x, xs = fp8.quantize_rows(randn(g, 1, 1024).to(torch.bfloat16))
+    want = []
+    for w in ws:
+        q, s = fp8.quantize_blocks(w)
+        torch.cuda.synchronize()
+        want.append(fp8.linear(x, xs, q, s))
+        torch.cuda.synchronize()
+    out = fp8.quantize_blocks(ws[0])
+    got = []
+    for w in ws:
+        fp8.quantize_blocks(w, out=out)
+        got.append(fp8.linear(x, xs, *out))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -526,11 +526,12 @@ int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, ui
 /* out[T, rows] (BF16, or FP32 with out_f32 = 1) = x . w^T on the values that x
  * [T, cols] and w [rows, cols] stand for, products summed in FP32.  cols must
  * be a multiple of 16; x, w and out are 16-byte aligned.  The workspace query
- * may return 0: workspace may then be NULL. */
+ * may return 0: workspace may then be NULL.  status (device int32, or NULL) is
+ * set to 1 if a bounded wait inside a kernel gave up; out is then not valid. */
 size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols);
 int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
                    int rows, int cols, void *out, int out_f32, void *workspace, size_t workspace_bytes,
-                   void *stream);
+                   int32_t *status, void *stream);
 
 /* The routed experts (the Qwen3_5MoeExperts.forward contract of
  * moe_layer_forward with route_in) on e4m3 banks gate_up [E, 2I, H] and down
@@ -540,12 +541,13 @@ int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, co
  * with FP32 sums and one rounding to BF16 at the end on the smallest batches;
  * larger ones keep each route's row as BF16 before the weighted sum.  Ids
  * outside [0, E) contribute nothing (a token with none left is 0).  hidden is
- * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024. */
+ * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024.
+ * status as in moe_linear_fp8. */
 size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner);
 int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up, const float *gate_up_scales,
                     const uint8_t *down, const float *down_scales, const int64_t *idx, const uint16_t *weights,
                     int tokens, int experts, int top_k, int hidden, int inner, uint16_t *out, void *workspace,
-                    size_t workspace_bytes, void *stream);
+                    size_t workspace_bytes, int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,42 @@ int check_experts(int tokens, int experts, int top_k, int hidden, int inner) {
     return MOE_OK;
 }
 
+// Where the scratch of moe_experts_fp8 lies in its workspace.
+struct Layout {
+    bool gemv;
+    int hist_ints;
+    size_t offsets, perm_token, perm_slot, route_pos, active, counters, hist, act, act_scales, y, bytes;
+};
+Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
+    Layout l{};
+    const size_t routes = static_cast<size_t>(tokens) * top_k;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    l.gemv = routes <= kGemvRoutes;
+    if (l.gemv) {
+        take(routes * inner * 4);
+        l.bytes = at;
+        return l;
+    }
+    l.hist_ints = permute_hist_ints(tokens, top_k, experts);
+    l.offsets = take(sizeof(int32_t) * (experts + 1));
+    l.perm_token = take(sizeof(int32_t) * routes);
+    l.perm_slot = take(sizeof(int32_t) * routes);
+    l.route_pos = take(sizeof(int32_t) * routes);
+    l.active = take(sizeof(int32_t) * experts);
+    l.counters = take(sizeof(int32_t) * 2);
+    l.hist = take(sizeof(int32_t) * static_cast<size_t>(l.hist_ints));
+    l.act = take(routes * inner);
+    l.act_scales = take(routes * (inner / fp8::kGroup) * sizeof(float));
+    l.y = take(routes * hidden * 2);
+    l.bytes = at;
+    return l;
+}
+
 }  // namespace
 }  // namespace lrb
 
@@ -33,7 +69,7 @@ extern "C" size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols)
 
 extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales,
                               int tokens, int rows, int cols, void *out, int out_f32, void *workspace,
-                              size_t workspace_bytes, void *stream) {
+                              size_t workspace_bytes, int32_t *status, void *stream) {
     LRB_REQUIRE(tokens >= 0 && rows >= 1, "moe_linear_fp8: bad tokens %d / rows %d", tokens, rows);
     LRB_REQUIRE(cols >= 16 && cols % 16 == 0, "moe_linear_fp8: cols %d must be a positive multiple of 16", cols);
     LRB_REQUIRE(out_f32 == 0 || out_f32 == 1, "moe_linear_fp8: out_f32 must be 0 or 1");
@@ -46,19 +82,20 @@ extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uin
                 "moe_linear_fp8: workspace of %zu bytes (256-byte aligned) required", need);
     if (int rc = require_sm100()) return rc;
     const LinearFp8 a{x, x_scales, w, w_scales, tokens, rows, cols, out, out_f32};
-    return launch_linear_fp8_gemv(a, as_stream(stream));
+    if (tokens <= kGemvTokens) return launch_linear_fp8_gemv(a, as_stream(stream));
+    return launch_linear_fp8_tiles(a, status, as_stream(stream));
 }
 
 extern "C" size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner) {
     if (check_experts(tokens, experts, top_k, hidden, inner) != MOE_OK) return 0;
-    return align256(static_cast<size_t>(tokens) * top_k * inner * 4);
+    return layout(tokens, experts, top_k, hidden, inner).bytes;
 }
 
 extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up,
                                const float *gate_up_scales, const uint8_t *down, const float *down_scales,
                                const int64_t *idx, const uint16_t *weights, int tokens, int experts, int top_k,
                                int hidden, int inner, uint16_t *out, void *workspace, size_t workspace_bytes,
-                               void *stream) {
+                               int32_t *status, void *stream) {
     if (int rc = check_experts(tokens, experts, top_k, hidden, inner)) return rc;
     if (tokens == 0) return MOE_OK;
     LRB_REQUIRE(x && x_scales && gate_up && gate_up_scales && down && down_scales && idx && weights && out,
@@ -72,5 +109,13 @@ extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const ui
     if (int rc = require_sm100()) return rc;
     const ExpertsFp8 a{x, x_scales, gate_up, down, gate_up_scales, down_scales, idx, weights, tokens, experts, top_k,
                        hidden, inner, out};
-    return launch_experts_fp8_gemv(a, static_cast<float *>(workspace), as_stream(stream));
+    const Layout l = layout(tokens, experts, top_k, hidden, inner);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    if (l.gemv) return launch_experts_fp8_gemv(a, reinterpret_cast<float *>(ws), as_stream(stream));
+    auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(ws + at); };
+    const ExpertsFp8Scratch s{ints(l.offsets),  ints(l.perm_token), ints(l.perm_slot),
+                              ints(l.route_pos), ints(l.active),    ints(l.counters),
+                              l.hist_ints ? ints(l.hist) : nullptr, ws + l.act,
+                              reinterpret_cast<float *>(ws + l.act_scales), reinterpret_cast<uint16_t *>(ws + l.y)};
+    return launch_experts_fp8_tiles(a, s, status, as_stream(stream));
 }

@@ -29,9 +29,20 @@ struct ExpertsFp8 {
     uint16_t *out;                    // [T, H] BF16
 };
 
-constexpr int kGemvTokens = 4;  // tokens per pass of the linear GEMV
+constexpr int kGemvTokens = 4;   // tokens per pass of the linear GEMV
+constexpr int kGemvRoutes = 32;  // routes up to which the experts take the GEMV kernels
 int launch_linear_fp8_gemv(const LinearFp8 &a, cudaStream_t stream);
 // h: FP32 [T * K, I] scratch
 int launch_experts_fp8_gemv(const ExpertsFp8 &a, float *h, cudaStream_t stream);
+
+// The tensor-core path.  status (or null): set to 1 if a bounded wait gave up.
+struct ExpertsFp8Scratch {
+    int32_t *offsets, *perm_token, *perm_slot, *route_pos, *active, *counters, *hist;  // as moe_permute_wide
+    uint8_t *act;       // [T * K, I]
+    float *act_scales;  // [T * K, I / 128]
+    uint16_t *y;        // [T * K, H]
+};
+int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream);
+int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream);
 
 }  // namespace lrb

@@ -1156,6 +1156,22 @@ int make_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *
     return MOE_OK;
 }
 
+// The same for one-byte elements: box {128, box_rows(, 1)}.
+int make_map_u8(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                uint32_t box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return set_error(MOE_ECUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+    cuuint64_t d[3], s[2];
+    cuuint32_t box[3] = {128, box_rows, 1}, es[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) d[i] = dims[i];
+    for (int i = 0; i < rank - 1; ++i) s[i] = strides_bytes[i];
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void *>(base), d, s, box, es,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(MOE_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return MOE_OK;
+}
+
 namespace {
 
 template <int BN, bool PAIR, bool TOKM = false>

@@ -152,6 +152,9 @@ struct EpP2PArgs {
 // BF16 tensor map: dims[0] innermost, 128-byte swizzle, box {64, box_rows(, 1)}.
 int make_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
                   uint32_t box_rows);
+// The same for one-byte elements: box {128, box_rows(, 1)}.
+int make_map_u8(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                uint32_t box_rows);
 // part != null: FP32 partials [ks][T][E] (router_select sums them); else BF16 logits.
 int launch_router_tc(const uint16_t *x, const uint16_t *router, int tokens, int hidden, int experts,
                      uint16_t *logits, float *part, int ks, int32_t *error, cudaStream_t stream);

@@ -152,10 +152,12 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
 
 
 def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *,
-           out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+           out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+           status: torch.Tensor | None = None) -> torch.Tensor:
     """x [T, K] . w [N, K]^T on the values that the e4m3 tensors and their
     scales stand for -> [T, N] in BF16 or FP32 (out_dtype, or out's).  K must be
-    a multiple of 16."""
+    a multiple of 16.  status: a device int32 [1] that becomes 1 if a bounded
+    wait inside a kernel gave up (the output is then not valid)."""
     _require(x.is_cuda and x.dim() == 2 and w.dim() == 2, "x and w must be CUDA [T, K] and [N, K] tensors")
     (tokens, cols), rows, dev = x.shape, w.shape[0], x.device
     _require(rows >= 1 and cols >= 16 and cols % 16 == 0, "K must be a positive multiple of 16 and N positive")
@@ -169,22 +171,25 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
     else:
         _require(out.dtype in (torch.bfloat16, torch.float32), "out must be BF16 or FP32")
         _check(out, "out", out.dtype, (tokens, rows), dev)
+    if status is not None:
+        _check(status, "status", torch.int32, (1,), dev)
     so = native.lib()
     ws = _workspace(so.moe_linear_fp8_workspace_bytes(tokens, rows, cols), dev)
     with _on(dev):
         native.check(so.moe_linear_fp8(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), tokens,
                                        rows, cols, out.data_ptr(), int(out.dtype == torch.float32), native._ptr(ws),
-                                       ws.numel() if ws is not None else 0, native._stream(dev)), "moe_linear_fp8")
+                                       ws.numel() if ws is not None else 0, native._ptr(status), native._stream(dev)),
+                     "moe_linear_fp8")
     return out
 
 
 def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate_up_scales: torch.Tensor,
             down: torch.Tensor, down_scales: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, *,
-            out: torch.Tensor | None = None) -> torch.Tensor:
+            out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """The routed experts on FP8 banks: x e4m3 [T, H] with its scales, gate_up
     [E, 2I, H] and down [E, H, I] with their block scales, idx int64 [T, K]
     (ids outside [0, E) contribute nothing), weights BF16 [T, K] -> BF16 [T, H].
-    H is a multiple of 16, I of 128."""
+    H is a multiple of 16, I of 128.  status as in linear."""
     _require(x.is_cuda and x.dim() == 2 and gate_up.dim() == 3 and down.dim() == 3 and idx.dim() == 2,
              "expected x [T, H], gate_up [E, 2I, H], down [E, H, I] and idx [T, K] on a CUDA device")
     (tokens, hidden), dev = x.shape, x.device
@@ -200,6 +205,8 @@ def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate
     if out is None:
         out = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=dev)
     _check(out, "out", torch.bfloat16, (tokens, hidden), dev)
+    if status is not None:
+        _check(status, "status", torch.int32, (1,), dev)
     so = native.lib()
     ws = _workspace(so.moe_experts_fp8_workspace_bytes(tokens, count, top_k, hidden, inner), dev)
     with _on(dev):
@@ -207,5 +214,5 @@ def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate
                                         gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(),
                                         idx.data_ptr(), weights.data_ptr(), tokens, count, top_k, hidden, inner,
                                         out.data_ptr(), native._ptr(ws), ws.numel() if ws is not None else 0,
-                                        native._stream(dev)), "moe_experts_fp8")
+                                        native._ptr(status), native._stream(dev)), "moe_experts_fp8")
     return out

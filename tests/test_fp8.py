@@ -57,7 +57,7 @@ def test_linear_refusals(so):
     ws = so.moe_linear_fp8_workspace_bytes
 
     def call(x=ok, w=ok, tokens=3, rows=64, cols=256, out=ok, f32=0, work=ok, nbytes=1 << 30):
-        return so.moe_linear_fp8(x, ok, w, ok, tokens, rows, cols, out, f32, work, nbytes, None)
+        return so.moe_linear_fp8(x, ok, w, ok, tokens, rows, cols, out, f32, work, nbytes, None, None)
 
     refused(so, call(cols=24), "multiple of 16")
     refused(so, call(cols=0), "multiple of 16")
@@ -81,7 +81,7 @@ def test_experts_refusals(so):
     def call(x=ok, gu=ok, dn=ok, idx=ok, tokens=3, experts=8, top_k=2, hidden=256, inner=128, out=ok, work=ok,
              nbytes=need):
         return so.moe_experts_fp8(x, ok, gu, ok, dn, ok, idx, ok, tokens, experts, top_k, hidden, inner, out, work,
-                                  nbytes, None)
+                                  nbytes, None, None)
 
     refused(so, call(hidden=250), "hidden")
     refused(so, call(inner=192), "inner")

@@ -56,6 +56,13 @@ __device__ __forceinline__ uint32_t pack4(const Divisor &f, float a, float b, fl
     return pack2(f(a), f(b)) | (pack2(f(c), f(d)) << 16);
 }
 
+// Two FP32 values as packed BF16 in one conversion (two separate ones and a
+// merge run at an eighth of the rate).
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // Two e4m3 values (the low 16 bits) as FP32; exact.
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);

@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(256) row_kernel(RowArgs a) {
             float p[8], r[8];
             unpack8(v[j], p);
             unpack8(add[j], r);
-            v[j] = make_uint4(pack_bf16x2(p[0] + r[0], p[1] + r[1]), pack_bf16x2(p[2] + r[2], p[3] + r[3]),
-                              pack_bf16x2(p[4] + r[4], p[5] + r[5]), pack_bf16x2(p[6] + r[6], p[7] + r[7]));
+            v[j] = make_uint4(fp8::pack_bf16(p[0] + r[0], p[1] + r[1]), fp8::pack_bf16(p[2] + r[2], p[3] + r[3]),
+                              fp8::pack_bf16(p[4] + r[4], p[5] + r[5]), fp8::pack_bf16(p[6] + r[6], p[7] + r[7]));
         }
         if (a.residual_out) {
             uint4 *dst = reinterpret_cast<uint4 *>(a.residual_out + static_cast<int64_t>(t) * a.hidden);
@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(256) row_kernel(RowArgs a) {
             for (int c = 0; c < 8; ++c) y[c] = y[c] * inv * (a.offset + w[c]);
             if (a.normed && row && u < units)
                 *reinterpret_cast<uint4 *>(a.normed + static_cast<int64_t>(t) * a.hidden + u * 8) =
-                    make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                               pack_bf16x2(y[6], y[7]));
+                    make_uint4(fp8::pack_bf16(y[0], y[1]), fp8::pack_bf16(y[2], y[3]), fp8::pack_bf16(y[4], y[5]),
+                               fp8::pack_bf16(y[6], y[7]));
         }
         float top = fp8::kTiny;
         if (u < units) {

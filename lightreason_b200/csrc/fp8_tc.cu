@@ -16,13 +16,19 @@
 // thread, and a partial tile's missing rows cost no epilogue work (whole warps
 // skip).  A stage is one group: 256 weight rows (32 KB, two boxes) and the
 // tile's rows (gathered by TMA from the token rows for gate/up, in boxes of 16
-// when the tile is partial), four stages deep: 128 KB of weights in flight per
+// when the tile is partial), three stages deep: 96 KB of weights in flight per
 // SM, which is what streams the banks at small and middle widths, where the
 // M = 128 products on padding are hidden under the weight stream.
 //
-// Warps: 0 TMA, 1 MMA, 2 the scales (a ring of eight groups in shared memory,
-// so that no epilogue thread waits for a scale), 3-10 epilogue.  Every wait is
-// bounded; a timeout raises *status, drains what is in flight and returns.
+// What bounds it at large widths: the four products of a group take 647 cycles
+// of the tensor core, and reading the group's 128 KB of sums out of TMEM takes
+// 228 more from it (both run alone at 647 and 385, together at 875 a group).
+//
+// Warps: 0 weight tiles, 1 MMA, 2 and 3 row tiles and scales (four groups at a
+// time, up to four such requests in flight), 4-11 epilogue; the first four hand registers to the
+// others (104 and 200 a thread of 168 at launch, 64,512 a CTA either way).
+// Every wait is bounded; a timeout raises *status, drains what is in flight and
+// returns.
 #include <algorithm>
 
 #include "fp8_kernels.cuh"
@@ -34,28 +40,29 @@ namespace {
 using fp8::kGroup;
 
 constexpr int kBM = 128, kBN = 256;
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 constexpr int kATile = kBM * kGroup, kBTile = kBN * kGroup, kStage = kATile + kBTile;
-constexpr int kThreads = 11 * 32;
-constexpr int kScaleSlots = 8;
+constexpr int kThreads = 12 * 32;
+constexpr int kScaleSlots = 4;   // of four groups each
+constexpr int kPiece = 8192;     // an epilogue warp's output: 32 rows of 256 bytes
 constexpr int kMaxExperts = 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 enum Mode { kLinear, kGateUp, kDown };
 
 struct Tail {
+    float4 row_scale[kScaleSlots][kBM];
+    float4 block_scale[kScaleSlots][2];
+    float top[2][2][kBM];
     uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], sfull[kScaleSlots], sempty[kScaleSlots], half[4],
         drain;
-    float row_scale[kScaleSlots][kBM];
-    float block_scale[kScaleSlots][2];
-    float top[2][2][kBM];
     int abort;
     uint32_t tmem;
     int32_t scan[16];
     int32_t items[kMaxExperts + 1];   // first item of each expert
-    int32_t offsets[kMaxExperts + 1];  // first route of each expert
 };
-constexpr int kSmem = kStages * kStage + static_cast<int>(sizeof(Tail)) + 1024;
+constexpr int kSmem = kStages * kStage + 8 * kPiece + static_cast<int>(sizeof(Tail)) + 1024;
+static_assert(kSmem <= 232448, "shared memory of one SM");
 
 struct Params {
     const float *row_scales;      // [rows, groups]
@@ -78,21 +85,24 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
+// Bounded wait; false once the CTA has given up.  Warps that work as one (the
+// scales' and the epilogue's) do not leave on false: from then on their waits
+// return at once and they run to the end on whatever is there, together.
+// The clock (and the flag) are looked at every 256th poll only: reading the
+// global timer takes longer than most waits.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    if (sm100::mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = now_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (sm100::mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t i = 1; !sm100::mbar_try_wait(bar, parity); ++i) {
+        if (i & 255) continue;
         if (*abort) return false;
-        if ((i & 63) == 0 && now_ns() - t0 > kWaitNs) {
+        const uint64_t t = now_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitNs) {
             *abort = 1;
             return false;
         }
     }
-}
-// The same for a whole warp: every lane gets one answer.
-__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+    return true;
 }
 
 struct Item {
@@ -117,7 +127,7 @@ __device__ __forceinline__ Item decode(const Params &P, const Tail *tail, int it
             if (tail->items[mid] <= item) lo = mid;
             else hi = mid;
         }
-        const int begin = tail->offsets[lo], count = tail->offsets[lo + 1] - begin;
+        const int begin = P.offsets[lo], count = P.offsets[lo + 1] - begin;
         const int mt = (count + kBM - 1) / kBM, at = item - tail->items[lo];
         r.e = lo;
         r.n = at / mt;
@@ -127,6 +137,15 @@ __device__ __forceinline__ Item decode(const Params &P, const Tail *tail, int it
         r.shared_tiles = mt > 1;
     }
     return r;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(sm100::smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+// This thread arrives on `bar` once its copies so far are complete.
+__device__ __forceinline__ void copy_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
 
 // Completes this warp's TMEM loads; the values pass through, so no use of them
@@ -139,25 +158,60 @@ __device__ __forceinline__ void wait_ld16(float (&v)[16]) {
                  : "memory");
 }
 
-__device__ __forceinline__ void store32(void *p, const uint32_t (&v)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
+// A warp's 32 rows of 64 bytes, one row a lane, to global memory as whole
+// 64-byte pieces: through 2 KB of shared memory, four lanes a row (a store of
+// 16 bytes per lane to 32 rows at once costs a pass of the load/store unit for
+// each row).  The 16-byte units of a row are permuted by its number, so neither
+// side has bank conflicts.  Rows from `rows` on, and units from `units` on, are
+// not stored.
+__device__ __forceinline__ void store_rows64(uint8_t *buf, const uint32_t (&v)[16], uint8_t *dst, int64_t pitch,
+                                             int rows, int units) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();  // the previous piece has been read
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint4 *>(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) * 16)) =
+            make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+    __syncwarp();
+    const int u = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = (lane >> 2) + 8 * i;
+        const uint4 w = *reinterpret_cast<const uint4 *>(buf + r * 64 + ((u ^ ((r >> 1) & 3)) * 16));
+        if (r < rows && u < units) *reinterpret_cast<uint4 *>(dst + r * pitch + u * 16) = w;
+    }
+}
+
+// x / (1 + exp(-x)) from the fast exponential and quotient: off by 2^-24 times
+// (4 + 1.2 |x|) of the value at most, below what the FP32 sums behind x leave.
+__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+
+// A warp's 32 rows of 256 bytes (128 BF16 columns), one row a lane, staged for
+// two TMA stores of 128 bytes a row under the 128-byte swizzle.
+__device__ __forceinline__ void stage_row256(uint8_t *buf, const float (&acc)[128]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+        *reinterpret_cast<uint4 *>(buf + (u >> 3) * 4096 + lane * 128 + (((u & 7) ^ (lane & 7)) * 16)) =
+            make_uint4(fp8::pack_bf16(acc[8 * u], acc[8 * u + 1]), fp8::pack_bf16(acc[8 * u + 2], acc[8 * u + 3]),
+                       fp8::pack_bf16(acc[8 * u + 4], acc[8 * u + 5]), fp8::pack_bf16(acc[8 * u + 6], acc[8 * u + 7]));
 }
 
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x16,
-                    const __grid_constant__ CUtensorMap tm_w, const Params P) {
+                    const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_out,
+                    const Params P) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Tail *tail = reinterpret_cast<Tail *>(smem + kStages * kStage);
+    uint8_t *pieces = smem + kStages * kStage;
+    Tail *tail = reinterpret_cast<Tail *>(pieces + 8 * kPiece);
     volatile int *abort = &tail->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            sm100::mbar_init(&tail->full[s], 1);
+            sm100::mbar_init(&tail->full[s], MODE == kGateUp ? 3 : 2);  // the warps that load into it
             sm100::mbar_init(&tail->empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -165,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             sm100::mbar_init(&tail->tempty[b], 8);
         }
         for (int s = 0; s < kScaleSlots; ++s) {
-            sm100::mbar_init(&tail->sfull[s], 1);
+            sm100::mbar_init(&tail->sfull[s], MODE == kGateUp ? 64 : 32);  // lanes
             sm100::mbar_init(&tail->sempty[s], 8);
         }
         for (int q = 0; q < 4; ++q) sm100::mbar_init(&tail->half[q], 2);
@@ -192,20 +246,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (MODE == kLinear) {
         total = nt * ((P.rows + kBM - 1) / kBM);
     } else {
-        // items[e]: an exclusive scan of the experts' tile counts, three
+        // items[e]: an exclusive scan of the experts' tile counts, a few
         // neighbouring experts a thread
-        constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
+        constexpr int kPer = (kMaxExperts + kThreads) / kThreads;
         int tiles[kPer], sum = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int e = threadIdx.x * kPer + i;
-            tiles[i] = 0;
-            if (e < P.experts) {
-                const int begin = P.offsets[e], end = P.offsets[e + 1];
-                tail->offsets[e] = begin;
-                if (e == P.experts - 1) tail->offsets[P.experts] = end;
-                tiles[i] = nt * ((end - begin + kBM - 1) / kBM);
-            }
+            tiles[i] = e < P.experts ? nt * ((P.offsets[e + 1] - P.offsets[e] + kBM - 1) / kBM) : 0;
             sum += tiles[i];
         }
         int incl = sum;
@@ -228,190 +276,230 @@ __global__ void __launch_bounds__(kThreads, 1)
         total = tail->items[P.experts];
     }
 
-    if (warp == 0) {
-        // ------------------------------------------------------ TMA producer
-        sm100::fence_proxy_async_global();
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+      if (warp == 0) {
+        // ------------------------------------------------------ weight tiles
         const uint64_t once = sm100::l2_evict_first_policy(), keep = sm100::l2_evict_normal_policy();
+        const bool one = sm100::elect_one();
         uint32_t stage = 0, phase = 0;
-        uint32_t issued = 0, parity = 0;  // bit per stage
         bool ok = true;
         for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
             const Item it = decode<MODE>(P, tail, item);
-            int tok[4];
-            if constexpr (MODE == kGateUp) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tok[i] = P.row_token[it.row0 + min(4 * lane + i, it.count - 1)];
-            }
-            // lanes that load: four rows each (gathered), or a box each
-            const int boxes = MODE == kGateUp ? (it.count + 3) / 4 : it.count == kBM ? 1 : (it.count + 15) / 16;
-            const int box_bytes = MODE == kGateUp ? 4 * kGroup : it.count == kBM ? kATile : 16 * kGroup;
             const uint64_t policy = it.shared_tiles ? keep : once;
             for (int kb = 0; kb < kbs; ++kb) {
-                if (!wait_warp(&tail->empty[stage], phase ^ 1, abort)) {
-                    ok = false;
-                    break;
-                }
-                uint8_t *a = smem + stage * kStage, *b = a + kATile;
+                ok = __all_sync(0xffffffffu, wait_bar(&tail->empty[stage], phase ^ 1, abort));
+                if (!ok) break;
+                uint8_t *b = smem + stage * kStage + kATile;
                 uint64_t *bar = &tail->full[stage];
-                if (lane == 0) {
-                    sm100::mbar_expect_tx(bar, kBTile + boxes * box_bytes);
+                const int r0 = MODE == kGateUp ? it.n * kGroup : it.n * kBN;
+                const int r1 = MODE == kGateUp ? P.n + r0 : r0 + 128;
+                if (one) {
+                    sm100::mbar_expect_tx(bar, kBTile);
                     if constexpr (MODE == kLinear) {
-                        sm100::tma_load_2d_hint(b, &tm_w, bar, kb * kGroup, it.n * kBN, policy);
-                        sm100::tma_load_2d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, it.n * kBN + 128, policy);
+                        sm100::tma_load_2d_hint(b, &tm_w, bar, kb * kGroup, r0, policy);
+                        sm100::tma_load_2d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, policy);
                     } else {
-                        const int r0 = MODE == kGateUp ? it.n * kGroup : it.n * kBN;
-                        const int r1 = MODE == kGateUp ? P.n + r0 : r0 + 128;
                         sm100::tma_load_3d_hint(b, &tm_w, bar, kb * kGroup, r0, it.e, policy);
                         sm100::tma_load_3d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, it.e, policy);
                     }
                 }
                 __syncwarp();
-                if (lane < boxes) {
-                    if constexpr (MODE == kGateUp)
-                        sm100::tma_gather4(a + lane * box_bytes, &tm_x, bar, kb * kGroup, tok);
-                    else
-                        sm100::tma_load_2d(a + lane * box_bytes, it.count == kBM ? &tm_x : &tm_x16, bar, kb * kGroup,
-                                           it.row0 + lane * 16);
-                }
-                issued |= 1u << stage;
-                parity = (parity & ~(1u << stage)) | (phase << stage);
                 if (++stage == kStages) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
         }
-        if (*abort) {
-            // let every load land before the CTA leaves
-            for (int s = 0; s < kStages; ++s) {
-                if (!(issued >> s & 1)) continue;
-                const uint64_t t0 = now_ns();
-                while (!sm100::mbar_try_wait(&tail->full[s], parity >> s & 1) && now_ns() - t0 < kWaitNs) {
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // --------------------------------------------------------- MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
-            uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
-            bool ok = true, any = false;
-            for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-                for (int kb = 0; kb < kbs; ++kb) {
-                    if (!wait_bar(&tail->tempty[buf], bphase ^ 1, abort) ||
-                        !wait_bar(&tail->full[stage], phase, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    sm100::tc_fence_after();
-                    const uint32_t base = sm100::smem_u32(smem + stage * kStage);
-                    const uint64_t a = sm100::desc_kmajor_sw128(base), b = sm100::desc_kmajor_sw128(base + kATile);
+      } else if (warp >= 2) {
+        // --------------------------------------------- row tiles and scales
+        // gate/up: warp 2 has the tile's first 64 rows, warp 3 the others, four
+        // rows a lane: gathered one instruction a lane (they issue one after
+        // another, so two warps halve that time), and the lanes' scales.
+        // Otherwise warp 2 loads the rows (one box, or 16-row boxes one a
+        // lane) and warp 3 all scales, four rows a lane.
+        constexpr bool kGather = MODE == kGateUp;
+        const bool loads = kGather || warp == 2, scales = kGather || warp == 3;
+        const int r0 = kGather ? 64 * (warp - 2) + 4 * lane : 4 * lane;
+        const bool mine = !kGather || lane < 16;
+        sm100::fence_proxy_async_global();
+        uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
+        auto rows_of = [&](const Item &it, int (&row)[4]) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        sm100::mma_e4m3(tmem + buf * kBN, a + 2 * kk, b + 2 * kk, idesc, kk != 0);
-                    sm100::mma_commit(&tail->empty[stage]);
-                    sm100::mma_commit(&tail->tfull[buf]);
-                    any = true;
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                    buf ^= 1;
-                    bphase ^= buf == 0;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int r = it.row0 + min(r0 + i, it.count - 1);
+                row[i] = kGather ? P.row_token[r] : r;
             }
-            if (*abort && any) {
-                sm100::mma_commit(&tail->drain);
-                const uint64_t t0 = now_ns();
-                while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
-                }
-            }
-        }
-        __syncwarp();
-    } else if (warp == 2) {
-        // ------------------------------------------------------------- scales
-        uint32_t slot = 0, phase = 0;
-        bool ok = true;
-        for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-            const Item it = decode<MODE>(P, tail, item);
-            const float *src[4];
+        };
+        const bool quads = kbs % 4 == 0 && (reinterpret_cast<uintptr_t>(P.row_scales) & 15) == 0 &&
+                           (reinterpret_cast<uintptr_t>(P.block_scales) & 15) == 0;
+        // the scales of groups kb .. kb + 3 to `slot`, on their way when this
+        // returns: up to kScaleSlots such requests are in flight
+        auto copy4 = [&](float4 *dst, const float *src, int kb) {
+            if (quads) {
+                copy_async<16>(dst, src + kb);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = min(lane + 32 * j, it.count - 1);
-                const int64_t row = MODE == kGateUp ? P.row_token[it.row0 + r] : it.row0 + r;
-                src[j] = P.row_scales + row * kbs;
+                for (int i = 0; i < 4; ++i)
+                    if (kb + i < kbs) copy_async<4>(reinterpret_cast<float *>(dst) + i, src + kb + i);
+            }
+        };
+        auto request_scales = [&](const Item &it, const int (&row)[4], int kb) {
+            if (mine) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    copy4(&tail->row_scale[slot][r0 + i], P.row_scales + static_cast<int64_t>(row[i]) * kbs, kb);
             }
             // lanes 0 and 1: the item's two weight blocks (gate and up, or the
             // two halves of the columns; one past the matrix is never used)
-            const float *blk = nullptr;
-            if (lane < 2) {
+            if (warp == 3 && lane < 2) {
+                int64_t blk;
                 if constexpr (MODE == kGateUp) {
-                    blk = P.block_scales +
-                          (static_cast<int64_t>(it.e) * 2 * nt + it.n + static_cast<int64_t>(lane) * nt) * kbs;
+                    blk = static_cast<int64_t>(it.e) * 2 * nt + it.n + lane * nt;
                 } else {
                     const int per = fp8::groups(P.n);
-                    blk = P.block_scales + (static_cast<int64_t>(it.e) * per + min(2 * it.n + lane, per - 1)) * kbs;
+                    blk = static_cast<int64_t>(it.e) * per + min(2 * it.n + lane, per - 1);
                 }
+                copy4(&tail->block_scale[slot][lane], P.block_scales + blk * kbs, kb);
             }
-            for (int kb0 = 0; ok && kb0 < kbs; kb0 += 4) {
-                float v[4][4], w[4];
+            copy_async_arrive(&tail->sfull[slot]);
+        };
+        int item = blockIdx.x;
+        Item next{};
+        int next_row[4] = {};
+        if (item < total) {
+            next = decode<MODE>(P, tail, item);
+            rows_of(next, next_row);
+        }
+        bool ok = true;
+        for (; ok && item < total; item += gridDim.x) {
+            const Item it = next;
+            int row[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kb = min(kb0 + i, kbs - 1);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i][j] = src[j][kb];
-                    w[i] = blk ? blk[kb] : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (kb0 + i >= kbs) break;
-                    if (!wait_warp(&tail->sempty[slot], phase ^ 1, abort)) {
-                        ok = false;
-                        break;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) tail->row_scale[slot][lane + 32 * j] = v[i][j];
-                    if (lane < 2) tail->block_scale[slot][lane] = w[i];
-                    __syncwarp();
-                    if (lane == 0) sm100::mbar_arrive(&tail->sfull[slot]);
+            for (int i = 0; i < 4; ++i) row[i] = next_row[i];
+            const bool more = item + static_cast<int>(gridDim.x) < total;
+            if (more) {
+                next = decode<MODE>(P, tail, item + gridDim.x);
+                rows_of(next, next_row);
+            }
+            // lanes that load, and what a lane loads
+            const int boxes = kGather ? min(16, (max(0, it.count - 64 * (warp - 2)) + 3) / 4)
+                                      : it.count == kBM ? 1 : (it.count + 15) / 16;
+            const int box_bytes = kGather ? 4 * kGroup : it.count == kBM ? kATile : 16 * kGroup;
+            for (int kb = 0; kb < kbs; ++kb) {
+                if (scales && (kb & 3) == 0) {
+                    ok = __all_sync(0xffffffffu, wait_bar(&tail->sempty[slot], sphase ^ 1, abort));
+                    if (!ok) break;
+                    request_scales(it, row, kb);
                     if (++slot == kScaleSlots) {
                         slot = 0;
-                        phase ^= 1;
+                        sphase ^= 1;
                     }
+                }
+                if (!loads) continue;
+                ok = __all_sync(0xffffffffu, wait_bar(&tail->empty[stage], phase ^ 1, abort));
+                if (!ok) break;
+                uint8_t *a = smem + stage * kStage;
+                uint64_t *bar = &tail->full[stage];
+                if (lane == 0) sm100::mbar_expect_tx(bar, boxes * box_bytes);
+                __syncwarp();
+                if (lane < boxes) {
+                    if constexpr (kGather)
+                        sm100::tma_gather4(a + (r0 - 4 * lane) * kGroup + lane * box_bytes, &tm_x, bar, kb * kGroup,
+                                           row);
+                    else
+                        sm100::tma_load_2d(a + lane * box_bytes, it.count == kBM ? &tm_x : &tm_x16, bar, kb * kGroup,
+                                           it.row0 + lane * 16);
+                }
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
                 }
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else if (warp == 1) {
+        // --------------------------------------------------------- MMA issuer
+        constexpr uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
+        const bool one = sm100::elect_one();
+        uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
+        bool ok = true, any = false;
+        for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
+            for (int kb = 0; kb < kbs; ++kb) {
+                ok = wait_bar(&tail->tempty[buf], bphase ^ 1, abort) && wait_bar(&tail->full[stage], phase, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                sm100::tc_fence_after();
+                const uint32_t base = sm100::smem_u32(smem + stage * kStage), d = tmem + buf * kBN;
+                const uint64_t a = sm100::desc_kmajor_sw128(base), b = sm100::desc_kmajor_sw128(base + kATile);
+                if (one) {
+                    sm100::mma_e4m3<false>(d, a, b, idesc);
+                    sm100::mma_e4m3<true>(d, a + 2, b + 2, idesc);
+                    sm100::mma_e4m3<true>(d, a + 4, b + 4, idesc);
+                    sm100::mma_e4m3<true>(d, a + 6, b + 6, idesc);
+                    sm100::mma_commit(&tail->tfull[buf]);
+                    sm100::mma_commit(&tail->empty[stage]);
+                }
+                __syncwarp();
+                any = true;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                buf ^= 1;
+                bphase ^= buf == 0;
+            }
+        }
+        if (*abort && any) {
+            if (one) sm100::mma_commit(&tail->drain);
+            const uint64_t t0 = now_ns();
+            while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
+            }
+        }
+        __syncwarp();
+      }
     } else {
         // ----------------------------------------------------------- epilogue
-        const int q = warp & 3, h = warp >= 7;  // TMEM lanes 32q.., half of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int q = warp & 3, h = warp >= 8;  // TMEM lanes 32q.., half of the columns
         const int r = 32 * q + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * q) << 16);
+        uint8_t *piece = pieces + (warp - 4) * kPiece;
         uint32_t slot = 0, sphase = 0, buf = 0, bphase = 0, iphase = 0;
-        bool ok = true;
-        for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
+        // the factors of the next four groups: row scale x weight scale (gate's and up's)
+        float s0[4], s1[4];
+        auto take_scales = [&] {
+            wait_bar(&tail->sfull[slot], sphase, abort);
+            const float4 rs = tail->row_scale[slot][r];
+            const float4 b0 = tail->block_scale[slot][MODE == kGateUp ? 0 : h];
+            s0[0] = rs.x * b0.x, s0[1] = rs.y * b0.y, s0[2] = rs.z * b0.z, s0[3] = rs.w * b0.w;
+            if constexpr (MODE == kGateUp) {
+                const float4 b1 = tail->block_scale[slot][1];
+                s1[0] = rs.x * b1.x, s1[1] = rs.y * b1.y, s1[2] = rs.z * b1.z, s1[3] = rs.w * b1.w;
+            }
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&tail->sempty[slot]);
+            if (++slot == kScaleSlots) {
+                slot = 0;
+                sphase ^= 1;
+            }
+        };
+        for (int item = blockIdx.x; item < total; item += gridDim.x) {
             const Item it = decode<MODE>(P, tail, item);
             const bool active = 32 * q < it.count;  // the warp has rows of the tile
             float acc[128];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+            take_scales();
             for (int kb = 0; kb < kbs; ++kb) {
-                if (!wait_warp(&tail->sfull[slot], sphase, abort)) {
-                    ok = false;
-                    break;
+                const float g0 = s0[0], g1 = MODE == kGateUp ? s1[0] : s0[0];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    s0[i] = s0[i + 1];
+                    if (MODE == kGateUp) s1[i] = s1[i + 1];
                 }
-                const float rs = tail->row_scale[slot][r];
-                const float s0 = rs * tail->block_scale[slot][MODE == kGateUp ? 0 : h];
-                const float s1 = MODE == kGateUp ? rs * tail->block_scale[slot][1] : s0;
-                __syncwarp();
-                if (lane == 0) sm100::mbar_arrive(&tail->sempty[slot]);
-                if (++slot == kScaleSlots) {
-                    slot = 0;
-                    sphase ^= 1;
-                }
-                if (!wait_warp(&tail->tfull[buf], bphase, abort)) {
-                    ok = false;
-                    break;
-                }
+                const bool refill = (kb & 3) == 3 && kb + 1 < kbs;
+                wait_bar(&tail->tfull[buf], bphase, abort);
                 sm100::tc_fence_after();
                 if (active) {
                     // 16 columns at a time; gate/up: 64 of the gate block, then
@@ -423,15 +511,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     };
                     float t[2][16];
                     sm100::tmem_ld16(col(0), t[0]);
+                    if (refill) take_scales();
                     wait_ld16(t[0]);
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         if (c < 7) sm100::tmem_ld16(col(c + 1), t[(c + 1) & 1]);
-                        const float s = c < 4 ? s0 : s1;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(t[c & 1][i], s, acc[16 * c + i]);
+                        for (int i = 0; i < 16; ++i)
+                            acc[16 * c + i] = fmaf(t[c & 1][i], c < 4 ? g0 : g1, acc[16 * c + i]);
                         if (c < 7) wait_ld16(t[(c + 1) & 1]);
                     }
+                } else if (refill) {
+                    take_scales();
                 }
                 sm100::tc_fence_before();
                 __syncwarp();
@@ -439,95 +530,91 @@ __global__ void __launch_bounds__(kThreads, 1)
                 buf ^= 1;
                 bphase ^= buf == 0;
             }
-            if (!ok) break;
-            const bool row = r < it.count;
-            const int64_t at = static_cast<int64_t>(it.row0) + r;
+            if (!active) continue;
+            const int rows = it.count - 32 * q;  // of this warp, if below 32
+            const int64_t first = static_cast<int64_t>(it.row0) + 32 * q;
             if constexpr (MODE == kGateUp) {
-                if (!active) continue;
                 float top = fp8::kTiny;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                    acc[i] = silu_f32(acc[i]) * acc[64 + i];
+                    acc[i] = silu_fast(acc[i]) * acc[64 + i];
                     top = fp8::max_nan(top, fabsf(acc[i]));
                 }
                 // the group's other 64 columns are the other half's
                 tail->top[iphase][h][r] = top;
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&tail->half[q]);
-                if (!wait_warp(&tail->half[q], iphase, abort)) {
-                    ok = false;
-                    break;
-                }
+                wait_bar(&tail->half[q], iphase, abort);
                 top = fp8::max_nan(top, tail->top[iphase][h ^ 1][r]);
                 iphase ^= 1;
-                if (row) {
-                    const fp8::Divisor f(top);
-                    uint8_t *dst = P.act + at * P.n + it.n * kGroup + 64 * h;
+                const fp8::Divisor f(top);
+                uint32_t v[16];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 32) {
-                        uint32_t v[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v[j] = fp8::pack4(f, acc[i + 4 * j], acc[i + 4 * j + 1], acc[i + 4 * j + 2],
-                                              acc[i + 4 * j + 3]);
-                        store32(dst + i, v);
+                for (int i = 0; i < 16; ++i)
+                    v[i] = fp8::pack4(f, acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+                store_rows64(piece, v, P.act + first * P.n + it.n * kGroup + 64 * h, P.n, rows, 4);
+                if (h == 0 && lane < rows) P.act_scales[(first + lane) * nt + it.n] = fp8::scale_of(top);
+            } else {
+                const int n0 = it.n * kBN + 128 * h;
+                const bool f32 = MODE == kLinear && P.out_f32;
+                // whole 16-byte units: 8 BF16 or 4 FP32 columns, all or none of
+                // them there (the down product's H is a multiple of 16)
+                const bool vec = MODE == kDown || P.n % (f32 ? 4 : 8) == 0;
+                if (vec && !f32 && (MODE == kLinear || rows >= 32)) {
+                    // The map cuts rows and columns past the matrix; another
+                    // expert's rows below a partial tile must not be written,
+                    // so those take the other way.
+                    if (lane == 0) sm100::bulk_wait_read();  // the last item's stores have left the buffer
+                    __syncwarp();
+                    stage_row256(piece, acc);
+                    sm100::fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (n0 < P.n) sm100::tma_store_2d(piece, &tm_out, n0, static_cast<int>(first));
+                        if (n0 + 64 < P.n) sm100::tma_store_2d(piece + 4096, &tm_out, n0 + 64, static_cast<int>(first));
+                        sm100::bulk_commit();
                     }
-                    if (h == 0) P.act_scales[at * nt + it.n] = fp8::scale_of(top);
-                }
-            } else if constexpr (MODE == kDown) {
-                // n % 16 == 0: 16 columns are 32 aligned bytes, all or none of them there
-                uint16_t *dst = static_cast<uint16_t *>(P.out) + at * P.n;
-                if (row) {
+                } else if (vec && !f32) {
+                    if (lane == 0) sm100::bulk_wait_read();
+                    uint16_t *dst = static_cast<uint16_t *>(P.out) + first * P.n + n0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = fp8::pack_bf16(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]);
+                        store_rows64(piece + 2048 * c, v, reinterpret_cast<uint8_t *>(dst + 32 * c),
+                                     2 * static_cast<int64_t>(P.n), rows, (P.n - n0 - 32 * c) / 8);
+                    }
+                } else if (vec) {
+                    float *dst = static_cast<float *>(P.out) + first * P.n + n0;
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
-                        const int n0 = it.n * kBN + 128 * h + 16 * c;
-                        if (n0 < P.n) {
-                            uint32_t v[8];
+                        uint32_t v[16];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = pack_bf16x2(acc[16 * c + 2 * j], acc[16 * c + 2 * j + 1]);
-                            store32(dst + n0, v);
-                        }
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(acc[16 * c + i]);
+                        store_rows64(piece + 2048 * (c & 3), v, reinterpret_cast<uint8_t *>(dst + 16 * c),
+                                     4 * static_cast<int64_t>(P.n), rows, (P.n - n0 - 16 * c) / 4);
                     }
-                }
-            } else {
-                const bool vec = P.n % 16 == 0;
+                } else if (lane < rows) {
+                    const int64_t at = (first + lane) * P.n + n0;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const int n0 = it.n * kBN + 128 * h + 16 * c;
-                    if (!row || n0 >= P.n) continue;
-                    if (P.out_f32) {
-                        float *dst = static_cast<float *>(P.out) + at * P.n + n0;
-                        if (vec) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                reinterpret_cast<float4 *>(dst)[i] =
-                                    make_float4(acc[16 * c + 4 * i], acc[16 * c + 4 * i + 1], acc[16 * c + 4 * i + 2],
-                                                acc[16 * c + 4 * i + 3]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (n0 + i < P.n) dst[i] = acc[16 * c + i];
-                        }
-                    } else {
-                        uint16_t *dst = static_cast<uint16_t *>(P.out) + at * P.n + n0;
-                        if (vec) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                reinterpret_cast<uint4 *>(dst)[i] =
-                                    make_uint4(pack_bf16x2(acc[16 * c + 8 * i], acc[16 * c + 8 * i + 1]),
-                                               pack_bf16x2(acc[16 * c + 8 * i + 2], acc[16 * c + 8 * i + 3]),
-                                               pack_bf16x2(acc[16 * c + 8 * i + 4], acc[16 * c + 8 * i + 5]),
-                                               pack_bf16x2(acc[16 * c + 8 * i + 6], acc[16 * c + 8 * i + 7]));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (n0 + i < P.n) dst[i] = f2bf(acc[16 * c + i]);
-                        }
+                    for (int i = 0; i < 128; ++i) {
+                        if (n0 + i >= P.n) continue;
+                        if (f32) static_cast<float *>(P.out)[at + i] = acc[i];
+                        else static_cast<uint16_t *>(P.out)[at + i] = f2bf(acc[i]);
                     }
                 }
             }
         }
+        if (lane == 0) sm100::bulk_wait_all();
+        __syncwarp();
         sm100::tc_fence_before();
+    }
+    if (*abort && warp < 4) {
+        // loads may be in flight whose barriers will never complete: give them
+        // a time far above any load's before the CTA leaves
+        const uint64_t t0 = now_ns();
+        while (now_ns() - t0 < 200000) __nanosleep(1000);
     }
     __syncthreads();
     if (warp == 1) {
@@ -574,16 +661,16 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const uint16_t *__rest
         }
     }
     *reinterpret_cast<uint4 *>(out + t * hidden + c) =
-        make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
-                   pack_bf16x2(acc[6], acc[7]));
+        make_uint4(fp8::pack_bf16(acc[0], acc[1]), fp8::pack_bf16(acc[2], acc[3]), fp8::pack_bf16(acc[4], acc[5]),
+                   fp8::pack_bf16(acc[6], acc[7]));
 }
 
 template <int MODE>
-int launch_tile(const CUtensorMap &x, const CUtensorMap &x16, const CUtensorMap &w, const Params &P, int64_t items,
-                cudaStream_t stream) {
+int launch_tile(const CUtensorMap &x, const CUtensorMap &x16, const CUtensorMap &w, const CUtensorMap &out,
+                const Params &P, int64_t items, cudaStream_t stream) {
     if (int rc = ensure_dynamic_smem(fp8_tile_kernel<MODE>, kSmem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
     return launch_pdl(fp8_tile_kernel<MODE>, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
-                      dim3(kThreads), kSmem, stream, "fp8_tile_kernel", x, x16, w, P);
+                      dim3(kThreads), kSmem, stream, "fp8_tile_kernel", x, x16, w, out, P);
 }
 
 int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int cols) {
@@ -593,14 +680,23 @@ int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int c
     return make_map_u8(m16, base, 2, dims, str, 16);
 }
 
+// BF16 output rows (cols % 8 == 0), stored 32 rows by 64 columns at a time.
+int out_map(CUtensorMap *m, const void *base, int rows, int cols) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+    const uint64_t str[1] = {static_cast<uint64_t>(cols) * 2};
+    return make_map_bf16(m, base, 2, dims, str, 32);
+}
+
 }  // namespace
 
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream) {
-    CUtensorMap x{}, x16{}, w{};
+    CUtensorMap x{}, x16{}, w{}, out{};
     if (int rc = row_maps(&x, &x16, a.x, a.tokens, a.cols)) return rc;
     const uint64_t dims[2] = {static_cast<uint64_t>(a.cols), static_cast<uint64_t>(a.rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(a.cols)};
     if (int rc = make_map_u8(&w, a.w, 2, dims, str, 128)) return rc;
+    if (!a.out_f32 && a.rows % 8 == 0)
+        if (int rc = out_map(&out, a.out, a.tokens, a.rows)) return rc;
     Params P{};
     P.row_scales = a.x_scales;
     P.block_scales = a.w_scales;
@@ -612,7 +708,7 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
     P.status = status;
     const int64_t items = static_cast<int64_t>((a.tokens + kBM - 1) / kBM) * ((a.rows + kBN - 1) / kBN);
     LRB_REQUIRE(items < (1ll << 31), "moe_linear_fp8: too many tiles");
-    return launch_tile<kLinear>(x, x16, w, P, items, stream);
+    return launch_tile<kLinear>(x, x16, w, out, P, items, stream);
 }
 
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream) {
@@ -624,7 +720,7 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     const int64_t tiles = std::min<int64_t>(a.experts, routes) + routes / kBM;
     const int64_t nt1 = a.inner / kGroup, nt2 = (a.hidden + kBN - 1) / kBN;
     LRB_REQUIRE(tiles * std::max(nt1, nt2) < (1ll << 31), "moe_experts_fp8: too many tiles");
-    CUtensorMap x{}, act{}, act16{}, gu{}, dn{};
+    CUtensorMap x{}, act{}, act16{}, gu{}, dn{}, y{};
     {
         // rows gathered four at a time: the map's box is one row
         const uint64_t dims[2] = {static_cast<uint64_t>(a.hidden), static_cast<uint64_t>(a.tokens)};
@@ -632,6 +728,7 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
         if (int rc = make_map_u8(&x, a.x, 2, dims, str, 1)) return rc;
     }
     if (int rc = row_maps(&act, &act16, s.act, routes, a.inner)) return rc;
+    if (int rc = out_map(&y, s.y, routes, a.hidden)) return rc;
     {
         const uint64_t H = a.hidden, I = a.inner, E = a.experts;
         const uint64_t d1[3] = {H, 2 * I, E}, s1[2] = {H, 2 * I * H}, d2[3] = {I, H, E}, s2[2] = {I, H * I};
@@ -650,13 +747,13 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     G.k = a.hidden;
     G.act = s.act;
     G.act_scales = s.act_scales;
-    if (int rc = launch_tile<kGateUp>(x, x, gu, G, tiles * nt1, stream)) return rc;
+    if (int rc = launch_tile<kGateUp>(x, x, gu, y, G, tiles * nt1, stream)) return rc;
     P.row_scales = s.act_scales;
     P.block_scales = a.down_scales;
     P.n = a.hidden;
     P.k = a.inner;
     P.out = s.y;
-    if (int rc = launch_tile<kDown>(act, act16, dn, P, tiles * nt2, stream)) return rc;
+    if (int rc = launch_tile<kDown>(act, act16, dn, y, P, tiles * nt2, stream)) return rc;
     const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 255) / 256;
     return launch_pdl(fp8_combine_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, stream,
                       "fp8_combine_kernel", static_cast<const uint16_t *>(s.y),

@@ -25,7 +25,7 @@ int check_experts(int tokens, int experts, int top_k, int hidden, int inner) {
 struct Layout {
     bool gemv;
     int hist_ints;
-    size_t offsets, perm_token, perm_slot, route_pos, active, counters, hist, act, act_scales, y, bytes;
+    size_t offsets, perm_token, perm_slot, route_pos, active, permute_counters, hist, counters, act, act_scales, y, bytes;
 };
 Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
     Layout l{};
@@ -48,8 +48,9 @@ Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
     l.perm_slot = take(sizeof(int32_t) * routes);
     l.route_pos = take(sizeof(int32_t) * routes);
     l.active = take(sizeof(int32_t) * experts);
-    l.counters = take(sizeof(int32_t) * 2);
+    l.permute_counters = take(sizeof(int32_t) * 2);
     l.hist = take(sizeof(int32_t) * static_cast<size_t>(l.hist_ints));
+    l.counters = take(sizeof(int32_t) * (experts + 1));
     l.act = take(routes * inner);
     l.act_scales = take(routes * (inner / fp8::kGroup) * sizeof(float));
     l.y = take(routes * hidden * 2);
@@ -113,9 +114,17 @@ extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const ui
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     if (l.gemv) return launch_experts_fp8_gemv(a, reinterpret_cast<float *>(ws), as_stream(stream));
     auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(ws + at); };
-    const ExpertsFp8Scratch s{ints(l.offsets),  ints(l.perm_token), ints(l.perm_slot),
-                              ints(l.route_pos), ints(l.active),    ints(l.counters),
-                              l.hist_ints ? ints(l.hist) : nullptr, ws + l.act,
-                              reinterpret_cast<float *>(ws + l.act_scales), reinterpret_cast<uint16_t *>(ws + l.y)};
+    ExpertsFp8Scratch s{};
+    s.offsets = ints(l.offsets);
+    s.perm_token = ints(l.perm_token);
+    s.perm_slot = ints(l.perm_slot);
+    s.route_pos = ints(l.route_pos);
+    s.active = ints(l.active);
+    s.permute_counters = ints(l.permute_counters);
+    s.hist = l.hist_ints ? ints(l.hist) : nullptr;
+    s.counters = ints(l.counters);
+    s.act = ws + l.act;
+    s.act_scales = reinterpret_cast<float *>(ws + l.act_scales);
+    s.y = reinterpret_cast<uint16_t *>(ws + l.y);
     return launch_experts_fp8_tiles(a, s, status, as_stream(stream));
 }

@@ -37,7 +37,8 @@ int launch_experts_fp8_gemv(const ExpertsFp8 &a, float *h, cudaStream_t stream);
 
 // The tensor-core path.  status (or null): set to 1 if a bounded wait gave up.
 struct ExpertsFp8Scratch {
-    int32_t *offsets, *perm_token, *perm_slot, *route_pos, *active, *counters, *hist;  // as moe_permute_wide
+    int32_t *offsets, *perm_token, *perm_slot, *route_pos, *active, *permute_counters, *hist;  // as moe_permute_wide
+    int32_t *counters;  // [E + 1]: items handed out, and per expert the finished parts of gate/up items
     uint8_t *act;       // [T * K, I]
     float *act_scales;  // [T * K, I / 128]
     uint16_t *y;        // [T * K, H]

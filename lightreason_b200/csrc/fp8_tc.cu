@@ -1,34 +1,45 @@
 // The FP8 products on the 5th-generation tensor cores: one persistent kernel
 // for a plain product and for the two grouped products of the routed experts.
 //
-// Mathematics.  A tile is 128 rows (tokens, or routes of one expert) by 256
-// weight rows.  Within a 128-column group g both scales are constants of the
+// Mathematics.  Within a 128-column group g both scales are constants of the
 // row and of the 128-row weight block, so
 //   out[m, n] = sum_g  xs[m, g] * ws[n / 128, g] * (sum over the group of xq wq).
 // tcgen05.mma (kind::f8f6f4) forms the inner sum of one group, four products of
-// 32 columns, in one of two TMEM buffers of 256 columns; eight warps read it
-// while the other buffer fills and add it, times the two scales, to FP32
-// registers (128 a thread).  The scales are any FP32 values, so they cannot ride
-// in the tensor core's own power-of-two block scales.
+// 32 columns, in one of several TMEM buffers; eight warps read it while the
+// next buffers fill and add it, times the two scales, to FP32 registers.  The
+// scales are any FP32 values, so they cannot ride in the tensor core's own
+// power-of-two block scales.
 //
-// Layout.  Rows are the M operand: a lane of the accumulator is one row, so a
-// group's factor is one number per thread, gate and up of a column meet in one
-// thread, and a partial tile's missing rows cost no epilogue work (whole warps
-// skip).  A stage is one group: 256 weight rows (32 KB, two boxes) and the
-// tile's rows (gathered by TMA from the token rows for gate/up, in boxes of 16
-// when the tile is partial), three stages deep: 96 KB of weights in flight per
-// SM, which is what streams the banks at small and middle widths, where the
-// M = 128 products on padding are hidden under the weight stream.
+// An item is a tile of rows (of one expert) by 256 weight rows: 128 gate and
+// the 128 up rows of the same columns, or 256 rows of down or of a plain
+// weight.  Two layouts:
+//  * BN = 0, rows as M: tiles of 128 rows against N = 256 weight rows.  An
+//    accumulator lane is one row, so a group's factor is one number per thread,
+//    gate and up of a column meet in one thread, and warps without rows of a
+//    partial tile skip.
+//  * BN = 16, 32, 64, weights as M: the two blocks of 128 weight rows against
+//    N = BN rows.  A lane is one weight row and the tile's few rows are its
+//    columns: at a few rows per expert all eight warps share the epilogue
+//    instead of one row's pair of warps doing it.
+// A stage is one group: the 256 weight rows (32 KB, two boxes) and the tile's
+// rows (gathered by TMA from the token rows for gate/up; boxes of 16 when the
+// tile is partial).  Three to six stages keep 96 to 192 KB of weights in flight
+// per SM, which is what streams the banks at small and middle widths.
 //
-// What bounds it at large widths: the four products of a group take 647 cycles
-// of the tensor core, and reading the group's 128 KB of sums out of TMEM takes
-// 228 more from it (both run alone at 647 and 385, together at 875 a group).
+// The experts are one launch: gate/up items, then down items, fetched in order
+// from a counter.  A down item's weights are requested at once, its rows when
+// the expert's gate/up items have counted in (done[e]); every such wait is for
+// an item that a running CTA already has, whatever else the GPU runs.
 //
-// Warps: 0 weight tiles, 1 MMA, 2 and 3 row tiles and scales (four groups at a
-// time, up to four such requests in flight), 4-11 epilogue; the first four hand registers to the
-// others (104 and 200 a thread of 168 at launch, 64,512 a CTA either way).
-// Every wait is bounded; a timeout raises *status, drains what is in flight and
-// returns.
+// What bounds it: the weight stream up to a few hundred rows per expert; above,
+// reading the sums: a group's four products take 512 cycles, with the eight
+// warps reading 128 KB of TMEM beside them 583 (each alone: 512 and 385).
+//
+// Warps: 0 items and weight tiles, 1 MMA, 2 and 3 row tiles and scales (four
+// groups at a time, up to four such requests in flight), 4-11 epilogue; the
+// first four hand registers to the others (104 and 200 a thread of 168 at
+// launch, 64,512 a CTA either way).  Every wait is bounded; a timeout raises
+// *status, drains what is in flight and returns.
 #include <algorithm>
 
 #include "fp8_kernels.cuh"
@@ -40,43 +51,57 @@ namespace {
 using fp8::kGroup;
 
 constexpr int kBM = 128, kBN = 256;
-constexpr int kStages = 3;
-constexpr int kATile = kBM * kGroup, kBTile = kBN * kGroup, kStage = kATile + kBTile;
+constexpr int kBTile = kBN * kGroup;
 constexpr int kThreads = 12 * 32;
-constexpr int kScaleSlots = 4;   // of four groups each
-constexpr int kPiece = 8192;     // an epilogue warp's output: 32 rows of 256 bytes
+constexpr int kScaleSlots = 4;  // of four groups each
+constexpr int kRing = 4;        // items on their way to the warps
 constexpr int kMaxExperts = 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-enum Mode { kLinear, kGateUp, kDown };
-
-struct Tail {
-    float4 row_scale[kScaleSlots][kBM];
-    float4 block_scale[kScaleSlots][2];
-    float top[2][2][kBM];
-    uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], sfull[kScaleSlots], sempty[kScaleSlots], half[4],
-        drain;
-    int abort;
-    uint32_t tmem;
-    int32_t scan[16];
-    int32_t items[kMaxExperts + 1];   // first item of each expert
+// LIN: the plain product; otherwise the experts.
+template <bool LIN, int BN>
+struct Shape {
+    static constexpr bool kSwap = BN != 0;
+    static constexpr int kRows = kSwap ? BN : kBM;  // rows of a tile
+    static constexpr int kATile = kRows * kGroup, kStage = kATile + kBTile;
+    static constexpr int kStages = kSwap ? (BN == 64 ? 5 : 6) : LIN ? 3 : 4;
+    static constexpr int kBufs = kSwap ? 4 : 2;
+    static constexpr int kBufCols = kSwap ? 2 * BN : kBN;
+    // an epilogue warp's output buffer: 32 rows of 256 bytes (stored by TMA) or of 64
+    static constexpr int kPiece = kSwap ? 0 : LIN ? 8192 : 2048;
+    struct Tail {
+        // rows as M: a row's four factors together; weights as M: a group's rows together
+        float row_scale[kScaleSlots][kRows * 4];
+        float4 block_scale[kScaleSlots][2];
+        float top[2][kSwap ? 4 : 2][kSwap ? 64 : kBM];
+        int4 ring[kRing][2];
+        uint64_t full[kStages], empty[kStages], tfull[kBufs], tempty[kBufs], sfull[kScaleSlots], sempty[kScaleSlots],
+            ifull[kRing], iempty[kRing], half[4], drain;
+        int abort;
+        uint32_t tmem;
+        int32_t scan[16];
+        int32_t tiles[LIN ? 1 : kMaxExperts + 1];  // row tiles of the experts before e
+    };
+    static constexpr int kSmem = kStages * kStage + 8 * kPiece + static_cast<int>(sizeof(Tail)) + 1024;
+    static_assert(kSmem <= 232448, "shared memory of one SM");
 };
-constexpr int kSmem = kStages * kStage + 8 * kPiece + static_cast<int>(sizeof(Tail)) + 1024;
-static_assert(kSmem <= 232448, "shared memory of one SM");
 
 struct Params {
-    const float *row_scales;      // [rows, groups]
-    const float *block_scales;    // [(E,) blocks, groups]
-    const int32_t *offsets;       // [E + 1] (experts)
-    const int32_t *row_token;     // [R] route -> token (gate/up)
-    int rows;                     // linear: T
-    int n;                        // output columns: rows of w, I (gate/up), H (down)
-    int k;                        // H, H, I
-    int experts;
-    void *out;                    // linear: [T, n]; down: BF16 [R, n]
+    // linear
+    const float *x_scales, *w_scales;  // [T, groups], [blocks, groups]
+    int rows, n, k;                    // T, weight rows, columns
+    void *out;                         // [T, n]
     int out_f32;
-    uint8_t *act;                 // gate/up: [R, I] e4m3
-    float *act_scales;            // gate/up: [R, I / 128]
+    // experts
+    const float *act_scales_in, *down_scales;  // phase 2: [R, I / 128], [E, blocks, I / 128]
+    const int32_t *offsets;                    // [E + 1]
+    const int32_t *row_token;                  // [R] route -> token
+    int experts, hidden, inner;
+    uint8_t *act;       // [R, I] e4m3
+    float *act_scales;  // [R, I / 128]
+    uint16_t *y;        // [R, H] BF16
+    int32_t *work;      // items handed out so far (zero at launch)
+    int32_t *done;      // [E] epilogue warps that finished an item of phase 1 (zero at launch)
     int32_t *status;
 };
 
@@ -85,11 +110,10 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Bounded wait; false once the CTA has given up.  Warps that work as one (the
-// scales' and the epilogue's) do not leave on false: from then on their waits
-// return at once and they run to the end on whatever is there, together.
-// The clock (and the flag) are looked at every 256th poll only: reading the
-// global timer takes longer than most waits.
+// Bounded wait; false once the CTA has given up.  The epilogue warps do not
+// leave on false: from then on their waits return at once and they run to the
+// end on whatever is there, together.  The clock (and the flag) are looked at
+// every 256th poll only: reading the global timer takes longer than most waits.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort) {
     uint64_t t0 = 0;
     for (uint32_t i = 1; !sm100::mbar_try_wait(bar, parity); ++i) {
@@ -104,40 +128,13 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
     }
     return true;
 }
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+}
 
 struct Item {
-    int e, row0, count, n;  // expert, first row, rows (<= 128), column tile
-    bool shared_tiles;      // other tiles read the same weight rows
+    int phase, e, row0, count, n, mt;  // 1 gate/up, 2 down or linear, 0 none; expert; first row, rows; weight tile; the expert's row tiles
 };
-
-template <int MODE>
-__device__ __forceinline__ Item decode(const Params &P, const Tail *tail, int item) {
-    Item r;
-    if constexpr (MODE == kLinear) {
-        const int mt = (P.rows + kBM - 1) / kBM;
-        r.e = 0;
-        r.n = item / mt;
-        r.row0 = (item % mt) * kBM;
-        r.count = min(kBM, P.rows - r.row0);
-        r.shared_tiles = mt > 1;
-    } else {
-        int lo = 0, hi = P.experts;  // the expert with items[e] <= item < items[e + 1]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (tail->items[mid] <= item) lo = mid;
-            else hi = mid;
-        }
-        const int begin = P.offsets[lo], count = P.offsets[lo + 1] - begin;
-        const int mt = (count + kBM - 1) / kBM, at = item - tail->items[lo];
-        r.e = lo;
-        r.n = at / mt;
-        const int m = at % mt;
-        r.row0 = begin + m * kBM;
-        r.count = min(kBM, count - m * kBM);
-        r.shared_tiles = mt > 1;
-    }
-    return r;
-}
 
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void *dst, const void *src) {
@@ -148,14 +145,35 @@ __device__ __forceinline__ void copy_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
 
+// N (8 or 16) TMEM columns of this warp's lanes.
+template <int N>
+__device__ __forceinline__ void load_cols(uint32_t at, float (&v)[N]) {
+    static_assert(N == 8 || N == 16, "columns");
+    if constexpr (N == 16) {
+        sm100::tmem_ld16(at, v);
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "r"(at)
+                     : "memory");
+    }
+}
 // Completes this warp's TMEM loads; the values pass through, so no use of them
 // can be moved before it.
-__device__ __forceinline__ void wait_ld16(float (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
-                 :
-                 : "memory");
+template <int N>
+__device__ __forceinline__ void wait_cols(float (&v)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                       "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                       "+f"(v[15])
+                     :
+                     : "memory");
+    else
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])
+                     :
+                     : "memory");
 }
 
 // A warp's 32 rows of 64 bytes, one row a lane, to global memory as whole
@@ -197,37 +215,56 @@ __device__ __forceinline__ void stage_row256(uint8_t *buf, const float (&acc)[12
                        fp8::pack_bf16(acc[8 * u + 4], acc[8 * u + 5]), fp8::pack_bf16(acc[8 * u + 6], acc[8 * u + 7]));
 }
 
-template <int MODE>
+// tm_x: linear, the row tiles; experts, the token rows (gathered).  tm_r, tm_r16:
+// full and 16-row boxes of the rows of linear or phase 2.  tm_w, tm_w2: weights
+// of linear or phase 1, and of phase 2.  tm_out: linear's BF16 output.
+template <bool LIN, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x16,
-                    const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_out,
+    fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_r,
+                    const __grid_constant__ CUtensorMap tm_r16, const __grid_constant__ CUtensorMap tm_w,
+                    const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ CUtensorMap tm_out,
                     const Params P) {
+    using S = Shape<LIN, BN>;
+    constexpr bool kSwap = S::kSwap;
+    constexpr int kRows = S::kRows;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *pieces = smem + kStages * kStage;
-    Tail *tail = reinterpret_cast<Tail *>(pieces + 8 * kPiece);
+    // a stage: the weight tile, then the rows (both on 1024-byte boundaries)
+    uint8_t *pieces = smem + S::kStages * S::kStage;
+    typename S::Tail *tail = reinterpret_cast<typename S::Tail *>(pieces + 8 * S::kPiece);
     volatile int *abort = &tail->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // gate/up rows as M: two warps gather a tile's rows
+    constexpr int kGatherWarps = kSwap ? 1 : 2;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            sm100::mbar_init(&tail->full[s], MODE == kGateUp ? 3 : 2);  // the warps that load into it
+        for (int s = 0; s < S::kStages; ++s) {
+            sm100::mbar_init(&tail->full[s], LIN ? 2 : 1 + kGatherWarps);  // the warps that load into it
             sm100::mbar_init(&tail->empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < S::kBufs; ++b) {
             sm100::mbar_init(&tail->tfull[b], 1);
             sm100::mbar_init(&tail->tempty[b], 8);
         }
         for (int s = 0; s < kScaleSlots; ++s) {
-            sm100::mbar_init(&tail->sfull[s], MODE == kGateUp ? 64 : 32);  // lanes
+            sm100::mbar_init(&tail->sfull[s], 32);  // the lanes of warp 3
             sm100::mbar_init(&tail->sempty[s], 8);
         }
-        for (int q = 0; q < 4; ++q) sm100::mbar_init(&tail->half[q], 2);
+        for (int s = 0; s < kRing; ++s) {
+            sm100::mbar_init(&tail->ifull[s], 1);
+            sm100::mbar_init(&tail->iempty[s], 11);  // every warp but 0
+        }
+        for (int q = 0; q < 4; ++q) sm100::mbar_init(&tail->half[q], kSwap ? 4 : 2);
         sm100::mbar_init(&tail->drain, 1);
         tail->abort = 0;
         sm100::fence_barrier_init();
         sm100::tma_prefetch_map(&tm_x);
         sm100::tma_prefetch_map(&tm_w);
+        if constexpr (!LIN) {
+            sm100::tma_prefetch_map(&tm_w2);
+            sm100::tma_prefetch_map(&tm_r);
+        }
+        sm100::tma_prefetch_map(&tm_r16);
     }
     if (warp == 1) {
         sm100::tmem_alloc(&tail->tmem, 512);
@@ -240,20 +277,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     grid_dependency_wait();
     grid_dependency_trigger();
 
-    const int kbs = fp8::groups(P.k);
-    const int nt = MODE == kGateUp ? P.n / kGroup : (P.n + kBN - 1) / kBN;
-    int total;
-    if constexpr (MODE == kLinear) {
-        total = nt * ((P.rows + kBM - 1) / kBM);
+    // groups and weight tiles of the two phases (linear is a phase 2)
+    const int kbs1 = LIN ? 0 : fp8::groups(P.hidden), kbs2 = fp8::groups(LIN ? P.k : P.inner);
+    const int n2 = LIN ? P.n : P.hidden;
+    const int nt1 = LIN ? 0 : P.inner / kGroup, nt2 = (n2 + kBN - 1) / kBN;
+    int items1 = 0, total;
+    if constexpr (LIN) {
+        total = nt2 * ((P.rows + kRows - 1) / kRows);
     } else {
-        // items[e]: an exclusive scan of the experts' tile counts, a few
+        // tiles[e]: an exclusive scan of the experts' row tiles, a few
         // neighbouring experts a thread
         constexpr int kPer = (kMaxExperts + kThreads) / kThreads;
         int tiles[kPer], sum = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int e = threadIdx.x * kPer + i;
-            tiles[i] = e < P.experts ? nt * ((P.offsets[e + 1] - P.offsets[e] + kBM - 1) / kBM) : 0;
+            tiles[i] = e < P.experts ? (P.offsets[e + 1] - P.offsets[e] + kRows - 1) / kRows : 0;
             sum += tiles[i];
         }
         int incl = sum;
@@ -269,214 +308,321 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int e = threadIdx.x * kPer + i;
-            if (e <= P.experts) tail->items[e] = at;
+            if (e <= P.experts) tail->tiles[e] = at;
             at += tiles[i];
         }
         __syncthreads();
-        total = tail->items[P.experts];
+        items1 = nt1 * tail->tiles[P.experts];
+        total = items1 + nt2 * tail->tiles[P.experts];
     }
+    auto decode = [&](int item) {
+        Item r;
+        if (item >= total) {
+            r.phase = 0;
+            return r;
+        }
+        if constexpr (LIN) {
+            r.mt = (P.rows + kRows - 1) / kRows;
+            r.phase = 2;
+            r.e = 0;
+            r.n = item / r.mt;
+            r.row0 = (item % r.mt) * kRows;
+            r.count = min(kRows, P.rows - r.row0);
+        } else {
+            r.phase = item < items1 ? 1 : 2;
+            const int nt = r.phase == 1 ? nt1 : nt2;
+            const int x = r.phase == 1 ? item : item - items1, u = x / nt;
+            int lo = 0, hi = P.experts;  // the expert with tiles[e] <= u < tiles[e + 1]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (tail->tiles[mid] <= u) lo = mid;
+                else hi = mid;
+            }
+            const int begin = P.offsets[lo], count = P.offsets[lo + 1] - begin;
+            // the tiles of one weight tile are neighbours
+            r.mt = (count + kRows - 1) / kRows;
+            const int at = x - nt * tail->tiles[lo];
+            r.e = lo;
+            r.n = at / r.mt;
+            const int m = at % r.mt;
+            r.row0 = begin + m * kRows;
+            r.count = min(kRows, count - m * kRows);
+        }
+        return r;
+    };
+    // The item after the last one this warp took: linear, the CTA's next of a
+    // fixed order; experts, from the ring that warp 0 fills.
+    int take_at = LIN ? blockIdx.x : 0;
+    auto take_item = [&]() {
+        if constexpr (LIN) {
+            const Item r = decode(take_at);
+            take_at += gridDim.x;
+            return r;
+        } else {
+            const int slot = take_at % kRing;
+            Item r;
+            r.phase = 0;
+            if (wait_warp(&tail->ifull[slot], (take_at / kRing) & 1, abort)) {
+                const int4 a = tail->ring[slot][0], b = tail->ring[slot][1];
+                r = Item{a.x, a.y, a.z, a.w, b.x, b.y};
+            }
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&tail->iempty[slot]);
+            ++take_at;
+            return r;
+        }
+    };
 
     if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-      if (warp == 0) {
-        // ------------------------------------------------------ weight tiles
-        const uint64_t once = sm100::l2_evict_first_policy(), keep = sm100::l2_evict_normal_policy();
-        const bool one = sm100::elect_one();
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         uint32_t stage = 0, phase = 0;
-        bool ok = true;
-        for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-            const Item it = decode<MODE>(P, tail, item);
-            const uint64_t policy = it.shared_tiles ? keep : once;
-            for (int kb = 0; kb < kbs; ++kb) {
-                ok = __all_sync(0xffffffffu, wait_bar(&tail->empty[stage], phase ^ 1, abort));
-                if (!ok) break;
-                uint8_t *b = smem + stage * kStage + kATile;
-                uint64_t *bar = &tail->full[stage];
-                const int r0 = MODE == kGateUp ? it.n * kGroup : it.n * kBN;
-                const int r1 = MODE == kGateUp ? P.n + r0 : r0 + 128;
-                if (one) {
-                    sm100::mbar_expect_tx(bar, kBTile);
-                    if constexpr (MODE == kLinear) {
-                        sm100::tma_load_2d_hint(b, &tm_w, bar, kb * kGroup, r0, policy);
-                        sm100::tma_load_2d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, policy);
-                    } else {
-                        sm100::tma_load_3d_hint(b, &tm_w, bar, kb * kGroup, r0, it.e, policy);
-                        sm100::tma_load_3d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, it.e, policy);
-                    }
-                }
-                __syncwarp();
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            }
-        }
-      } else if (warp >= 2) {
-        // --------------------------------------------- row tiles and scales
-        // gate/up: warp 2 has the tile's first 64 rows, warp 3 the others, four
-        // rows a lane: gathered one instruction a lane (they issue one after
-        // another, so two warps halve that time), and the lanes' scales.
-        // Otherwise warp 2 loads the rows (one box, or 16-row boxes one a
-        // lane) and warp 3 all scales, four rows a lane.
-        constexpr bool kGather = MODE == kGateUp;
-        const bool loads = kGather || warp == 2, scales = kGather || warp == 3;
-        const int r0 = kGather ? 64 * (warp - 2) + 4 * lane : 4 * lane;
-        const bool mine = !kGather || lane < 16;
-        sm100::fence_proxy_async_global();
-        uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
-        auto rows_of = [&](const Item &it, int (&row)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = it.row0 + min(r0 + i, it.count - 1);
-                row[i] = kGather ? P.row_token[r] : r;
+        auto next_stage = [&] {
+            if (++stage == S::kStages) {
+                stage = 0;
+                phase ^= 1;
             }
         };
-        const bool quads = kbs % 4 == 0 && (reinterpret_cast<uintptr_t>(P.row_scales) & 15) == 0 &&
-                           (reinterpret_cast<uintptr_t>(P.block_scales) & 15) == 0;
-        // the scales of groups kb .. kb + 3 to `slot`, on their way when this
-        // returns: up to kScaleSlots such requests are in flight
-        auto copy4 = [&](float4 *dst, const float *src, int kb) {
-            if (quads) {
-                copy_async<16>(dst, src + kb);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (kb + i < kbs) copy_async<4>(reinterpret_cast<float *>(dst) + i, src + kb + i);
-            }
-        };
-        auto request_scales = [&](const Item &it, const int (&row)[4], int kb) {
-            if (mine) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    copy4(&tail->row_scale[slot][r0 + i], P.row_scales + static_cast<int64_t>(row[i]) * kbs, kb);
-            }
-            // lanes 0 and 1: the item's two weight blocks (gate and up, or the
-            // two halves of the columns; one past the matrix is never used)
-            if (warp == 3 && lane < 2) {
-                int64_t blk;
-                if constexpr (MODE == kGateUp) {
-                    blk = static_cast<int64_t>(it.e) * 2 * nt + it.n + lane * nt;
+        if (warp == 0) {
+            // ---------------------------------------------- items, weight tiles
+            const uint64_t once = sm100::l2_evict_first_policy(), keep = sm100::l2_evict_normal_policy();
+            const bool one = sm100::elect_one();
+            bool ok = true;
+            int put_at = 0, fetched = 0;
+            // the next item, also handed to the other warps (one ahead of the
+            // item whose weights are being loaded)
+            auto fetch = [&]() {
+                if constexpr (LIN) {
+                    return take_item();
                 } else {
-                    const int per = fp8::groups(P.n);
-                    blk = static_cast<int64_t>(it.e) * per + min(2 * it.n + lane, per - 1);
+                    if (lane == 0) fetched = atomicAdd(P.work, 1);
+                    fetched = __shfl_sync(0xffffffffu, fetched, 0);
+                    const Item r = decode(fetched);
+                    const int slot = put_at % kRing;
+                    ok = wait_warp(&tail->iempty[slot], ((put_at / kRing) & 1) ^ 1, abort);
+                    if (lane == 0) {
+                        tail->ring[slot][0] = make_int4(r.phase, r.e, r.row0, r.count);
+                        tail->ring[slot][1] = make_int4(r.n, r.mt, 0, 0);
+                        sm100::mbar_arrive(&tail->ifull[slot]);
+                    }
+                    __syncwarp();
+                    ++put_at;
+                    return r;
                 }
-                copy4(&tail->block_scale[slot][lane], P.block_scales + blk * kbs, kb);
-            }
-            copy_async_arrive(&tail->sfull[slot]);
-        };
-        int item = blockIdx.x;
-        Item next{};
-        int next_row[4] = {};
-        if (item < total) {
-            next = decode<MODE>(P, tail, item);
-            rows_of(next, next_row);
-        }
-        bool ok = true;
-        for (; ok && item < total; item += gridDim.x) {
-            const Item it = next;
-            int row[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) row[i] = next_row[i];
-            const bool more = item + static_cast<int>(gridDim.x) < total;
-            if (more) {
-                next = decode<MODE>(P, tail, item + gridDim.x);
-                rows_of(next, next_row);
-            }
-            // lanes that load, and what a lane loads
-            const int boxes = kGather ? min(16, (max(0, it.count - 64 * (warp - 2)) + 3) / 4)
-                                      : it.count == kBM ? 1 : (it.count + 15) / 16;
-            const int box_bytes = kGather ? 4 * kGroup : it.count == kBM ? kATile : 16 * kGroup;
-            for (int kb = 0; kb < kbs; ++kb) {
-                if (scales && (kb & 3) == 0) {
-                    ok = __all_sync(0xffffffffu, wait_bar(&tail->sempty[slot], sphase ^ 1, abort));
+            };
+            Item next = fetch();
+            while (ok && next.phase) {
+                const Item it = next;
+                next = fetch();
+                if (!ok) break;
+                const bool p1 = !LIN && it.phase == 1;
+                const uint64_t policy = it.mt > 1 ? keep : once;  // other tiles read the same weight rows
+                const int kbs = p1 ? kbs1 : kbs2;
+                const int r0 = it.n * (p1 ? kGroup : kBN), r1 = p1 ? P.inner + r0 : r0 + 128;
+                for (int kb = 0; kb < kbs; ++kb) {
+                    ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
                     if (!ok) break;
-                    request_scales(it, row, kb);
-                    if (++slot == kScaleSlots) {
-                        slot = 0;
-                        sphase ^= 1;
+                    uint8_t *b = smem + stage * S::kStage;
+                    uint64_t *bar = &tail->full[stage];
+                    if (one) {
+                        sm100::mbar_expect_tx(bar, kBTile);
+                        if constexpr (LIN) {
+                            sm100::tma_load_2d_hint(b, &tm_w, bar, kb * kGroup, r0, policy);
+                            sm100::tma_load_2d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, policy);
+                        } else if (p1) {
+                            sm100::tma_load_3d_hint(b, &tm_w, bar, kb * kGroup, r0, it.e, policy);
+                            sm100::tma_load_3d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, it.e, policy);
+                        } else {
+                            sm100::tma_load_3d_hint(b, &tm_w2, bar, kb * kGroup, r0, it.e, policy);
+                            sm100::tma_load_3d_hint(b + kBTile / 2, &tm_w2, bar, kb * kGroup, r1, it.e, policy);
+                        }
+                    }
+                    __syncwarp();
+                    next_stage();
+                }
+            }
+        } else if (warp == 1) {
+            // ----------------------------------------------------- MMA issuer
+            const bool one = sm100::elect_one();
+            uint32_t buf = 0, bphase = 0;
+            bool ok = true, any = false;
+            for (Item it = take_item(); ok && it.phase; it = take_item()) {
+                const int kbs = !LIN && it.phase == 1 ? kbs1 : kbs2;
+                const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kSwap ? (it.count + 15) & ~15 : kBN);
+                for (int kb = 0; kb < kbs; ++kb) {
+                    ok = wait_bar(&tail->tempty[buf], bphase ^ 1, abort) && wait_bar(&tail->full[stage], phase, abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    sm100::tc_fence_after();
+                    const uint32_t base = sm100::smem_u32(smem + stage * S::kStage), d = tmem + buf * S::kBufCols;
+                    const uint64_t w = sm100::desc_kmajor_sw128(base), w1 = sm100::desc_kmajor_sw128(base + kBTile / 2);
+                    const uint64_t r = sm100::desc_kmajor_sw128(base + kBTile);
+                    if (one) {
+                        if constexpr (kSwap) {
+                            sm100::mma_e4m3<false>(d, w, r, idesc);
+                            sm100::mma_e4m3<false>(d + BN, w1, r, idesc);
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) {
+                                sm100::mma_e4m3<true>(d, w + 2 * kk, r + 2 * kk, idesc);
+                                sm100::mma_e4m3<true>(d + BN, w1 + 2 * kk, r + 2 * kk, idesc);
+                            }
+                        } else {
+                            sm100::mma_e4m3<false>(d, r, w, idesc);
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) sm100::mma_e4m3<true>(d, r + 2 * kk, w + 2 * kk, idesc);
+                        }
+                        sm100::mma_commit(&tail->tfull[buf]);
+                        sm100::mma_commit(&tail->empty[stage]);
+                    }
+                    __syncwarp();
+                    any = true;
+                    next_stage();
+                    if (++buf == S::kBufs) {
+                        buf = 0;
+                        bphase ^= 1;
                     }
                 }
-                if (!loads) continue;
-                ok = __all_sync(0xffffffffu, wait_bar(&tail->empty[stage], phase ^ 1, abort));
-                if (!ok) break;
-                uint8_t *a = smem + stage * kStage;
-                uint64_t *bar = &tail->full[stage];
-                if (lane == 0) sm100::mbar_expect_tx(bar, boxes * box_bytes);
-                __syncwarp();
-                if (lane < boxes) {
-                    if constexpr (kGather)
-                        sm100::tma_gather4(a + (r0 - 4 * lane) * kGroup + lane * box_bytes, &tm_x, bar, kb * kGroup,
-                                           row);
-                    else
-                        sm100::tma_load_2d(a + lane * box_bytes, it.count == kBM ? &tm_x : &tm_x16, bar, kb * kGroup,
-                                           it.row0 + lane * 16);
-                }
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
+            }
+            if (*abort && any) {
+                if (one) sm100::mma_commit(&tail->drain);
+                const uint64_t t0 = now_ns();
+                while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
                 }
             }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      } else if (warp == 1) {
-        // --------------------------------------------------------- MMA issuer
-        constexpr uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
-        const bool one = sm100::elect_one();
-        uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
-        bool ok = true, any = false;
-        for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-            for (int kb = 0; kb < kbs; ++kb) {
-                ok = wait_bar(&tail->tempty[buf], bphase ^ 1, abort) && wait_bar(&tail->full[stage], phase, abort);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                sm100::tc_fence_after();
-                const uint32_t base = sm100::smem_u32(smem + stage * kStage), d = tmem + buf * kBN;
-                const uint64_t a = sm100::desc_kmajor_sw128(base), b = sm100::desc_kmajor_sw128(base + kATile);
-                if (one) {
-                    sm100::mma_e4m3<false>(d, a, b, idesc);
-                    sm100::mma_e4m3<true>(d, a + 2, b + 2, idesc);
-                    sm100::mma_e4m3<true>(d, a + 4, b + 4, idesc);
-                    sm100::mma_e4m3<true>(d, a + 6, b + 6, idesc);
-                    sm100::mma_commit(&tail->tfull[buf]);
-                    sm100::mma_commit(&tail->empty[stage]);
+            __syncwarp();
+        } else {
+            // --------------------------------------------- row tiles, scales
+            // Warp 2 loads the rows: gathered four a lane, or one box, or
+            // boxes of 16 rows one a lane.  Warp 3 requests the scales, and
+            // with 128-row tiles gathers the second 64 rows: a warp's lanes
+            // issue their gathers one after another, two warps halve that time.
+            sm100::fence_proxy_async_global();
+            constexpr int kPerWarp = kRows / kGatherWarps;  // gathered rows of a warp
+            const int g0 = kPerWarp * (warp - 2) + 4 * lane;
+            uint32_t slot = 0, sphase = 0;
+            // warp 3, lane l: the scales of rows l, l + 32, ... of the tile
+            constexpr int kScaleRows = (kRows + 31) / 32;
+            auto copy4 = [&](float *dst, int step, const float *src, int kb, int kbs, bool quads) {
+                if (quads && step == 1) {
+                    copy_async<16>(dst, src + kb);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (kb + i < kbs) copy_async<4>(dst + i * step, src + kb + i);
                 }
-                __syncwarp();
-                any = true;
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
+            };
+            Item next = take_item();
+            int next_gather[4] = {}, next_scaled[kScaleRows] = {};
+            auto rows_of = [&](const Item &it) {
+                if (!it.phase) return;
+                const bool p1 = !LIN && it.phase == 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (p1) next_gather[i] = P.row_token[it.row0 + min(g0 + i, it.count - 1)];
+#pragma unroll
+                for (int j = 0; j < kScaleRows; ++j) {
+                    const int r = it.row0 + min(lane + 32 * j, it.count - 1);
+                    next_scaled[j] = p1 ? (warp == 3 ? P.row_token[r] : 0) : r;
                 }
-                buf ^= 1;
-                bphase ^= buf == 0;
+            };
+            rows_of(next);
+            bool ok = true;
+            while (ok && next.phase) {
+                const Item it = next;
+                int gather[4], scaled[kScaleRows];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gather[i] = next_gather[i];
+#pragma unroll
+                for (int j = 0; j < kScaleRows; ++j) scaled[j] = next_scaled[j];
+                next = take_item();
+                rows_of(next);
+                const bool p1 = !LIN && it.phase == 1;
+                const int kbs = p1 ? kbs1 : kbs2;
+                const float *rs = LIN || p1 ? P.x_scales : P.act_scales_in;
+                const float *bs = LIN || p1 ? P.w_scales : P.down_scales;
+                const bool quads = kbs % 4 == 0 && ((reinterpret_cast<uintptr_t>(rs) | reinterpret_cast<uintptr_t>(bs)) & 15) == 0;
+                if (!LIN && !p1) {
+                    // the expert's activations: every epilogue warp of its phase-1 items
+                    const int need = 8 * nt1 * it.mt;
+                    const uint64_t t0 = now_ns();
+                    while (sm100::ld_acquire(P.done + it.e) < need) {
+                        if (*abort || now_ns() - t0 > kWaitNs) {
+                            *abort = 1;
+                            break;
+                        }
+                        __nanosleep(32);
+                    }
+                    ok = __all_sync(0xffffffffu, !*abort);
+                    if (!ok) break;
+                    sm100::fence_proxy_async_global();
+                }
+                const bool loads = warp == 2 || (p1 && kGatherWarps == 2);
+                // lanes that load, and what a lane loads
+                const int boxes = p1 ? min(kPerWarp / 4, (max(0, it.count - kPerWarp * (warp - 2)) + 3) / 4)
+                                     : it.count == kRows ? 1 : (it.count + 15) / 16;
+                const int box_bytes = p1 ? 4 * kGroup : it.count == kRows ? S::kATile : 16 * kGroup;
+                for (int kb = 0; kb < kbs; ++kb) {
+                    if (warp == 3 && (kb & 3) == 0) {
+                        // the scales of groups kb .. kb + 3, on their way from here
+                        ok = wait_warp(&tail->sempty[slot], sphase ^ 1, abort);
+                        if (!ok) break;
+#pragma unroll
+                        for (int j = 0; j < kScaleRows; ++j) {
+                            const int r = lane + 32 * j;
+                            if (r < kRows)
+                                copy4(&tail->row_scale[slot][kSwap ? r : 4 * r], kSwap ? kRows : 1,
+                                      rs + static_cast<int64_t>(scaled[j]) * kbs, kb, kbs, quads);
+                        }
+                        // lanes 0 and 1: the item's two weight blocks (gate and
+                        // up, or the two halves of the 256 weight rows; one
+                        // past the matrix is never used)
+                        if (lane < 2) {
+                            const int per = fp8::groups(n2);
+                            const int64_t blk = p1 ? static_cast<int64_t>(it.e) * 2 * nt1 + it.n + lane * nt1
+                                                   : static_cast<int64_t>(it.e) * per + min(2 * it.n + lane, per - 1);
+                            copy4(&tail->block_scale[slot][lane].x, 1, bs + blk * kbs, kb, kbs, quads);
+                        }
+                        copy_async_arrive(&tail->sfull[slot]);
+                        if (++slot == kScaleSlots) {
+                            slot = 0;
+                            sphase ^= 1;
+                        }
+                    }
+                    if (warp == 3 && (LIN || kGatherWarps == 1)) continue;
+                    ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
+                    if (!ok) break;
+                    uint8_t *a = smem + stage * S::kStage + kBTile;
+                    uint64_t *bar = &tail->full[stage];
+                    if (lane == 0) {
+                        if (loads) sm100::mbar_expect_tx(bar, boxes * box_bytes);
+                        else sm100::mbar_arrive(bar);
+                    }
+                    __syncwarp();
+                    if (loads && lane < boxes) {
+                        if (p1) sm100::tma_gather4(a + g0 * kGroup, &tm_x, bar, kb * kGroup, gather);
+                        else sm100::tma_load_2d(a + lane * box_bytes, it.count == kRows ? &tm_r : &tm_r16, bar,
+                                                kb * kGroup, it.row0 + lane * 16);
+                    }
+                    next_stage();
+                }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        if (*abort && any) {
-            if (one) sm100::mma_commit(&tail->drain);
-            const uint64_t t0 = now_ns();
-            while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
-            }
-        }
-        __syncwarp();
-      }
     } else {
         // ----------------------------------------------------------- epilogue
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-        const int q = warp & 3, h = warp >= 8;  // TMEM lanes 32q.., half of the columns
-        const int r = 32 * q + lane;
+        const int q = warp & 3, h = warp >= 8;  // TMEM lanes 32q..; half of the columns
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * q) << 16);
-        uint8_t *piece = pieces + (warp - 4) * kPiece;
         uint32_t slot = 0, sphase = 0, buf = 0, bphase = 0, iphase = 0;
-        // the factors of the next four groups: row scale x weight scale (gate's and up's)
-        float s0[4], s1[4];
-        auto take_scales = [&] {
-            wait_bar(&tail->sfull[slot], sphase, abort);
-            const float4 rs = tail->row_scale[slot][r];
-            const float4 b0 = tail->block_scale[slot][MODE == kGateUp ? 0 : h];
-            s0[0] = rs.x * b0.x, s0[1] = rs.y * b0.y, s0[2] = rs.z * b0.z, s0[3] = rs.w * b0.w;
-            if constexpr (MODE == kGateUp) {
-                const float4 b1 = tail->block_scale[slot][1];
-                s1[0] = rs.x * b1.x, s1[1] = rs.y * b1.y, s1[2] = rs.z * b1.z, s1[3] = rs.w * b1.w;
+        auto next_buf = [&] {
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&tail->tempty[buf]);
+            if (++buf == S::kBufs) {
+                buf = 0;
+                bphase ^= 1;
             }
+        };
+        auto next_slot = [&] {
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&tail->sempty[slot]);
             if (++slot == kScaleSlots) {
@@ -484,129 +630,247 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sphase ^= 1;
             }
         };
-        for (int item = blockIdx.x; item < total; item += gridDim.x) {
-            const Item it = decode<MODE>(P, tail, item);
-            const bool active = 32 * q < it.count;  // the warp has rows of the tile
-            float acc[128];
+        // this warp's part of a phase-1 item is stored
+        auto count_in = [&](const Item &it) {
+            __syncwarp();
+            if (lane == 0) {
+                __threadfence();
+                atomicAdd(P.done + it.e, 1);
+            }
+        };
+        if constexpr (kSwap) {
+            // This warp: weight rows 32q + lane of both blocks, rows NJ h .. of the tile.
+            constexpr int NJ = BN / 2, NL = NJ < 16 ? NJ : 16;
+            const int j0 = NJ * h;
+            for (Item it = take_item(); it.phase; it = take_item()) {
+                const bool p1 = !LIN && it.phase == 1;
+                const int kbs = p1 ? kbs1 : kbs2;
+                const bool active = j0 < it.count;
+                float acc0[NJ], acc1[NJ];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-            take_scales();
-            for (int kb = 0; kb < kbs; ++kb) {
-                const float g0 = s0[0], g1 = MODE == kGateUp ? s1[0] : s0[0];
+                for (int j = 0; j < NJ; ++j) acc0[j] = acc1[j] = 0.f;
+                for (int kb = 0; kb < kbs; ++kb) {
+                    if ((kb & 3) == 0) wait_bar(&tail->sfull[slot], sphase, abort);
+                    const float b0 = reinterpret_cast<const float *>(&tail->block_scale[slot][0])[kb & 3];
+                    const float b1 = reinterpret_cast<const float *>(&tail->block_scale[slot][1])[kb & 3];
+                    wait_bar(&tail->tfull[buf], bphase, abort);
+                    sm100::tc_fence_after();
+                    if (active) {
+                        const uint32_t at = lanes + buf * S::kBufCols + j0;
 #pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    s0[i] = s0[i + 1];
-                    if (MODE == kGateUp) s1[i] = s1[i + 1];
+                        for (int c = 0; c < NJ; c += NL) {
+                            float t0[NL], t1[NL], s[NL];
+                            load_cols<NL>(at + c, t0);
+                            load_cols<NL>(at + BN + c, t1);
+#pragma unroll
+                            for (int j = 0; j < NL; j += 4)
+                                *reinterpret_cast<float4 *>(&s[j]) = *reinterpret_cast<const float4 *>(
+                                    &tail->row_scale[slot][(kb & 3) * kRows + j0 + c + j]);
+                            wait_cols(t0);
+                            wait_cols(t1);
+#pragma unroll
+                            for (int j = 0; j < NL; ++j) {
+                                acc0[c + j] = fmaf(t0[j], s[j] * b0, acc0[c + j]);
+                                acc1[c + j] = fmaf(t1[j], s[j] * b1, acc1[c + j]);
+                            }
+                        }
+                    }
+                    next_buf();
+                    if ((kb & 3) == 3 || kb + 1 == kbs) next_slot();
                 }
-                const bool refill = (kb & 3) == 3 && kb + 1 < kbs;
-                wait_bar(&tail->tfull[buf], bphase, abort);
-                sm100::tc_fence_after();
-                if (active) {
-                    // 16 columns at a time; gate/up: 64 of the gate block, then
-                    // the same 64 of the up block
-                    const uint32_t base = lanes + buf * kBN;
-                    auto col = [&](int c) {
-                        return MODE == kGateUp ? base + 64 * h + 16 * (c & 3) + (c >= 4 ? 128 : 0)
-                                               : base + 128 * h + 16 * c;
-                    };
-                    float t[2][16];
-                    sm100::tmem_ld16(col(0), t[0]);
-                    if (refill) take_scales();
-                    wait_ld16(t[0]);
+                const int left = it.count - j0;  // rows of this warp, if below NJ
+                if (p1) {
+                    if (active) {
+                        // |h| over the 128 lanes of the block: bit patterns of
+                        // magnitudes order like the values, NaN above all
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (c < 7) sm100::tmem_ld16(col(c + 1), t[(c + 1) & 1]);
+                        for (int j = 0; j < NJ; ++j) {
+                            acc0[j] = silu_fast(acc0[j]) * acc1[j];
+                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(acc0[j])));
+                            if (lane == (j & 31)) tail->top[iphase][q][j0 + j] = __uint_as_float(m);
+                        }
+                        __syncwarp();
+                        if (lane == 0) sm100::mbar_arrive(&tail->half[h]);
+                        wait_bar(&tail->half[h], iphase, abort);
+                        uint8_t *dst = P.act + static_cast<int64_t>(it.row0 + j0) * P.inner + it.n * kGroup + 32 * q + lane;
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) {
+                            float top = fp8::kTiny;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) top = fp8::max_nan(top, tail->top[iphase][i][j0 + j]);
+                            const fp8::Divisor f(top);
+                            if (j < left) {
+                                dst[static_cast<int64_t>(j) * P.inner] = static_cast<uint8_t>(fp8::pack2(f(acc0[j]), 0.f));
+                                if (q == 0 && lane == (j & 31))
+                                    P.act_scales[static_cast<int64_t>(it.row0 + j0 + j) * nt1 + it.n] = fp8::scale_of(top);
+                            }
+                        }
+                        iphase ^= 1;
+                    }
+                    count_in(it);
+                } else if (active) {
+                    const int c0 = it.n * kBN + 32 * q + lane;
+                    const bool f32 = LIN && P.out_f32;
+                    const int64_t at = static_cast<int64_t>(it.row0 + j0) * n2 + c0;
+                    uint16_t *y = (LIN ? static_cast<uint16_t *>(P.out) : P.y) + at;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if (j >= left) break;
+                        const int64_t o = static_cast<int64_t>(j) * n2;
+                        if (f32) {
+                            float *z = static_cast<float *>(P.out) + at;
+                            if (c0 < n2) z[o] = acc0[j];
+                            if (c0 + 128 < n2) z[o + 128] = acc1[j];
+                        } else {
+                            if (c0 < n2) y[o] = f2bf(acc0[j]);
+                            if (c0 + 128 < n2) y[o + 128] = f2bf(acc1[j]);
+                        }
+                    }
+                }
+            }
+        } else {
+            const int r = 32 * q + lane;
+            uint8_t *piece = pieces + (warp - 4) * S::kPiece;
+            // the factors of the next four groups: row scale x weight scale (gate's and up's)
+            float s0[4], s1[4];
+            auto take_scales = [&](bool p1) {
+                wait_bar(&tail->sfull[slot], sphase, abort);
+                const float4 rs = *reinterpret_cast<const float4 *>(&tail->row_scale[slot][4 * r]);
+                const float4 b0 = tail->block_scale[slot][p1 ? 0 : h];
+                s0[0] = rs.x * b0.x, s0[1] = rs.y * b0.y, s0[2] = rs.z * b0.z, s0[3] = rs.w * b0.w;
+                if constexpr (!LIN) {
+                    const float4 b1 = tail->block_scale[slot][p1 ? 1 : h];
+                    s1[0] = rs.x * b1.x, s1[1] = rs.y * b1.y, s1[2] = rs.z * b1.z, s1[3] = rs.w * b1.w;
+                }
+                next_slot();
+            };
+            Item next = take_item();
+            bool ready = false;  // s0 and s1 are the next item's
+            while (next.phase) {
+                const Item it = next;
+                const bool p1 = !LIN && it.phase == 1;
+                const int kbs = p1 ? kbs1 : kbs2;
+                const bool active = 32 * q < it.count;  // the warp has rows of the tile
+                float acc[128];
+#pragma unroll
+                for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+                if (!ready) take_scales(p1);
+                ready = false;
+                // 16 columns at a time; gate/up: 64 of the gate block, then the
+                // same 64 of the up block
+                const uint32_t at = lanes + (p1 ? 64 * h : 128 * h), skip = p1 ? 64 : 0;
+                for (int kb = 0; kb < kbs; ++kb) {
+                    const float g0 = s0[0], g1 = LIN ? s0[0] : s1[0];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        s0[i] = s0[i + 1];
+                        if (!LIN) s1[i] = s1[i + 1];
+                    }
+                    wait_bar(&tail->tfull[buf], bphase, abort);
+                    sm100::tc_fence_after();
+                    if (active) {
+                        const uint32_t base = at + buf * kBN;
+                        float t[2][16];
+                        load_cols<16>(base, t[0]);
+                        wait_cols(t[0]);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            if (c < 7) load_cols<16>(base + 16 * (c + 1) + (c >= 3 ? skip : 0), t[(c + 1) & 1]);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                acc[16 * c + i] = fmaf(t[c & 1][i], c < 4 ? g0 : g1, acc[16 * c + i]);
+                            if (c < 7) wait_cols(t[(c + 1) & 1]);
+                        }
+                    }
+                    next_buf();
+                    // behind the buffer's release: the products go on meanwhile
+                    if ((kb & 3) == 3 && kb + 1 < kbs) take_scales(p1);
+                }
+                // The next item's first factors, before this one is stored --
+                // unless they may be waiting for this very item's rows.
+                next = take_item();
+                if (next.phase && (LIN || next.phase == it.phase)) {
+                    take_scales(!LIN && next.phase == 1);
+                    ready = true;
+                }
+                const int rows = it.count - 32 * q;  // of this warp, if below 32
+                const int64_t first = static_cast<int64_t>(it.row0) + 32 * q;
+                if (p1) {
+                    if (active) {
+                        float top = fp8::kTiny;
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) {
+                            acc[i] = silu_fast(acc[i]) * acc[64 + i];
+                            top = fp8::max_nan(top, fabsf(acc[i]));
+                        }
+                        // the group's other 64 columns are the other half's
+                        tail->top[iphase][h][r] = top;
+                        __syncwarp();
+                        if (lane == 0) sm100::mbar_arrive(&tail->half[q]);
+                        wait_bar(&tail->half[q], iphase, abort);
+                        top = fp8::max_nan(top, tail->top[iphase][h ^ 1][r]);
+                        iphase ^= 1;
+                        const fp8::Divisor f(top);
+                        uint32_t v[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            acc[16 * c + i] = fmaf(t[c & 1][i], c < 4 ? g0 : g1, acc[16 * c + i]);
-                        if (c < 7) wait_ld16(t[(c + 1) & 1]);
+                            v[i] = fp8::pack4(f, acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+                        store_rows64(piece, v, P.act + first * P.inner + it.n * kGroup + 64 * h, P.inner, rows, 4);
+                        if (h == 0 && lane < rows) P.act_scales[(first + lane) * nt1 + it.n] = fp8::scale_of(top);
                     }
-                } else if (refill) {
-                    take_scales();
-                }
-                sm100::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) sm100::mbar_arrive(&tail->tempty[buf]);
-                buf ^= 1;
-                bphase ^= buf == 0;
-            }
-            if (!active) continue;
-            const int rows = it.count - 32 * q;  // of this warp, if below 32
-            const int64_t first = static_cast<int64_t>(it.row0) + 32 * q;
-            if constexpr (MODE == kGateUp) {
-                float top = fp8::kTiny;
+                    count_in(it);
+                } else if (active) {
+                    const int n0 = it.n * kBN + 128 * h;
+                    const bool f32 = LIN && P.out_f32;
+                    // whole 16-byte units: 8 BF16 or 4 FP32 columns, all or none
+                    // of them there (the experts' H is a multiple of 16)
+                    const bool vec = !LIN || n2 % (f32 ? 4 : 8) == 0;
+                    if (LIN && vec && !f32) {
+                        // the map cuts rows and columns past the matrix
+                        if (lane == 0) sm100::bulk_wait_read();  // the last item's stores have left the buffer
+                        __syncwarp();
+                        stage_row256(piece, acc);
+                        sm100::fence_proxy_async_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (n0 < n2) sm100::tma_store_2d(piece, &tm_out, n0, static_cast<int>(first));
+                            if (n0 + 64 < n2)
+                                sm100::tma_store_2d(piece + 4096, &tm_out, n0 + 64, static_cast<int>(first));
+                            sm100::bulk_commit();
+                        }
+                    } else if (!LIN) {
+                        uint16_t *dst = P.y + first * n2 + n0;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    acc[i] = silu_fast(acc[i]) * acc[64 + i];
-                    top = fp8::max_nan(top, fabsf(acc[i]));
-                }
-                // the group's other 64 columns are the other half's
-                tail->top[iphase][h][r] = top;
-                __syncwarp();
-                if (lane == 0) sm100::mbar_arrive(&tail->half[q]);
-                wait_bar(&tail->half[q], iphase, abort);
-                top = fp8::max_nan(top, tail->top[iphase][h ^ 1][r]);
-                iphase ^= 1;
-                const fp8::Divisor f(top);
-                uint32_t v[16];
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    v[i] = fp8::pack4(f, acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-                store_rows64(piece, v, P.act + first * P.n + it.n * kGroup + 64 * h, P.n, rows, 4);
-                if (h == 0 && lane < rows) P.act_scales[(first + lane) * nt + it.n] = fp8::scale_of(top);
-            } else {
-                const int n0 = it.n * kBN + 128 * h;
-                const bool f32 = MODE == kLinear && P.out_f32;
-                // whole 16-byte units: 8 BF16 or 4 FP32 columns, all or none of
-                // them there (the down product's H is a multiple of 16)
-                const bool vec = MODE == kDown || P.n % (f32 ? 4 : 8) == 0;
-                if (vec && !f32 && (MODE == kLinear || rows >= 32)) {
-                    // The map cuts rows and columns past the matrix; another
-                    // expert's rows below a partial tile must not be written,
-                    // so those take the other way.
-                    if (lane == 0) sm100::bulk_wait_read();  // the last item's stores have left the buffer
-                    __syncwarp();
-                    stage_row256(piece, acc);
-                    sm100::fence_proxy_async_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (n0 < P.n) sm100::tma_store_2d(piece, &tm_out, n0, static_cast<int>(first));
-                        if (n0 + 64 < P.n) sm100::tma_store_2d(piece + 4096, &tm_out, n0 + 64, static_cast<int>(first));
-                        sm100::bulk_commit();
-                    }
-                } else if (vec && !f32) {
-                    if (lane == 0) sm100::bulk_wait_read();
-                    uint16_t *dst = static_cast<uint16_t *>(P.out) + first * P.n + n0;
+                            for (int i = 0; i < 16; ++i) v[i] = fp8::pack_bf16(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]);
+                            store_rows64(piece, v, reinterpret_cast<uint8_t *>(dst + 32 * c), 2 * static_cast<int64_t>(n2),
+                                         rows, (n2 - n0 - 32 * c) / 8);
+                        }
+                    } else if (vec) {
+                        float *dst = static_cast<float *>(P.out) + first * n2 + n0;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[16];
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t v[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = fp8::pack_bf16(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]);
-                        store_rows64(piece + 2048 * c, v, reinterpret_cast<uint8_t *>(dst + 32 * c),
-                                     2 * static_cast<int64_t>(P.n), rows, (P.n - n0 - 32 * c) / 8);
-                    }
-                } else if (vec) {
-                    float *dst = static_cast<float *>(P.out) + first * P.n + n0;
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(acc[16 * c + i]);
+                            store_rows64(piece + 2048 * (c & 3), v, reinterpret_cast<uint8_t *>(dst + 16 * c),
+                                         4 * static_cast<int64_t>(n2), rows, (n2 - n0 - 16 * c) / 4);
+                        }
+                    } else if (lane < rows) {
+                        const int64_t o = (first + lane) * n2 + n0;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t v[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(acc[16 * c + i]);
-                        store_rows64(piece + 2048 * (c & 3), v, reinterpret_cast<uint8_t *>(dst + 16 * c),
-                                     4 * static_cast<int64_t>(P.n), rows, (P.n - n0 - 16 * c) / 4);
-                    }
-                } else if (lane < rows) {
-                    const int64_t at = (first + lane) * P.n + n0;
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) {
-                        if (n0 + i >= P.n) continue;
-                        if (f32) static_cast<float *>(P.out)[at + i] = acc[i];
-                        else static_cast<uint16_t *>(P.out)[at + i] = f2bf(acc[i]);
+                        for (int i = 0; i < 128; ++i) {
+                            if (n0 + i >= n2) continue;
+                            if (f32) static_cast<float *>(P.out)[o + i] = acc[i];
+                            else static_cast<uint16_t *>(P.out)[o + i] = f2bf(acc[i]);
+                        }
                     }
                 }
             }
+            if (LIN && lane == 0) sm100::bulk_wait_all();
         }
-        if (lane == 0) sm100::bulk_wait_all();
         __syncwarp();
         sm100::tc_fence_before();
     }
@@ -622,6 +886,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tmem_dealloc(tmem, 512);
     }
     if (threadIdx.x == 0 && *abort && P.status) atomicExch(P.status, 1);
+}
+
+// The experts' plan for up to kPlanRoutes routes, one a thread: routes in order
+// of (expert, token, slot).  A route's place among its expert's routes is its
+// rank among the equal ids of its warp plus the warps' counts before it.  Also
+// zeroes the tile kernel's counters.
+constexpr int kPlanRoutes = 1024;
+__global__ void __launch_bounds__(kPlanRoutes) fp8_plan_kernel(const int64_t *__restrict__ idx, int routes, int top_k,
+                                                               int experts, int32_t *__restrict__ offsets,
+                                                               int32_t *__restrict__ row_token,
+                                                               int32_t *__restrict__ route_pos,
+                                                               int32_t *__restrict__ counters) {
+    extern __shared__ uint8_t warp_count[];  // [warps][experts]
+    __shared__ int32_t begin[kMaxExperts], scan[32];
+    const int r = threadIdx.x, lane = r & 31, warp = r >> 5, warps = blockDim.x >> 5;
+    for (int i = r; i < (warps * experts + 3) / 4; i += blockDim.x) reinterpret_cast<uint32_t *>(warp_count)[i] = 0;
+    grid_dependency_wait();
+    grid_dependency_trigger();
+    for (int i = r; i <= experts; i += blockDim.x) counters[i] = 0;
+    const int64_t id = r < routes ? idx[r] : -1;
+    const int e = id >= 0 && id < experts ? static_cast<int>(id) : -1;
+    __syncthreads();
+    const unsigned peers = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(peers & ((1u << lane) - 1));
+    if (e >= 0 && rank == 0) warp_count[warp * experts + e] = static_cast<uint8_t>(__popc(peers));
+    __syncthreads();
+    // expert x: its routes, then an exclusive scan over the experts
+    int base = 0;  // experts may exceed the threads: chunks of blockDim.x
+    for (int x0 = 0; x0 < experts; x0 += blockDim.x) {
+        const int x = x0 + r;
+        int count = 0;
+        if (x < experts)
+            for (int w = 0; w < warps; ++w) count += warp_count[w * experts + x];
+        int incl = count;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += v;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        int before = base, all = base;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) before += scan[w];
+            all += scan[w];
+        }
+        if (x < experts) {
+            begin[x] = offsets[x] = before + incl - count;
+            if (x == experts - 1) offsets[experts] = before + incl;
+        }
+        base = all;
+        __syncthreads();
+    }
+    if (r < routes) {
+        int pos = -1;
+        if (e >= 0) {
+            pos = begin[e] + rank;
+            for (int w = 0; w < warp; ++w) pos += warp_count[w * experts + e];
+            row_token[pos] = r / top_k;
+        }
+        route_pos[r] = pos;
+    }
 }
 
 // out[t] = sum over the token's routes, in slot order, of weight * row, in
@@ -665,18 +991,19 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const uint16_t *__rest
                    fp8::pack_bf16(acc[6], acc[7]));
 }
 
-template <int MODE>
-int launch_tile(const CUtensorMap &x, const CUtensorMap &x16, const CUtensorMap &w, const CUtensorMap &out,
-                const Params &P, int64_t items, cudaStream_t stream) {
-    if (int rc = ensure_dynamic_smem(fp8_tile_kernel<MODE>, kSmem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
-    return launch_pdl(fp8_tile_kernel<MODE>, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
-                      dim3(kThreads), kSmem, stream, "fp8_tile_kernel", x, x16, w, out, P);
+template <bool LIN, int BN>
+int launch_tile(const CUtensorMap (&m)[6], const Params &P, int64_t items, cudaStream_t stream) {
+    constexpr int smem = Shape<LIN, BN>::kSmem;
+    if (int rc = ensure_dynamic_smem(fp8_tile_kernel<LIN, BN>, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
+    return launch_pdl(fp8_tile_kernel<LIN, BN>, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
+                      dim3(kThreads), smem, stream, "fp8_tile_kernel", m[0], m[1], m[2], m[3], m[4], m[5], P);
 }
 
-int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int cols) {
+// Rows [rows, cols] in boxes of `full` and of 16 rows.
+int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int cols, int full) {
     const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(cols)};
-    if (int rc = make_map_u8(m, base, 2, dims, str, kBM)) return rc;
+    if (int rc = make_map_u8(m, base, 2, dims, str, full)) return rc;
     return make_map_u8(m16, base, 2, dims, str, 16);
 }
 
@@ -690,70 +1017,95 @@ int out_map(CUtensorMap *m, const void *base, int rows, int cols) {
 }  // namespace
 
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream) {
-    CUtensorMap x{}, x16{}, w{}, out{};
-    if (int rc = row_maps(&x, &x16, a.x, a.tokens, a.cols)) return rc;
+    const int bn = a.tokens <= 16 ? 16 : a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : 0;
+    CUtensorMap m[6]{};
+    if (int rc = row_maps(&m[1], &m[2], a.x, a.tokens, a.cols, bn ? bn : kBM)) return rc;
+    m[0] = m[1];
     const uint64_t dims[2] = {static_cast<uint64_t>(a.cols), static_cast<uint64_t>(a.rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(a.cols)};
-    if (int rc = make_map_u8(&w, a.w, 2, dims, str, 128)) return rc;
+    if (int rc = make_map_u8(&m[3], a.w, 2, dims, str, 128)) return rc;
+    m[4] = m[3];
+    m[5] = m[3];
     if (!a.out_f32 && a.rows % 8 == 0)
-        if (int rc = out_map(&out, a.out, a.tokens, a.rows)) return rc;
+        if (int rc = out_map(&m[5], a.out, a.tokens, a.rows)) return rc;
     Params P{};
-    P.row_scales = a.x_scales;
-    P.block_scales = a.w_scales;
+    P.x_scales = a.x_scales;
+    P.w_scales = a.w_scales;
     P.rows = a.tokens;
     P.n = a.rows;
     P.k = a.cols;
     P.out = a.out;
     P.out_f32 = a.out_f32;
     P.status = status;
-    const int64_t items = static_cast<int64_t>((a.tokens + kBM - 1) / kBM) * ((a.rows + kBN - 1) / kBN);
+    const int tile = bn ? bn : kBM;
+    const int64_t items = static_cast<int64_t>((a.tokens + tile - 1) / tile) * ((a.rows + kBN - 1) / kBN);
     LRB_REQUIRE(items < (1ll << 31), "moe_linear_fp8: too many tiles");
-    return launch_tile<kLinear>(x, x16, w, out, P, items, stream);
+    switch (bn) {
+        case 16: return launch_tile<true, 16>(m, P, items, stream);
+        case 32: return launch_tile<true, 32>(m, P, items, stream);
+        case 64: return launch_tile<true, 64>(m, P, items, stream);
+        default: return launch_tile<true, 0>(m, P, items, stream);
+    }
 }
 
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream) {
     const int routes = a.tokens * a.top_k;
-    if (int rc = launch_permute(a.idx, a.tokens, a.top_k, a.experts, s.offsets, s.perm_token, s.perm_slot, s.route_pos,
-                                s.active, s.counters, s.counters + 1, stream, s.hist))
-        return rc;
+    if (routes <= kPlanRoutes) {
+        const int threads = (routes + 31) / 32 * 32;
+        const int smem = (threads / 32 * a.experts + 3) / 4 * 4;
+        if (int rc = launch_pdl(fp8_plan_kernel, dim3(1), dim3(threads), smem, stream, "fp8_plan_kernel", a.idx, routes,
+                                a.top_k, a.experts, s.offsets, s.perm_token, s.route_pos, s.counters))
+            return rc;
+    } else {
+        LRB_CUDA(cudaMemsetAsync(s.counters, 0, sizeof(int32_t) * (a.experts + 1), stream));
+        if (int rc = launch_permute(a.idx, a.tokens, a.top_k, a.experts, s.offsets, s.perm_token, s.perm_slot,
+                                    s.route_pos, s.active, s.permute_counters, s.permute_counters + 1, stream, s.hist))
+            return rc;
+    }
+    // the row tile by the average rows of an expert
+    const int mean = routes / a.experts;
+    const int bn = mean <= 6 ? 16 : mean <= 16 ? 32 : mean <= 40 ? 64 : 0;
+    const int tile = bn ? bn : kBM;
     // at most one partial tile per expert beside the full ones
-    const int64_t tiles = std::min<int64_t>(a.experts, routes) + routes / kBM;
-    const int64_t nt1 = a.inner / kGroup, nt2 = (a.hidden + kBN - 1) / kBN;
-    LRB_REQUIRE(tiles * std::max(nt1, nt2) < (1ll << 31), "moe_experts_fp8: too many tiles");
-    CUtensorMap x{}, act{}, act16{}, gu{}, dn{}, y{};
+    const int64_t tiles = std::min<int64_t>(a.experts, routes) + routes / tile;
+    const int64_t items = tiles * (a.inner / kGroup + (a.hidden + kBN - 1) / kBN);
+    LRB_REQUIRE(items < (1ll << 31) - 65536, "moe_experts_fp8: too many tiles");
+    CUtensorMap m[6]{};
+    const uint64_t H = a.hidden, I = a.inner, E = a.experts, T = a.tokens;
     {
         // rows gathered four at a time: the map's box is one row
-        const uint64_t dims[2] = {static_cast<uint64_t>(a.hidden), static_cast<uint64_t>(a.tokens)};
-        const uint64_t str[1] = {static_cast<uint64_t>(a.hidden)};
-        if (int rc = make_map_u8(&x, a.x, 2, dims, str, 1)) return rc;
+        const uint64_t dims[2] = {H, T}, str[1] = {H};
+        if (int rc = make_map_u8(&m[0], a.x, 2, dims, str, 1)) return rc;
     }
-    if (int rc = row_maps(&act, &act16, s.act, routes, a.inner)) return rc;
-    if (int rc = out_map(&y, s.y, routes, a.hidden)) return rc;
-    {
-        const uint64_t H = a.hidden, I = a.inner, E = a.experts;
-        const uint64_t d1[3] = {H, 2 * I, E}, s1[2] = {H, 2 * I * H}, d2[3] = {I, H, E}, s2[2] = {I, H * I};
-        if (int rc = make_map_u8(&gu, a.gate_up, 3, d1, s1, 128)) return rc;
-        if (int rc = make_map_u8(&dn, a.down, 3, d2, s2, 128)) return rc;
-    }
+    if (int rc = row_maps(&m[1], &m[2], s.act, routes, a.inner, tile)) return rc;
+    const uint64_t d1[3] = {H, 2 * I, E}, s1[2] = {H, 2 * I * H}, d2[3] = {I, H, E}, s2[2] = {I, H * I};
+    if (int rc = make_map_u8(&m[3], a.gate_up, 3, d1, s1, 128)) return rc;
+    if (int rc = make_map_u8(&m[4], a.down, 3, d2, s2, 128)) return rc;
+    m[5] = m[4];
     Params P{};
+    P.x_scales = a.x_scales;
+    P.w_scales = a.gate_up_scales;
+    P.act_scales_in = s.act_scales;
+    P.down_scales = a.down_scales;
     P.offsets = s.offsets;
+    P.row_token = s.perm_token;
     P.experts = a.experts;
+    P.hidden = a.hidden;
+    P.inner = a.inner;
+    P.act = s.act;
+    P.act_scales = s.act_scales;
+    P.y = s.y;
+    P.work = s.counters;
+    P.done = s.counters + 1;
     P.status = status;
-    Params G = P;
-    G.row_scales = a.x_scales;
-    G.block_scales = a.gate_up_scales;
-    G.row_token = s.perm_token;
-    G.n = a.inner;
-    G.k = a.hidden;
-    G.act = s.act;
-    G.act_scales = s.act_scales;
-    if (int rc = launch_tile<kGateUp>(x, x, gu, y, G, tiles * nt1, stream)) return rc;
-    P.row_scales = s.act_scales;
-    P.block_scales = a.down_scales;
-    P.n = a.hidden;
-    P.k = a.inner;
-    P.out = s.y;
-    if (int rc = launch_tile<kDown>(act, act16, dn, y, P, tiles * nt2, stream)) return rc;
+    int rc = MOE_OK;
+    switch (bn) {
+        case 16: rc = launch_tile<false, 16>(m, P, items, stream); break;
+        case 32: rc = launch_tile<false, 32>(m, P, items, stream); break;
+        case 64: rc = launch_tile<false, 64>(m, P, items, stream); break;
+        default: rc = launch_tile<false, 0>(m, P, items, stream); break;
+    }
+    if (rc) return rc;
     const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 255) / 256;
     return launch_pdl(fp8_combine_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, stream,
                       "fp8_combine_kernel", static_cast<const uint16_t *>(s.y),

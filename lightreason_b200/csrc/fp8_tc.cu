@@ -17,7 +17,7 @@
 //    accumulator lane is one row, so a group's factor is one number per thread,
 //    gate and up of a column meet in one thread, and warps without rows of a
 //    partial tile skip.
-//  * BN = 16, 32, 64, weights as M: the two blocks of 128 weight rows against
+//  * BN = 16, 32 (64 for a plain product), weights as M: the two blocks of 128 weight rows against
 //    N = BN rows.  A lane is one weight row and the tile's few rows are its
 //    columns: at a few rows per expert all eight warps share the epilogue
 //    instead of one row's pair of warps doing it.
@@ -215,6 +215,14 @@ __device__ __forceinline__ void stage_row256(uint8_t *buf, const float (&acc)[12
                        fp8::pack_bf16(acc[8 * u + 4], acc[8 * u + 5]), fp8::pack_bf16(acc[8 * u + 6], acc[8 * u + 7]));
 }
 
+// 32 bytes to a 32-byte boundary: a whole sector, so that a lane can store its
+// own row's columns without staging.
+__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // tm_x: linear, the row tiles; experts, the token rows (gathered).  tm_r, tm_r16:
 // full and 16-row boxes of the rows of linear or phase 2.  tm_w, tm_w2: weights
 // of linear or phase 1, and of phase 2.  tm_out: linear's BF16 output.
@@ -332,12 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             r.phase = item < items1 ? 1 : 2;
             const int nt = r.phase == 1 ? nt1 : nt2;
             const int x = r.phase == 1 ? item : item - items1, u = x / nt;
-            int lo = 0, hi = P.experts;  // the expert with tiles[e] <= u < tiles[e + 1]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (tail->tiles[mid] <= u) lo = mid;
-                else hi = mid;
-            }
+            int lo = __popc(__ballot_sync(0xffffffffu, 32 * lane <= P.experts && tail->tiles[min(32 * lane, P.experts)] <= u));
+            lo = 32 * (lo - 1);
+            lo += __popc(__ballot_sync(0xffffffffu, lo + lane < P.experts && tail->tiles[min(lo + lane, P.experts)] <= u)) - 1;
             const int begin = P.offsets[lo], count = P.offsets[lo + 1] - begin;
             // the tiles of one weight tile are neighbours
             r.mt = (count + kRows - 1) / kRows;
@@ -367,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 r = Item{a.x, a.y, a.z, a.w, b.x, b.y};
             }
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&tail->iempty[slot]);
+            sm100::mbar_arrive_if(&tail->iempty[slot], lane == 0);
             ++take_at;
             return r;
         }
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 0) {
             // ---------------------------------------------- items, weight tiles
             const uint64_t once = sm100::l2_evict_first_policy(), keep = sm100::l2_evict_normal_policy();
-            const bool one = sm100::elect_one();
+            const uint32_t one = sm100::elect_one();
             bool ok = true;
             int put_at = 0, fetched = 0;
             // the next item, also handed to the other warps (one ahead of the
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 1) {
             // ----------------------------------------------------- MMA issuer
-            const bool one = sm100::elect_one();
+            const uint32_t one = sm100::elect_one();
             uint32_t buf = 0, bphase = 0;
             bool ok = true, any = false;
             for (Item it = take_item(); ok && it.phase; it = take_item()) {
@@ -456,23 +461,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t base = sm100::smem_u32(smem + stage * S::kStage), d = tmem + buf * S::kBufCols;
                     const uint64_t w = sm100::desc_kmajor_sw128(base), w1 = sm100::desc_kmajor_sw128(base + kBTile / 2);
                     const uint64_t r = sm100::desc_kmajor_sw128(base + kBTile);
-                    if (one) {
-                        if constexpr (kSwap) {
-                            sm100::mma_e4m3<false>(d, w, r, idesc);
-                            sm100::mma_e4m3<false>(d + BN, w1, r, idesc);
+                    if constexpr (kSwap) {
+                        sm100::mma_e4m3<false>(d, w, r, idesc, one);
+                        sm100::mma_e4m3<false>(d + BN, w1, r, idesc, one);
 #pragma unroll
-                            for (int kk = 1; kk < 4; ++kk) {
-                                sm100::mma_e4m3<true>(d, w + 2 * kk, r + 2 * kk, idesc);
-                                sm100::mma_e4m3<true>(d + BN, w1 + 2 * kk, r + 2 * kk, idesc);
-                            }
-                        } else {
-                            sm100::mma_e4m3<false>(d, r, w, idesc);
-#pragma unroll
-                            for (int kk = 1; kk < 4; ++kk) sm100::mma_e4m3<true>(d, r + 2 * kk, w + 2 * kk, idesc);
+                        for (int kk = 1; kk < 4; ++kk) {
+                            sm100::mma_e4m3<true>(d, w + 2 * kk, r + 2 * kk, idesc, one);
+                            sm100::mma_e4m3<true>(d + BN, w1 + 2 * kk, r + 2 * kk, idesc, one);
                         }
-                        sm100::mma_commit(&tail->tfull[buf]);
-                        sm100::mma_commit(&tail->empty[stage]);
+                    } else {
+                        sm100::mma_e4m3<false>(d, r, w, idesc, one);
+#pragma unroll
+                        for (int kk = 1; kk < 4; ++kk) sm100::mma_e4m3<true>(d, r + 2 * kk, w + 2 * kk, idesc, one);
                     }
+                    sm100::mma_commit_if(&tail->tfull[buf], one);
+                    sm100::mma_commit_if(&tail->empty[stage], one);
                     __syncwarp();
                     any = true;
                     next_stage();
@@ -616,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto next_buf = [&] {
             sm100::tc_fence_before();
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&tail->tempty[buf]);
+            sm100::mbar_arrive_if(&tail->tempty[buf], lane == 0);
             if (++buf == S::kBufs) {
                 buf = 0;
                 bphase ^= 1;
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto next_slot = [&] {
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&tail->sempty[slot]);
+            sm100::mbar_arrive_if(&tail->sempty[slot], lane == 0);
             if (++slot == kScaleSlots) {
                 slot = 0;
                 sphase ^= 1;
@@ -690,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (lane == (j & 31)) tail->top[iphase][q][j0 + j] = __uint_as_float(m);
                         }
                         __syncwarp();
-                        if (lane == 0) sm100::mbar_arrive(&tail->half[h]);
+                        sm100::mbar_arrive_if(&tail->half[h], lane == 0);
                         wait_bar(&tail->half[h], iphase, abort);
                         uint8_t *dst = P.act + static_cast<int64_t>(it.row0 + j0) * P.inner + it.n * kGroup + 32 * q + lane;
 #pragma unroll
@@ -806,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // the group's other 64 columns are the other half's
                         tail->top[iphase][h][r] = top;
                         __syncwarp();
-                        if (lane == 0) sm100::mbar_arrive(&tail->half[q]);
+                        sm100::mbar_arrive_if(&tail->half[q], lane == 0);
                         wait_bar(&tail->half[q], iphase, abort);
                         top = fp8::max_nan(top, tail->top[iphase][h ^ 1][r]);
                         iphase ^= 1;
@@ -839,14 +842,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                             sm100::bulk_commit();
                         }
                     } else if (!LIN) {
-                        uint16_t *dst = P.y + first * n2 + n0;
+                        uint16_t *dst = P.y + (first + lane) * n2 + n0;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t v[16];
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t v[8];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] = fp8::pack_bf16(acc[32 * c + 2 * i], acc[32 * c + 2 * i + 1]);
-                            store_rows64(piece, v, reinterpret_cast<uint8_t *>(dst + 32 * c), 2 * static_cast<int64_t>(n2),
-                                         rows, (n2 - n0 - 32 * c) / 8);
+                            for (int i = 0; i < 8; ++i) v[i] = fp8::pack_bf16(acc[16 * c + 2 * i], acc[16 * c + 2 * i + 1]);
+                            if (lane < rows && n0 + 16 * c < n2) store32(dst + 16 * c, v);
                         }
                     } else if (vec) {
                         float *dst = static_cast<float *>(P.out) + first * n2 + n0;
@@ -1062,9 +1064,12 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
                                     s.route_pos, s.active, s.permute_counters, s.permute_counters + 1, stream, s.hist))
             return rc;
     }
-    // the row tile by the average rows of an expert
+    // The row tile by the average rows of an expert (256 experts of 2048 x 512,
+    // top-8, us at 32 / 128 / 256 / 512 / 1024 tokens, so 1 / 4 / 8 / 16 / 32
+    // rows: tiles of 16 86 / 125 / 154 / 190 / 268, of 32 88 / 123 / 148 / 168 /
+    // 205, rows as M 94 / 133 / 156 / 168 / 178).
     const int mean = routes / a.experts;
-    const int bn = mean <= 6 ? 16 : mean <= 16 ? 32 : mean <= 40 ? 64 : 0;
+    const int bn = mean < 4 ? 16 : mean < 16 ? 32 : 0;
     const int tile = bn ? bn : kBM;
     // at most one partial tile per expert beside the full ones
     const int64_t tiles = std::min<int64_t>(a.experts, routes) + routes / tile;
@@ -1102,7 +1107,6 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     switch (bn) {
         case 16: rc = launch_tile<false, 16>(m, P, items, stream); break;
         case 32: rc = launch_tile<false, 32>(m, P, items, stream); break;
-        case 64: rc = launch_tile<false, 64>(m, P, items, stream); break;
         default: rc = launch_tile<false, 0>(m, P, items, stream); break;
     }
     if (rc) return rc;

@@ -21,7 +21,7 @@ the caller keeps.
 
 from __future__ import annotations
 
-import contextlib
+from functools import lru_cache
 
 import torch
 
@@ -30,23 +30,50 @@ from lightreason_b200.native import _require
 
 GROUP = 128
 E4M3 = torch.float8_e4m3fn
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+# These calls sit in decode loops that may run uncaptured, where a few
+# microseconds of Python a call show: the stream comes from torch's raw getter,
+# sizes of workspaces are remembered per shape, and a tensor is checked in one
+# expression.
+
+
+def _device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _groups(n: int) -> int:
     return -(-n // GROUP)
 
 
-def _on(device: torch.device):
-    """The calls launch on the current device: make it the tensors'."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == device and t.shape == shape
+def _check(t, name: str, dtype: torch.dtype, shape: tuple, index: int) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == index
             and t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on cuda:{index}")
+
+
+def _check_all(checks, index: int) -> None:
+    """_check of every (tensor, name, dtype, shape), in one loop."""
+    for t, name, dtype, shape in checks:
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+            _check(t, name, dtype, shape, index)
+
+
+def _call(name: str, index: int, args: tuple) -> None:
+    """Entry point `name` on device `index` and its current stream (the last
+    argument of every entry point)."""
+    fn = getattr(native.lib(), name)
+    if _device() == index:
+        rc = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        native.check(rc, name)
 
 
 def _no_grad(*tensors) -> None:
@@ -57,12 +84,14 @@ def _no_grad(*tensors) -> None:
 
 def _rows(t: torch.Tensor, name: str) -> int:
     """The row stride of a [T, H] BF16 CUDA tensor with dense rows."""
-    _require(t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 2, f"{name} must be a CUDA BF16 [T, H] tensor")
+    if not (t.is_cuda and t.dtype is _BF16 and t.dim() == 2):
+        raise ValueError(f"{name} must be a CUDA BF16 [T, H] tensor")
     tokens, hidden = t.shape
+    step, unit = t.stride()
     _require(hidden >= 1, f"{name} has no columns")
-    _require((hidden == 1 or t.stride(1) == 1) and (tokens <= 1 or t.stride(0) >= hidden),
+    _require((hidden == 1 or unit == 1) and (tokens <= 1 or step >= hidden),
              f"{name} must have dense rows that do not overlap")
-    return t.stride(0) if tokens > 1 else hidden
+    return step if tokens > 1 else hidden
 
 
 def quantize_rows(x: torch.Tensor, *, out=None):
@@ -70,17 +99,15 @@ def quantize_rows(x: torch.Tensor, *, out=None):
     [T, ceil(H / 128)]).  out: the same pair, to be written."""
     stride = _rows(x, "x")
     _no_grad(x)
-    (tokens, hidden), dev = x.shape, x.device
+    tokens, hidden = x.shape
+    index, groups = x.get_device(), _groups(hidden)
     if out is None:
-        out = (torch.empty((tokens, hidden), dtype=E4M3, device=dev),
-               torch.empty((tokens, _groups(hidden)), dtype=torch.float32, device=dev))
+        out = (torch.empty((tokens, hidden), dtype=E4M3, device=x.device),
+               torch.empty((tokens, groups), dtype=_F32, device=x.device))
     q, scales = out
-    _check(q, "out[0]", E4M3, (tokens, hidden), dev)
-    _check(scales, "out[1]", torch.float32, (tokens, _groups(hidden)), dev)
-    with _on(dev):
-        native.check(native.lib().moe_rmsnorm_fp8(x.data_ptr(), stride, None, 0, None, 0.0, 0.0, tokens, hidden,
-                                                  q.data_ptr(), scales.data_ptr(), None, None, native._stream(dev)),
-                     "moe_rmsnorm_fp8")
+    _check_all(((q, "out[0]", E4M3, x.shape), (scales, "out[1]", _F32, (tokens, groups))), index)
+    _call("moe_rmsnorm_fp8", index, (x.data_ptr(), stride, None, 0, None, 0.0, 0.0, tokens, hidden, q.data_ptr(),
+                                     scales.data_ptr(), None, None))
     return q, scales
 
 
@@ -93,56 +120,63 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     weight is stored around zero; 0 for plain norms.  out: the same four, to be
     written; its residual_out may be `residual` itself and its normed `x`."""
     stride = _rows(x, "x")
-    (tokens, hidden), dev = x.shape, x.device
+    tokens, hidden = shape = x.shape
+    index, groups = x.get_device(), _groups(hidden)
     _no_grad(x, weight, residual)
-    _check(weight, "weight", torch.bfloat16, (hidden,), dev)
     rstride = 0
     if residual is not None:
         rstride = _rows(residual, "residual")
-        _require(residual.shape == x.shape and residual.device == dev, "residual must have x's shape and device")
+        _require(residual.shape == shape and residual.get_device() == index,
+                 "residual must have x's shape and device")
     if out is None:
-        bf = dict(dtype=torch.bfloat16, device=dev)
-        out = (torch.empty((tokens, hidden), dtype=E4M3, device=dev),
-               torch.empty((tokens, _groups(hidden)), dtype=torch.float32, device=dev),
-               torch.empty((tokens, hidden), **bf) if normed else None,
-               torch.empty((tokens, hidden), **bf) if residual is not None else None)
+        dev = x.device
+        out = (torch.empty(shape, dtype=E4M3, device=dev), torch.empty((tokens, groups), dtype=_F32, device=dev),
+               torch.empty(shape, dtype=_BF16, device=dev) if normed else None,
+               torch.empty(shape, dtype=_BF16, device=dev) if residual is not None else None)
     q, scales, y, r = out
-    _check(q, "out[0]", E4M3, (tokens, hidden), dev)
-    _check(scales, "out[1]", torch.float32, (tokens, _groups(hidden)), dev)
+    _check_all(((weight, "weight", _BF16, (hidden,)), (q, "out[0]", E4M3, shape),
+                (scales, "out[1]", _F32, (tokens, groups))), index)
     if y is not None:
-        _check(y, "out[2]", torch.bfloat16, (tokens, hidden), dev)
+        _check(y, "out[2]", _BF16, shape, index)
     if r is not None:
         _require(residual is not None, "out[3] without a residual")
-        _check(r, "out[3]", torch.bfloat16, (tokens, hidden), dev)
-    with _on(dev):
-        native.check(native.lib().moe_rmsnorm_fp8(
-            x.data_ptr(), stride, native._ptr(residual), rstride, weight.data_ptr(), weight_offset, eps, tokens,
-            hidden, q.data_ptr(), scales.data_ptr(), native._ptr(y), native._ptr(r), native._stream(dev)),
-            "moe_rmsnorm_fp8")
+        _check(r, "out[3]", _BF16, shape, index)
+    _call("moe_rmsnorm_fp8", index,
+          (x.data_ptr(), stride, None if residual is None else residual.data_ptr(), rstride, weight.data_ptr(),
+           weight_offset, eps, tokens, hidden, q.data_ptr(), scales.data_ptr(), None if y is None else y.data_ptr(),
+           None if r is None else r.data_ptr()))
     return out
 
 
 def quantize_blocks(w: torch.Tensor, *, out=None):
     """BF16 weights [N, K] or [banks, N, K] -> (q e4m3, scales f32 [(banks,)
     ceil(N / 128), ceil(K / 128)])."""
-    _require(w.is_cuda and w.dtype == torch.bfloat16 and w.dim() in (2, 3) and w.is_contiguous(),
-             "w must be a contiguous CUDA BF16 [N, K] or [banks, N, K] tensor")
+    if not (w.is_cuda and w.dtype is _BF16 and w.dim() in (2, 3) and w.is_contiguous()):
+        raise ValueError("w must be a contiguous CUDA BF16 [N, K] or [banks, N, K] tensor")
     _no_grad(w)
-    rows, cols = w.shape[-2:]
-    banks = w.shape[0] if w.dim() == 3 else 1
+    shape = w.shape
+    rows, cols = shape[-2], shape[-1]
+    banks = shape[0] if len(shape) == 3 else 1
     _require(rows >= 1 and cols >= 1, "w has no rows or columns")
-    shape = (*w.shape[:-2], _groups(rows), _groups(cols))
+    index = w.get_device()
+    blocks = (_groups(rows), _groups(cols)) if len(shape) == 2 else (banks, _groups(rows), _groups(cols))
     if out is None:
-        out = (torch.empty(w.shape, dtype=E4M3, device=w.device),
-               torch.empty(shape, dtype=torch.float32, device=w.device))
-    q, scales = out
-    _check(q, "out[0]", E4M3, tuple(w.shape), w.device)
-    _check(scales, "out[1]", torch.float32, shape, w.device)
-    with _on(w.device):
-        native.check(native.lib().moe_quantize_fp8_blocks(w.data_ptr(), banks, rows, cols, q.data_ptr(),
-                                                          scales.data_ptr(), native._stream(w.device)),
-                     "moe_quantize_fp8_blocks")
+        out = (torch.empty(shape, dtype=E4M3, device=w.device), torch.empty(blocks, dtype=_F32, device=w.device))
+    else:
+        _check(out[0], "out[0]", E4M3, shape, index)
+        _check(out[1], "out[1]", _F32, blocks, index)
+    _call("moe_quantize_fp8_blocks", index, (w.data_ptr(), banks, rows, cols, out[0].data_ptr(), out[1].data_ptr()))
     return out
+
+
+@lru_cache(maxsize=4096)
+def _linear_workspace(*sizes) -> int:
+    return native.lib().moe_linear_fp8_workspace_bytes(*sizes)
+
+
+@lru_cache(maxsize=4096)
+def _experts_workspace(*sizes) -> int:
+    return native.lib().moe_experts_fp8_workspace_bytes(*sizes)
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
@@ -158,28 +192,28 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
     scales stand for -> [T, N] in BF16 or FP32 (out_dtype, or out's).  K must be
     a multiple of 16.  status: a device int32 [1] that becomes 1 if a bounded
     wait inside a kernel gave up (the output is then not valid)."""
-    _require(x.is_cuda and x.dim() == 2 and w.dim() == 2, "x and w must be CUDA [T, K] and [N, K] tensors")
-    (tokens, cols), rows, dev = x.shape, w.shape[0], x.device
-    _require(rows >= 1 and cols >= 16 and cols % 16 == 0, "K must be a positive multiple of 16 and N positive")
-    _check(x, "x", E4M3, (tokens, cols), dev)
-    _check(x_scales, "x_scales", torch.float32, (tokens, _groups(cols)), dev)
-    _check(w, "w", E4M3, (rows, cols), dev)
-    _check(w_scales, "w_scales", torch.float32, (_groups(rows), _groups(cols)), dev)
+    if not (x.is_cuda and x.dim() == 2 and w.dim() == 2):
+        raise ValueError("x and w must be CUDA [T, K] and [N, K] tensors")
+    tokens, cols = x.shape
+    rows, index, groups = w.shape[0], x.get_device(), _groups(cols)
+    if rows < 1 or cols < 16 or cols % 16:
+        raise ValueError("K must be a positive multiple of 16 and N positive")
+    _check_all(((x, "x", E4M3, (tokens, cols)), (x_scales, "x_scales", _F32, (tokens, groups)),
+                (w, "w", E4M3, (rows, cols)), (w_scales, "w_scales", _F32, (_groups(rows), groups))), index)
     if out is None:
-        _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be BF16 or FP32")
-        out = torch.empty((tokens, rows), dtype=out_dtype, device=dev)
+        _require(out_dtype in (_BF16, _F32), "out_dtype must be BF16 or FP32")
+        out = torch.empty((tokens, rows), dtype=out_dtype, device=x.device)
     else:
-        _require(out.dtype in (torch.bfloat16, torch.float32), "out must be BF16 or FP32")
-        _check(out, "out", out.dtype, (tokens, rows), dev)
+        _require(out.dtype in (_BF16, _F32), "out must be BF16 or FP32")
+        _check(out, "out", out.dtype, (tokens, rows), index)
     if status is not None:
-        _check(status, "status", torch.int32, (1,), dev)
-    so = native.lib()
-    ws = _workspace(so.moe_linear_fp8_workspace_bytes(tokens, rows, cols), dev)
-    with _on(dev):
-        native.check(so.moe_linear_fp8(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), tokens,
-                                       rows, cols, out.data_ptr(), int(out.dtype == torch.float32), native._ptr(ws),
-                                       ws.numel() if ws is not None else 0, native._ptr(status), native._stream(dev)),
-                     "moe_linear_fp8")
+        _check(status, "status", torch.int32, (1,), index)
+    nbytes = _linear_workspace(tokens, rows, cols)
+    ws = _workspace(nbytes, x.device)
+    _call("moe_linear_fp8", index,
+          (x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), tokens, rows, cols, out.data_ptr(),
+           out.dtype is _F32, None if ws is None else ws.data_ptr(), nbytes,
+           None if status is None else status.data_ptr()))
     return out
 
 
@@ -190,29 +224,28 @@ def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate
     [E, 2I, H] and down [E, H, I] with their block scales, idx int64 [T, K]
     (ids outside [0, E) contribute nothing), weights BF16 [T, K] -> BF16 [T, H].
     H is a multiple of 16, I of 128.  status as in linear."""
-    _require(x.is_cuda and x.dim() == 2 and gate_up.dim() == 3 and down.dim() == 3 and idx.dim() == 2,
-             "expected x [T, H], gate_up [E, 2I, H], down [E, H, I] and idx [T, K] on a CUDA device")
-    (tokens, hidden), dev = x.shape, x.device
+    if not (x.is_cuda and x.dim() == 2 and gate_up.dim() == 3 and down.dim() == 3 and idx.dim() == 2):
+        raise ValueError("expected x [T, H], gate_up [E, 2I, H], down [E, H, I] and idx [T, K] on a CUDA device")
+    tokens, hidden = shape = x.shape
+    index, groups = x.get_device(), _groups(hidden)
     count, inner, top_k = gate_up.shape[0], down.shape[2], idx.shape[1]
-    _check(x, "x", E4M3, (tokens, hidden), dev)
-    _check(x_scales, "x_scales", torch.float32, (tokens, _groups(hidden)), dev)
-    _check(gate_up, "gate_up", E4M3, (count, 2 * inner, hidden), dev)
-    _check(gate_up_scales, "gate_up_scales", torch.float32, (count, _groups(2 * inner), _groups(hidden)), dev)
-    _check(down, "down", E4M3, (count, hidden, inner), dev)
-    _check(down_scales, "down_scales", torch.float32, (count, _groups(hidden), _groups(inner)), dev)
-    _check(idx, "idx", torch.int64, (tokens, top_k), dev)
-    _check(weights, "weights", torch.bfloat16, (tokens, top_k), dev)
+    _check_all(((x, "x", E4M3, shape), (x_scales, "x_scales", _F32, (tokens, groups)),
+                (gate_up, "gate_up", E4M3, (count, 2 * inner, hidden)),
+                (gate_up_scales, "gate_up_scales", _F32, (count, _groups(2 * inner), groups)),
+                (down, "down", E4M3, (count, hidden, inner)),
+                (down_scales, "down_scales", _F32, (count, groups, _groups(inner))),
+                (idx, "idx", torch.int64, (tokens, top_k)), (weights, "weights", _BF16, (tokens, top_k))), index)
     if out is None:
-        out = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=dev)
-    _check(out, "out", torch.bfloat16, (tokens, hidden), dev)
+        out = torch.empty(shape, dtype=_BF16, device=x.device)
+    else:
+        _check(out, "out", _BF16, shape, index)
     if status is not None:
-        _check(status, "status", torch.int32, (1,), dev)
-    so = native.lib()
-    ws = _workspace(so.moe_experts_fp8_workspace_bytes(tokens, count, top_k, hidden, inner), dev)
-    with _on(dev):
-        native.check(so.moe_experts_fp8(x.data_ptr(), x_scales.data_ptr(), gate_up.data_ptr(),
-                                        gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(),
-                                        idx.data_ptr(), weights.data_ptr(), tokens, count, top_k, hidden, inner,
-                                        out.data_ptr(), native._ptr(ws), ws.numel() if ws is not None else 0,
-                                        native._ptr(status), native._stream(dev)), "moe_experts_fp8")
+        _check(status, "status", torch.int32, (1,), index)
+    nbytes = _experts_workspace(tokens, count, top_k, hidden, inner)
+    ws = _workspace(nbytes, x.device)
+    _call("moe_experts_fp8", index,
+          (x.data_ptr(), x_scales.data_ptr(), gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(),
+           down_scales.data_ptr(), idx.data_ptr(), weights.data_ptr(), tokens, count, top_k, hidden, inner,
+           out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+           None if status is None else status.data_ptr()))
     return out

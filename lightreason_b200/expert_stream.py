@@ -26,6 +26,11 @@ three residencies:
   "b200-packed"  as b200-host with the rows kept in the lossless row codec
                  (bf16_expert_codec), 25% fewer bytes over the host link --
                  also "packed".
+A fourth trades the bit-exact BF16 arithmetic for half the weight bytes:
+  "b200-fp8"     experts in HBM as e4m3 with an FP32 scale per 128 x 128 block
+                 (lightreason_b200.fp8), the hidden states brought to e4m3 per
+                 row and 128 columns on each call; sums in FP32, one expert's
+                 row rounded to BF16 before the weighted sum.
 With capacity_bytes > 0 the host residencies keep up to capacity_bytes of
 experts per layer in HBM slots across calls (a device-side LRU, the role of
 the reference pool's byte-bounded row cache, expert_stream.py:132-174): only
@@ -42,16 +47,18 @@ from dataclasses import asdict, dataclass
 import numpy as np
 import torch
 
-from lightreason_b200 import native
+from lightreason_b200 import fp8, native
 
 REFERENCE_MODES = ("dense", "selected", "cached", "packed", "scheduled", "grouped", "pipelined", "fused",
                    "batched", "cpu", "seeded", "hybrid")
-B200_MODES = ("b200", "b200-host", "b200-packed")
+B200_MODES = ("b200", "b200-host", "b200-packed", "b200-fp8")
+HOST_RESIDENCIES = ("b200-host", "b200-packed")
 MODES = REFERENCE_MODES + B200_MODES
 RESIDENCY = {
     **{m: "b200" for m in ("b200", "fused", "batched", "scheduled", "grouped", "seeded")},
     **{m: "b200-host" for m in ("b200-host", "dense", "selected", "cached", "pipelined", "cpu", "hybrid")},
     **{m: "b200-packed" for m in ("b200-packed", "packed")},
+    "b200-fp8": "b200-fp8",
 }
 
 
@@ -61,6 +68,7 @@ class TransferStats:
     b200_layer_calls: int = 0
     host_layer_calls: int = 0
     packed_layer_calls: int = 0
+    fp8_layer_calls: int = 0
     tokens: int = 0
     resident_bytes: int = 0
     pinned_bytes: int = 0
@@ -122,11 +130,21 @@ class ExpertPool:
         reference keeps one LRU of device rows under capacity_bytes for all
         layers (expert_stream.py:147-174); here each patched layer gets an even
         share of the budget as its own device-planned slot bank."""
-        if layer.residency == "b200" or not self._capacity_bytes:
+        if layer.residency not in HOST_RESIDENCIES or not self._capacity_bytes:
             return 0
         share = self._capacity_bytes // max(1, self._cache_layers)
         slots = min(share // layer.row_bytes, layer.module.num_experts, 1024)
         return slots if slots >= routed else 0
+
+    def _fp8_banks(self, layer: "_Layer", owner=None, shared=None) -> fp8.ExpertBanks:
+        """The FP8 banks of one patched module (with its shared expert, for a
+        whole-block patch), made on first use."""
+        key = (id(owner if owner is not None else layer.module), layer.residency, 0)
+        banks = self._layers.get(key)
+        if banks is None:
+            banks = self._layers[key] = fp8.ExpertBanks(layer.gate_up, layer.down, self.device, shared=shared)
+            self.stats.resident_bytes += banks.nbytes()
+        return banks
 
     def _native_layer(self, layer: "_Layer", top_k: int, owner=None, extra=None, cache: int = 0) -> native.Layer:
         """The native layer of one patched module, built on first use: the
@@ -199,8 +217,10 @@ class _Layer:
         if "forward" in vars(module) or getattr(module, "_hf_hook", None) is not None:
             raise ValueError(f"{name}: expert forwards must have no existing offload hooks")
         _check_module(name, module)
-        if self.residency != "b200" and self.gate_up.device.type != "cpu":
+        if self.residency in HOST_RESIDENCIES and self.gate_up.device.type != "cpu":
             raise ValueError(f"{name}: host residency needs CPU expert parameters")
+        if self.residency == "b200-fp8":
+            fp8.check_widths(module.hidden_dim, module.intermediate_dim)
         self.row_bytes = (self.gate_up.numel() + self.down.numel()) * 2 // module.num_experts
 
     def _check_sources(self):
@@ -227,7 +247,8 @@ class _Layer:
             raise ValueError(f"{self.name}: expected BF16 states [T, H], int64 expert ids and BF16 weights [T, K]")
         pool.stats.layer_calls += 1
         pool.stats.tokens += hidden_states.shape[0]
-        counter = {"b200": "b200_layer_calls", "b200-host": "host_layer_calls", "b200-packed": "packed_layer_calls"}
+        counter = {"b200": "b200_layer_calls", "b200-host": "host_layer_calls", "b200-packed": "packed_layer_calls",
+                   "b200-fp8": "fp8_layer_calls"}
         setattr(pool.stats, counter[self.residency], getattr(pool.stats, counter[self.residency]) + 1)
         return self.run(hidden_states, top_k_index, top_k_weights)
 
@@ -235,6 +256,9 @@ class _Layer:
         """The device chain itself, shared by the per-path entry points."""
         if hidden_states.shape[0] == 0:
             return torch.zeros_like(hidden_states)
+        if self.residency == "b200-fp8":
+            return self.pool._fp8_banks(self)(hidden_states.contiguous(), top_k_index.contiguous(),
+                                              top_k_weights.contiguous())
         routed = min(self.module.num_experts, top_k_index.numel())
         layer = self.pool._native_layer(self, top_k_index.shape[1], cache=self.pool.cache_slots(self, routed))
         return layer(hidden_states.contiguous(), route_in=top_k_index.contiguous(),
@@ -256,7 +280,7 @@ def patch_experts(model, *, mode, pool):
     if not layers:
         raise ValueError("No Transformers Qwen3_5MoeExperts modules found")
     pool._check_context()
-    if RESIDENCY[mode] != "b200":
+    if RESIDENCY[mode] in HOST_RESIDENCIES:
         layouts = {(tuple(layer.gate_up.shape[1:]), tuple(layer.down.shape[1:])) for layer in layers}
         if len(layouts) != 1:
             raise ValueError("Host-resident expert layers must share one gate/down layout")

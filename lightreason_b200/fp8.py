@@ -12,8 +12,8 @@ the group's largest magnitude (at least 1e-10), and read back as q * scale.
   experts            the routed SwiGLU experts (Qwen3_5MoeExperts.forward) on
                      FP8 banks, routes given
 
-`patch_experts(model, mode="b200-fp8", pool=...)` runs a model's experts on
-them.  Like the rest of the package they are inference operators: no gradients.
+`patch_experts(model, mode="b200-fp8", pool=...)` and `patch_moe_blocks` run a
+model's experts on them (ExpertBanks).  Like the rest of the package they are inference operators: no gradients.
 Work is enqueued on the tensors' device's current stream without a host
 synchronisation and can be captured in a CUDA graph; `out=` takes outputs that
 the caller keeps.
@@ -249,3 +249,56 @@ def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate
            out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
            None if status is None else status.data_ptr()))
     return out
+
+
+class ExpertBanks:
+    """The FP8 banks of one layer's experts, made from BF16 ones.
+
+    gate_up [E, 2I, H] and down [E, H, I] may live on the CPU or on the device;
+    they are brought over and quantised a few experts at a time, so the BF16
+    bank is never whole on the device because of this.  shared: a further
+    expert (gate [I, H], up [I, H], down [H, I]), kept as expert id E."""
+
+    CHUNK = 16  # experts quantised at once
+
+    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, device, *, shared=None):
+        count, rows, hidden = gate_up.shape
+        inner = rows // 2
+        _require(tuple(down.shape) == (count, hidden, inner), "gate_up must be [E, 2I, H] and down [E, H, I]")
+        check_widths(hidden, inner)
+        total = count + (shared is not None)
+        self.experts, self.hidden, self.inner, self.device = count, hidden, inner, torch.device(device)
+        make = lambda n, k: (torch.empty((total, n, k), dtype=E4M3, device=self.device),  # noqa: E731
+                             torch.empty((total, _groups(n), _groups(k)), dtype=_F32, device=self.device))
+        self.gate_up, self.gate_up_scales = make(rows, hidden)
+        self.down, self.down_scales = make(hidden, inner)
+        parts = [(a, min(a + self.CHUNK, count)) for a in range(0, count, self.CHUNK)]
+        with torch.no_grad():
+            for source, q, scales in ((gate_up, self.gate_up, self.gate_up_scales),
+                                      (down, self.down, self.down_scales)):
+                for a, b in parts:
+                    quantize_blocks(source[a:b].detach().to(self.device).contiguous(), out=(q[a:b], scales[a:b]))
+            if shared is not None:
+                gate, up, last = (t.detach().to(self.device) for t in shared)
+                _require(tuple(gate.shape) == tuple(up.shape) == (inner, hidden)
+                         and tuple(last.shape) == (hidden, inner), "the shared expert must have the experts' widths")
+                quantize_blocks(torch.cat([gate, up])[None], out=(self.gate_up[count:], self.gate_up_scales[count:]))
+                quantize_blocks(last[None].contiguous(), out=(self.down[count:], self.down_scales[count:]))
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size()
+                   for t in (self.gate_up, self.gate_up_scales, self.down, self.down_scales))
+
+    def release(self) -> None:
+        """Part of the pool's layer interface; the banks go with their tensors."""
+
+    def __call__(self, hidden: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+        """The experts' forward on BF16 states: quantised rows, then experts()."""
+        q, scales = quantize_rows(hidden)
+        return experts(q, scales, self.gate_up, self.gate_up_scales, self.down, self.down_scales, idx, weights)
+
+
+def check_widths(hidden: int, inner: int) -> None:
+    """The widths the expert kernels take."""
+    _require(hidden % 16 == 0 and inner % 128 == 0,
+             f"FP8 experts need hidden a multiple of 16 and inner of 128, got {hidden} and {inner}")

@@ -7,7 +7,9 @@ routed experts -> + sigmoid(shared gate) * shared expert.  patch_moe_blocks
 runs all of it as moe_layer_forward: the router and the shared expert move to
 the pool device once, the routed experts keep the residency of the chosen
 mode (HBM, pinned host rows, or packed host rows), and no host read happens
-inside the forward.  The router weights are rounded to BF16 before the
+inside the forward.  In mode "b200-fp8" the block is moe_router_topk and
+moe_experts_fp8, the shared expert one more expert of the FP8 bank, weighted
+with its sigmoid gate.  The router weights are rounded to BF16 before the
 combine, the contract of the reference's expert forwards
 (expert_stream.py:356, fused_experts.py:41-45).
 """
@@ -18,6 +20,7 @@ from contextlib import contextmanager
 
 import torch
 
+from lightreason_b200 import native
 from lightreason_b200.expert_stream import MODES, _Layer
 
 
@@ -32,6 +35,10 @@ class _Block:
                 block.experts.num_experts, block.experts.hidden_dim):
             raise ValueError(f"{name}: expected a BF16 router [experts, hidden]")
         self.top_k = gate.top_k
+        self._route = None   # router and shared gate weights on the device (FP8 blocks)
+        if self.experts.residency == "b200-fp8" and \
+                block.shared_expert.gate_proj.weight.shape[0] != block.experts.intermediate_dim:
+            raise ValueError(f"{name}: FP8 blocks need a shared expert of the experts' width")
 
     def _extra(self):
         dev = self.pool.device
@@ -55,10 +62,25 @@ class _Block:
         pool.stats.tokens += x.shape[0]
         if x.shape[0] == 0:
             return torch.zeros_like(hidden_states)
+        if self.experts.residency == "b200-fp8":
+            return self._fp8(x).reshape(shape)
         routed = min(self.block.experts.num_experts, x.shape[0] * self.top_k)
         layer = pool._native_layer(self.experts, self.top_k, owner=self.block, extra=self._extra(),
                                    cache=pool.cache_slots(self.experts, routed))
         return layer(x).reshape(shape)
+
+    def _fp8(self, x):
+        """The block on FP8 banks: the shared expert is expert E, its weight the sigmoid gate."""
+        b, dev = self.block, self.pool.device
+        shared = b.shared_expert
+        banks = self.pool._fp8_banks(self.experts, owner=b, shared=(
+            shared.gate_proj.weight, shared.up_proj.weight, shared.down_proj.weight))
+        if self._route is None:
+            self._route = (b.gate.weight.detach().to(dev).contiguous(),
+                           b.shared_expert_gate.weight.reshape(-1).detach().to(dev).contiguous())
+        idx, _, scores, _, sig = native.router_topk(x, self._route[0], None, self._route[1], self.top_k)
+        idx = torch.nn.functional.pad(idx, (0, 1), value=banks.experts)
+        return banks(x, idx, torch.cat([scores, sig[:, None]], 1))
 
 
 @contextmanager

@@ -111,3 +111,20 @@ def test_python_refuses_cpu_tensors_and_wrong_types():
                                      torch.zeros(4, 1).bfloat16())):
         with pytest.raises(ValueError):
             call()
+
+
+def test_patch_refuses_widths_without_kernels():
+    """A model whose widths the FP8 kernels do not take is refused when it is
+    patched, not when it runs."""
+    from lightreason_b200 import expert_stream
+    from transformers.models.qwen3_5_moe.configuration_qwen3_5_moe import Qwen3_5MoeTextConfig
+    from transformers.models.qwen3_5_moe.modeling_qwen3_5_moe import Qwen3_5MoeExperts
+
+    config = Qwen3_5MoeTextConfig(hidden_size=256, moe_intermediate_size=192, num_experts=4, num_experts_per_tok=2)
+    config._experts_implementation = "eager"
+    experts = Qwen3_5MoeExperts(config).to(torch.bfloat16).eval().requires_grad_(False)
+    pool = expert_stream.ExpertPool("cuda:0")
+    with pytest.raises(ValueError, match="inner of 128"):
+        expert_stream._Layer("e", experts, pool, "b200-fp8")
+    with pytest.raises(ValueError, match="inner of 128"):
+        fp8.check_widths(256, 192)

@@ -424,3 +424,115 @@ def test_back_to_back_calls_with_new_weights(dev):
         got.append(fp8.linear(x, xs, *out))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------ in a model ---
+
+EXPERTS = 32
+
+
+@pytest.fixture(scope="module")
+def model():
+    from tests.dropin_model import make_model
+
+    return make_model(experts=EXPERTS, layers=2)[0]
+
+
+def states(tokens, dev, seed=0):
+    g = gen(seed + tokens, dev)
+    x = randn(g, tokens, 2048).to(torch.bfloat16)
+    idx = torch.rand(tokens, EXPERTS, generator=g, device=dev).topk(8, -1)[1]
+    return x, idx, torch.softmax(randn(g, tokens, 8), -1).to(torch.bfloat16)
+
+
+def rms_ratio(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+# e4m3 rounds a value by 2^-4 of itself at most, uniformly within its step and
+# so by 2^-4 / sqrt(3) rms at the worst place of a binade; rows and weights of
+# both products are four such independent roundings of the terms that a result
+# sums, and SwiGLU multiplies two of the first sums: sqrt(2 + 2 + 2) of them
+MODEL_RMS = 6 ** 0.5 * 2.0 ** -4 / 3 ** 0.5
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 20])
+def test_patched_experts_fp8(dev, model, tokens):
+    """patch_experts(mode="b200-fp8") is the operators on the module's
+    quantised banks, and near the BF16 experts."""
+    from lightreason_b200 import expert_stream
+
+    pool = expert_stream.ExpertPool(dev)
+    args = states(tokens, dev)
+    with torch.inference_mode(), expert_stream.patch_experts(model, mode="b200-fp8", pool=pool):
+        got = [layer.experts(*args) for layer in model.layers]
+        again = model.layers[0].experts(*args)
+    assert pool.stats.fp8_layer_calls == 3 and pool.stats.resident_bytes > 0
+    assert torch.equal(again, got[0])
+    bf16 = expert_stream.ExpertPool(dev)
+    with torch.inference_mode(), expert_stream.patch_experts(model, mode="b200", pool=bf16):
+        want = [layer.experts(*args) for layer in model.layers]
+    for layer, g, w in zip(model.layers, got, want):
+        m = layer.experts
+        q, s = fp8.quantize_rows(args[0])
+        gu, dn = (fp8.quantize_blocks(t.detach().to(dev)) for t in (m.gate_up_proj, m.down_proj))
+        assert torch.equal(g, fp8.experts(q, s, *gu, *dn, args[1], args[2]))
+        assert rms_ratio(g, w) < MODEL_RMS
+    pool.clear()
+
+
+@pytest.mark.parametrize("tokens", [1, 33])
+def test_patched_blocks_fp8(dev, model, tokens):
+    """The whole block on FP8 banks against its BF16 chain: same routes, the
+    shared expert weighted by its gate."""
+    from lightreason_b200 import expert_stream, moe_block
+
+    x = states(tokens, dev, seed=9)[0].reshape(1, tokens, 2048)
+    outs = {}
+    for mode in ("b200", "b200-fp8"):
+        pool = expert_stream.ExpertPool(dev)
+        with torch.inference_mode(), moe_block.patch_moe_blocks(model, mode=mode, pool=pool):
+            outs[mode] = [b(x) for b in model.layers]
+            assert model.layers[0](x[:, :0]).shape == (1, 0, 2048)
+        pool.clear()
+    for got, want in zip(outs["b200-fp8"], outs["b200"]):
+        assert got.shape == want.shape and rms_ratio(got, want) < MODEL_RMS
+
+
+def test_patched_experts_fp8_replayed(dev, model):
+    """Captured graphs per layer and width give the eager calls' values."""
+    from lightreason_b200 import expert_stream, scheduled_graph
+
+    pool = expert_stream.ExpertPool(dev)
+    with torch.inference_mode(), expert_stream.patch_experts(model, mode="b200-fp8", pool=pool):
+        cases = [states(t, dev, seed=s) for t in (1, 5) for s in range(2)]
+        want = [[layer.experts(*c) for layer in model.layers] for c in cases]
+        with scheduled_graph.replay_experts(pool):
+            got = [[layer.experts(*c).clone() for layer in model.layers] for c in cases]
+        scheduled_graph.release_graphs(pool)
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    pool.clear()
+
+
+def test_layer_as_a_decoder_would_run_it(dev):
+    """Residual and norm, router, experts and a projection together, against
+    the same chain of 64-bit forms on the operators' own intermediate values."""
+    g = gen(21, dev)
+    tokens, hidden, inner, count, top_k = 19, 1024, 256, 16, 4
+    x, res = (randn(g, tokens, hidden).to(torch.bfloat16) for _ in range(2))
+    w = (0.1 * randn(g, hidden)).to(torch.bfloat16)
+    router = (0.05 * randn(g, count, hidden)).to(torch.bfloat16)
+    gu, gus = fp8.quantize_blocks((0.05 * randn(g, count, 2 * inner, hidden)).to(torch.bfloat16))
+    dn, dns = fp8.quantize_blocks((0.05 * randn(g, count, hidden, inner)).to(torch.bfloat16))
+    proj, ps = fp8.quantize_blocks((0.05 * randn(g, 384, hidden)).to(torch.bfloat16))
+    q, s, normed, total = fp8.rmsnorm_quantize(x, w, res)
+    check_norm((q, s, normed, total), x, w, res)
+    idx, _, scores, _, _ = native.router_topk(normed, router, top_k=top_k)
+    out = fp8.experts(q, s, gu, gus, dn, dns, idx, scores)
+    want, bound = R.experts(q, s, gu, gus, dn, dns, idx, scores)
+    within(out, want, bound, "experts")
+    q2, s2, _, total2 = fp8.rmsnorm_quantize(out, w, total)
+    check_norm((q2, s2, _, total2), out, w, total)
+    y = fp8.linear(q2, s2, proj, ps, out_dtype=torch.float32)
+    want, bound = R.linear(q2, s2, proj, ps)
+    within(y, want, bound + R.F32 * want.abs(), "projection")

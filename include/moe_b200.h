@@ -538,8 +538,8 @@ int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, co
  * [E, H, I]: for each route (t, k) of expert e = idx[t, k]
  *   h = silu(gate . x_t) * (up . x_t)  in FP32, brought to e4m3 per 128 values
  *   out[t] += weights[t, k] * (down . h)
- * with FP32 sums and one rounding to BF16 at the end on the smallest batches;
- * larger ones keep each route's row as BF16 before the weighted sum.  Ids
+ * with FP32 sums and one rounding to BF16 at the end; batches of more than 2048
+ * routes keep each route's row as BF16 before the weighted sum.  Ids
  * outside [0, E) contribute nothing (a token with none left is 0).  hidden is
  * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024.
  * status as in moe_linear_fp8. */

@@ -24,8 +24,7 @@ int check_experts(int tokens, int experts, int top_k, int hidden, int inner) {
 // Where the scratch of moe_experts_fp8 lies in its workspace.
 struct Layout {
     bool gemv;
-    int hist_ints;
-    size_t offsets, perm_token, perm_slot, route_pos, active, permute_counters, hist, counters, act, act_scales, y, bytes;
+    size_t offsets, row_token, route_pos, counters, act, act_scales, y, bytes;
 };
 Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
     Layout l{};
@@ -42,18 +41,13 @@ Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
         l.bytes = at;
         return l;
     }
-    l.hist_ints = permute_hist_ints(tokens, top_k, experts);
     l.offsets = take(sizeof(int32_t) * (experts + 1));
-    l.perm_token = take(sizeof(int32_t) * routes);
-    l.perm_slot = take(sizeof(int32_t) * routes);
+    l.row_token = take(sizeof(int32_t) * routes);
     l.route_pos = take(sizeof(int32_t) * routes);
-    l.active = take(sizeof(int32_t) * experts);
-    l.permute_counters = take(sizeof(int32_t) * 2);
-    l.hist = take(sizeof(int32_t) * static_cast<size_t>(l.hist_ints));
     l.counters = take(sizeof(int32_t) * (experts + 1));
     l.act = take(routes * inner);
     l.act_scales = take(routes * (inner / fp8::kGroup) * sizeof(float));
-    l.y = take(routes * hidden * 2);
+    l.y = take(routes * hidden * (experts_fp8_wide_rows(static_cast<int>(routes)) ? 4 : 2));
     l.bytes = at;
     return l;
 }
@@ -116,15 +110,11 @@ extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const ui
     auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(ws + at); };
     ExpertsFp8Scratch s{};
     s.offsets = ints(l.offsets);
-    s.perm_token = ints(l.perm_token);
-    s.perm_slot = ints(l.perm_slot);
+    s.row_token = ints(l.row_token);
     s.route_pos = ints(l.route_pos);
-    s.active = ints(l.active);
-    s.permute_counters = ints(l.permute_counters);
-    s.hist = l.hist_ints ? ints(l.hist) : nullptr;
     s.counters = ints(l.counters);
     s.act = ws + l.act;
     s.act_scales = reinterpret_cast<float *>(ws + l.act_scales);
-    s.y = reinterpret_cast<uint16_t *>(ws + l.y);
+    s.y = ws + l.y;
     return launch_experts_fp8_tiles(a, s, status, as_stream(stream));
 }

@@ -40,12 +40,18 @@ int launch_experts_fp8_gemv(const ExpertsFp8 &a, float *h, cudaStream_t stream);
 
 // The tensor-core path.  status (or null): set to 1 if a bounded wait gave up.
 struct ExpertsFp8Scratch {
-    int32_t *offsets, *perm_token, *perm_slot, *route_pos, *active, *permute_counters, *hist;  // as moe_permute_wide
-    int32_t *counters;  // [E + 1]: items handed out, and per expert the finished parts of gate/up items
-    uint8_t *act;       // [T * K, I]
-    float *act_scales;  // [T * K, I / 128]
-    uint16_t *y;        // [T * K, H]
+    int32_t *offsets;    // [E + 1]
+    int32_t *row_token;  // [T * K]
+    int32_t *route_pos;  // [T, K]
+    int32_t *counters;   // [E + 1]: items handed out, and per expert the finished parts of gate/up items
+    uint8_t *act;        // [T * K, I]
+    float *act_scales;   // [T * K, I / 128]
+    void *y;             // [T * K, H], BF16 or (experts_fp8_wide_rows) FP32
 };
+// Rows of the experts' tiles: 16, 32 (weights as M) or 0 for 128 (rows as M).
+int experts_fp8_tile(int routes, int experts);
+// Whether a route's down row is kept in FP32 until the weighted sum.
+bool experts_fp8_wide_rows(int routes);
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream);
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream);
 

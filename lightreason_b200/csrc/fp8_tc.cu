@@ -99,7 +99,8 @@ struct Params {
     int experts, hidden, inner;
     uint8_t *act;       // [R, I] e4m3
     float *act_scales;  // [R, I / 128]
-    uint16_t *y;        // [R, H] BF16
+    void *y;            // [R, H] BF16 or FP32
+    int y_f32;
     int32_t *work;      // items handed out so far (zero at launch)
     int32_t *done;      // [E] epilogue warps that finished an item of phase 1 (zero at launch)
     int32_t *status;
@@ -713,15 +714,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     count_in(it);
                 } else if (active) {
                     const int c0 = it.n * kBN + 32 * q + lane;
-                    const bool f32 = LIN && P.out_f32;
+                    const bool f32 = LIN ? P.out_f32 : P.y_f32;
+                    void *base = LIN ? P.out : P.y;
                     const int64_t at = static_cast<int64_t>(it.row0 + j0) * n2 + c0;
-                    uint16_t *y = (LIN ? static_cast<uint16_t *>(P.out) : P.y) + at;
+                    uint16_t *y = static_cast<uint16_t *>(base) + at;
+                    float *z = static_cast<float *>(base) + at;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
                         if (j >= left) break;
                         const int64_t o = static_cast<int64_t>(j) * n2;
                         if (f32) {
-                            float *z = static_cast<float *>(P.out) + at;
                             if (c0 < n2) z[o] = acc0[j];
                             if (c0 + 128 < n2) z[o + 128] = acc1[j];
                         } else {
@@ -842,13 +844,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                             sm100::bulk_commit();
                         }
                     } else if (!LIN) {
-                        uint16_t *dst = P.y + (first + lane) * n2 + n0;
+                        const int64_t o = (first + lane) * n2 + n0;
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
+                            if (lane >= rows || n0 + 16 * c >= n2) continue;
                             uint32_t v[8];
+                            if (P.y_f32) {
+                                float *dst = static_cast<float *>(P.y) + o + 16 * c;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] = fp8::pack_bf16(acc[16 * c + 2 * i], acc[16 * c + 2 * i + 1]);
-                            if (lane < rows && n0 + 16 * c < n2) store32(dst + 16 * c, v);
+                                for (int g = 0; g < 2; ++g) {
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(acc[16 * c + 8 * g + i]);
+                                    store32(dst + 8 * g, v);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    v[i] = fp8::pack_bf16(acc[16 * c + 2 * i], acc[16 * c + 2 * i + 1]);
+                                store32(static_cast<uint16_t *>(P.y) + o + 16 * c, v);
+                            }
                         }
                     } else if (vec) {
                         float *dst = static_cast<float *>(P.out) + first * n2 + n0;
@@ -890,74 +904,88 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && *abort && P.status) atomicExch(P.status, 1);
 }
 
-// The experts' plan for up to kPlanRoutes routes, one a thread: routes in order
-// of (expert, token, slot).  A route's place among its expert's routes is its
-// rank among the equal ids of its warp plus the warps' counts before it.  Also
-// zeroes the tile kernel's counters.
-constexpr int kPlanRoutes = 1024;
-__global__ void __launch_bounds__(kPlanRoutes) fp8_plan_kernel(const int64_t *__restrict__ idx, int routes, int top_k,
-                                                               int experts, int32_t *__restrict__ offsets,
-                                                               int32_t *__restrict__ row_token,
-                                                               int32_t *__restrict__ route_pos,
-                                                               int32_t *__restrict__ counters) {
-    extern __shared__ uint8_t warp_count[];  // [warps][experts]
-    __shared__ int32_t begin[kMaxExperts], scan[32];
-    const int r = threadIdx.x, lane = r & 31, warp = r >> 5, warps = blockDim.x >> 5;
-    for (int i = r; i < (warps * experts + 3) / 4; i += blockDim.x) reinterpret_cast<uint32_t *>(warp_count)[i] = 0;
+// The experts' plan, by one CTA or a cluster of eight with an equal share of
+// the routes each: count the share's routes per expert in shared memory, scan
+// the experts' totals over the cluster, and hand out places from one counter
+// per expert.  The rows of an expert come in no fixed order; no result depends
+// on it, since a row's products are its own and the weighted sum goes by
+// route_pos.  Also zeroes the tile kernel's counters.
+__global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restrict__ idx, int routes, int top_k,
+                                                                int experts, int32_t *__restrict__ offsets,
+                                                                int32_t *__restrict__ row_token,
+                                                                int32_t *__restrict__ route_pos,
+                                                                int32_t *__restrict__ counters) {
+    __shared__ int32_t count[kMaxExperts], cursor[kMaxExperts], scan[32];
+    const int x = threadIdx.x, lane = x & 31, warp = x >> 5;
+    const int threads = blockDim.x;                // at least the experts
+    const int ctas = gridDim.x, cta = blockIdx.x;  // one cluster
+    count[x] = 0;
     grid_dependency_wait();
     grid_dependency_trigger();
-    for (int i = r; i <= experts; i += blockDim.x) counters[i] = 0;
-    const int64_t id = r < routes ? idx[r] : -1;
-    const int e = id >= 0 && id < experts ? static_cast<int>(id) : -1;
+    if (cta == 0)
+        for (int i = x; i <= experts; i += threads) counters[i] = 0;
     __syncthreads();
-    const unsigned peers = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(peers & ((1u << lane) - 1));
-    if (e >= 0 && rank == 0) warp_count[warp * experts + e] = static_cast<uint8_t>(__popc(peers));
-    __syncthreads();
-    // expert x: its routes, then an exclusive scan over the experts
-    int base = 0;  // experts may exceed the threads: chunks of blockDim.x
-    for (int x0 = 0; x0 < experts; x0 += blockDim.x) {
-        const int x = x0 + r;
-        int count = 0;
-        if (x < experts)
-            for (int w = 0; w < warps; ++w) count += warp_count[w * experts + x];
-        int incl = count;
+    const int per = (routes + ctas - 1) / ctas, r0 = cta * per, r1 = min(routes, r0 + per);
+    constexpr int kU = 4;  // routes of a thread in flight
+    auto each = [&](auto &&f) {
+        for (int r = r0 + x; r < r1; r += kU * threads) {
+            int64_t id[kU];
 #pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, s);
-            if (lane >= s) incl += v;
+            for (int u = 0; u < kU; ++u) id[u] = r + u * threads < r1 ? idx[r + u * threads] : -1;
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+                if (r + u * threads < r1)
+                    f(r + u * threads, id[u] >= 0 && id[u] < experts ? static_cast<int>(id[u]) : -1);
         }
-        if (lane == 31) scan[warp] = incl;
-        __syncthreads();
-        int before = base, all = base;
-        for (int w = 0; w < warps; ++w) {
-            if (w < warp) before += scan[w];
-            all += scan[w];
+    };
+    each([&](int, int e) {
+        if (e >= 0) atomicAdd(&count[e], 1);
+    });
+    if (ctas > 1) sm100::cluster_sync();
+    else __syncthreads();
+    int before = 0, total = 0;  // expert x: its routes in the CTAs before, in all
+    if (x < experts) {
+        for (int c = 0; c < ctas; ++c) {
+            const int v = ctas > 1 ? sm100::ld_cluster_s32(sm100::mapa(&count[x], c)) : count[x];
+            if (c < cta) before += v;
+            total += v;
         }
-        if (x < experts) {
-            begin[x] = offsets[x] = before + incl - count;
-            if (x == experts - 1) offsets[experts] = before + incl;
-        }
-        base = all;
-        __syncthreads();
     }
-    if (r < routes) {
-        int pos = -1;
-        if (e >= 0) {
-            pos = begin[e] + rank;
-            for (int w = 0; w < warp; ++w) pos += warp_count[w * experts + e];
-            row_token[pos] = r / top_k;
+    int incl = total;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, s);
+        if (lane >= s) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int begin = incl - total;
+    for (int w = 0; w < warp; ++w) begin += scan[w];
+    if (x < experts) {
+        cursor[x] = begin + before;
+        if (cta == 0) {
+            offsets[x] = begin;
+            if (x == experts - 1) offsets[experts] = begin + total;
         }
+    }
+    __syncthreads();
+    each([&](int r, int e) {
+        const int pos = e >= 0 ? atomicAdd(&cursor[e], 1) : -1;
+        if (e >= 0) row_token[pos] = r / top_k;
         route_pos[r] = pos;
-    }
+    });
+    if (ctas > 1) sm100::cluster_sync();  // no CTA leaves while another reads its counts
 }
 
 // out[t] = sum over the token's routes, in slot order, of weight * row, in
-// FP32.  A thread per 8 columns of a token, eight rows in flight.
-__global__ void __launch_bounds__(256) fp8_combine_kernel(const uint16_t *__restrict__ y,
+// FP32.  A thread per 8 columns of a token, eight (BF16) or four rows in flight.
+template <class Y>
+__global__ void __launch_bounds__(256) fp8_combine_kernel(const Y *__restrict__ y,
                                                           const int32_t *__restrict__ route_pos,
                                                           const uint16_t *__restrict__ weights, int tokens, int top_k,
                                                           int hidden, uint16_t *__restrict__ out) {
+    constexpr bool kWide = sizeof(Y) == 4;
+    constexpr int kU = kWide ? 4 : 8;
     grid_dependency_wait();
     grid_dependency_trigger();
     const int units = hidden / 8;
@@ -968,23 +996,32 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const uint16_t *__rest
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int k0 = 0; k0 < top_k; k0 += 8) {
-        uint4 v[8];
-        float w[8];
+    for (int k0 = 0; k0 < top_k; k0 += kU) {
+        uint4 v[kU][kWide ? 2 : 1];
+        float w[kU];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kU; ++k) {
             const int64_t at = t * top_k + k0 + k;
             const int p = k0 + k < top_k ? route_pos[at] : -1;
             w[k] = p >= 0 ? bf2f(weights[at]) : 0.f;
-            v[k] = p >= 0 ? ld_stream(y + static_cast<int64_t>(p) * hidden + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int h = 0; h < (kWide ? 2 : 1); ++h)
+                v[k][h] = p >= 0 ? ld_stream(y + static_cast<int64_t>(p) * hidden + c + 4 * h) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        for (int k = 0; k < kU; ++k) {
+            if constexpr (kWide) {
+                const uint32_t u[8] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w,
+                                       v[k][1].x, v[k][1].y, v[k][1].z, v[k][1].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                acc[2 * j] = fmaf(bf16_lo(u[j]), w[k], acc[2 * j]);
-                acc[2 * j + 1] = fmaf(bf16_hi(u[j]), w[k], acc[2 * j + 1]);
+                for (int j = 0; j < 8; ++j) acc[j] = fmaf(__uint_as_float(u[j]), w[k], acc[j]);
+            } else {
+                const uint32_t u[4] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[2 * j] = fmaf(bf16_lo(u[j]), w[k], acc[2 * j]);
+                    acc[2 * j + 1] = fmaf(bf16_hi(u[j]), w[k], acc[2 * j + 1]);
+                }
             }
         }
     }
@@ -1007,6 +1044,26 @@ int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int c
     const uint64_t str[1] = {static_cast<uint64_t>(cols)};
     if (int rc = make_map_u8(m, base, 2, dims, str, full)) return rc;
     return make_map_u8(m16, base, 2, dims, str, 16);
+}
+
+// One CTA up to 2048 routes; eight (6 us at 32,768 routes) above.
+int launch_plan(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int routes, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(routes <= 2048 ? 1 : 8);
+    cfg.blockDim = dim3((std::max(a.experts, std::min(routes, 1024)) + 31) / 32 * 32);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cfg.gridDim.x;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cfg.gridDim.x > 1 ? 2 : 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, fp8_plan_kernel, a.idx, routes, a.top_k, a.experts, s.offsets,
+                                               s.row_token, s.route_pos, s.counters);
+    return err == cudaSuccess ? MOE_OK : cuda_error(err, "fp8_plan_kernel");
 }
 
 // BF16 output rows (cols % 8 == 0), stored 32 rows by 64 columns at a time.
@@ -1050,26 +1107,24 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
     }
 }
 
+// The row tile by the average rows of an expert (256 experts of 2048 x 512,
+// top-8, us at 32 / 128 / 256 / 512 / 1024 tokens, so 1 / 4 / 8 / 16 / 32 rows:
+// tiles of 16 86 / 125 / 154 / 190 / 268, of 32 88 / 123 / 148 / 168 / 205, rows
+// as M 94 / 133 / 156 / 168 / 178).
+int experts_fp8_tile(int routes, int experts) {
+    const int mean = routes / experts;
+    return mean < 4 ? 16 : mean < 16 ? 32 : 0;
+}
+
+// FP32 rows cost nothing beside the weights on small batches; above 2048 routes
+// they are rounded to BF16, half the traffic of what then takes a tenth of the
+// time.
+bool experts_fp8_wide_rows(int routes) { return routes <= 2048; }
+
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream) {
     const int routes = a.tokens * a.top_k;
-    if (routes <= kPlanRoutes) {
-        const int threads = (routes + 31) / 32 * 32;
-        const int smem = (threads / 32 * a.experts + 3) / 4 * 4;
-        if (int rc = launch_pdl(fp8_plan_kernel, dim3(1), dim3(threads), smem, stream, "fp8_plan_kernel", a.idx, routes,
-                                a.top_k, a.experts, s.offsets, s.perm_token, s.route_pos, s.counters))
-            return rc;
-    } else {
-        LRB_CUDA(cudaMemsetAsync(s.counters, 0, sizeof(int32_t) * (a.experts + 1), stream));
-        if (int rc = launch_permute(a.idx, a.tokens, a.top_k, a.experts, s.offsets, s.perm_token, s.perm_slot,
-                                    s.route_pos, s.active, s.permute_counters, s.permute_counters + 1, stream, s.hist))
-            return rc;
-    }
-    // The row tile by the average rows of an expert (256 experts of 2048 x 512,
-    // top-8, us at 32 / 128 / 256 / 512 / 1024 tokens, so 1 / 4 / 8 / 16 / 32
-    // rows: tiles of 16 86 / 125 / 154 / 190 / 268, of 32 88 / 123 / 148 / 168 /
-    // 205, rows as M 94 / 133 / 156 / 168 / 178).
-    const int mean = routes / a.experts;
-    const int bn = mean < 4 ? 16 : mean < 16 ? 32 : 0;
+    if (int rc = launch_plan(a, s, routes, stream)) return rc;
+    const int bn = experts_fp8_tile(routes, a.experts);
     const int tile = bn ? bn : kBM;
     // at most one partial tile per expert beside the full ones
     const int64_t tiles = std::min<int64_t>(a.experts, routes) + routes / tile;
@@ -1093,13 +1148,14 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     P.act_scales_in = s.act_scales;
     P.down_scales = a.down_scales;
     P.offsets = s.offsets;
-    P.row_token = s.perm_token;
+    P.row_token = s.row_token;
     P.experts = a.experts;
     P.hidden = a.hidden;
     P.inner = a.inner;
     P.act = s.act;
     P.act_scales = s.act_scales;
     P.y = s.y;
+    P.y_f32 = experts_fp8_wide_rows(routes);
     P.work = s.counters;
     P.done = s.counters + 1;
     P.status = status;
@@ -1111,9 +1167,13 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     }
     if (rc) return rc;
     const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 255) / 256;
-    return launch_pdl(fp8_combine_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, stream,
-                      "fp8_combine_kernel", static_cast<const uint16_t *>(s.y),
-                      static_cast<const int32_t *>(s.route_pos), a.weights, a.tokens, a.top_k, a.hidden, a.out);
+    const dim3 grid(static_cast<unsigned>(ctas)), block(256);
+    const int32_t *pos = s.route_pos;
+    if (!P.y_f32)
+        return launch_pdl(fp8_combine_kernel<uint16_t>, grid, block, 0, stream, "fp8_combine_kernel",
+                          static_cast<const uint16_t *>(s.y), pos, a.weights, a.tokens, a.top_k, a.hidden, a.out);
+    return launch_pdl(fp8_combine_kernel<float>, grid, block, 0, stream, "fp8_combine_kernel",
+                      static_cast<const float *>(s.y), pos, a.weights, a.tokens, a.top_k, a.hidden, a.out);
 }
 
 }  // namespace lrb

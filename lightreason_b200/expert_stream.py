@@ -29,8 +29,8 @@ three residencies:
 A fourth trades the bit-exact BF16 arithmetic for half the weight bytes:
   "b200-fp8"     experts in HBM as e4m3 with an FP32 scale per 128 x 128 block
                  (lightreason_b200.fp8), the hidden states brought to e4m3 per
-                 row and 128 columns on each call; sums in FP32, one expert's
-                 row rounded to BF16 before the weighted sum.
+                 row and 128 columns on each call; sums in FP32, on large batches
+                 each route's row rounded to BF16 before the weighted sum.
 With capacity_bytes > 0 the host residencies keep up to capacity_bytes of
 experts per layer in HBM slots across calls (a device-side LRU, the role of
 the reference pool's byte-bounded row cache, expert_stream.py:132-174): only

@@ -63,33 +63,33 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Two e4m3 values (the low 16 bits) as FP32; exact.
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
-    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
-}
-__device__ __forceinline__ void unpack16(uint4 v, float (&f)[16]) {
+// Sixteen e4m3 values as FP16 (exact).
+__device__ __forceinline__ void halves16(uint4 v, uint16_t (&f)[16]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack2(w[i] & 0xffff), b = unpack2(w[i] >> 16);
+        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xffff), __NV_E4M3);
+        const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3);
         f[4 * i] = a.x;
         f[4 * i + 1] = a.y;
         f[4 * i + 2] = b.x;
         f[4 * i + 3] = b.y;
     }
 }
-// dot(16 e4m3 weights, 16 FP32 activations) in FP32.
-__device__ __forceinline__ float dot16(uint4 w, const float (&x)[16]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// acc + x * y with FP16 factors in one FP32 FMA (the product is exact).
+__device__ __forceinline__ float fma_f16(uint16_t x, uint16_t y, float acc) {
+    asm("fma.rn.f32.f16 %0, %1, %2, %0;" : "+f"(acc) : "h"(x), "h"(y));
+    return acc;
+}
+// dot(16 e4m3 weights, 16 FP16 activations) in FP32.
+__device__ __forceinline__ float dot16(uint4 w, const uint16_t (&x)[16]) {
+    uint16_t f[16];
+    halves16(w, f);
     float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 lo = unpack2(u[i] & 0xffff), hi = unpack2(u[i] >> 16);
-        a = fmaf(lo.x, x[4 * i], a);
-        b = fmaf(lo.y, x[4 * i + 1], b);
-        a = fmaf(hi.x, x[4 * i + 2], a);
-        b = fmaf(hi.y, x[4 * i + 3], b);
+    for (int i = 0; i < 16; i += 2) {
+        a = fma_f16(f[i], x[i], a);
+        b = fma_f16(f[i + 1], x[i + 1], b);
     }
     return a + b;
 }

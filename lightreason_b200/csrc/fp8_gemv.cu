@@ -1,6 +1,6 @@
 // The FP8 products at the smallest sizes: a warp per weight row (or pair of
-// rows), every lane a 16-byte piece of it, FP32 FMA over the unpacked e4m3
-// values.  The rows are the traffic: they are streamed once with all of a
+// rows), every lane a 16-byte piece of it, FP32 FMA over the e4m3 values
+// (widened to FP16, whose products an FP32 FMA takes exactly).  The rows are the traffic: they are streamed once with all of a
 // row's loads in flight, and the few activations come from L1 and L2.
 #include <algorithm>
 
@@ -11,7 +11,7 @@ namespace {
 
 using fp8::dot16;
 using fp8::kGroup;
-using fp8::unpack16;
+using fp8::halves16;
 
 constexpr int kWarps = 8;
 constexpr int kChunk = 32 * 16;  // weight bytes a warp reads per load
@@ -51,8 +51,8 @@ __global__ void __launch_bounds__(kWarps * 32) linear_gemv_kernel(LinearFp8 a) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     const int t = min(m0 + m, a.tokens - 1);
-                    float x[16];
-                    unpack16(ld_cached(a.x + static_cast<int64_t>(t) * a.cols + c), x);
+                    uint16_t x[16];
+                    halves16(ld_cached(a.x + static_cast<int64_t>(t) * a.cols + c), x);
                     acc[m] = fmaf(dot16(v[u], x), s * a.x_scales[static_cast<int64_t>(t) * gk + c / kGroup], acc[m]);
                 }
             }
@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kWarps * 32) gate_up_gemv_kernel(ExpertsFp8 a,
         for (int u = 0; u < kUnroll; ++u) {
             const int c = c0 + u * kChunk;
             if (c >= a.hidden) break;
-            float f[16];
-            unpack16(ld_cached(x + c), f);
+            uint16_t f[16];
+            halves16(ld_cached(x + c), f);
             const float s = xs[c / kGroup], g = s * gs[c / kGroup], up = s * us[c / kGroup];
             acc[0] = fmaf(dot16(v[u][0], f), g, acc[0]);
             acc[1] = fmaf(dot16(v[u][1], f), g, acc[1]);
@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32) gate_up_gemv_kernel(ExpertsFp8 a,
 // (the same values in every CTA).  The kernel follows gate_up_gemv_kernel,
 // which has seen every earlier kernel of the stream complete before it lets
 // this one start: the route ids and the weights are final then, so the first
-// 512 bytes of each route's row are on their way before the wait for h.
+// 512 bytes of each route's row, their scales and the routes' weights are on
+// their way before the wait for h.
 constexpr int kRoutes = 8;
 __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, const float *__restrict__ h,
                                                                 int blocks_per_token) {
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
         const int count = min(kRoutes, a.top_k - k0);
         int e[kRoutes];
         uint4 v[kRoutes];
+        float sc[kRoutes], rw[kRoutes];  // the lane's first scale and the weight of each route
 #pragma unroll
         for (int j = 0; j < kRoutes; ++j) {
             const int64_t id = j < count ? __ldcg(a.idx + t * a.top_k + k0 + j) : -1;
@@ -155,6 +157,12 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
 #pragma unroll
         for (int j = 0; j < kRoutes; ++j)
             v[j] = live && e[j] >= 0 && lane * 16 < a.inner ? ld_stream(row(j) + lane * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kRoutes; ++j) {
+            sc[j] = live && e[j] >= 0 && lane * 16 < a.inner
+                        ? __ldcg(a.down_scales + (static_cast<int64_t>(e[j]) * gn + n / kGroup) * gi + lane / 8) : 0.f;
+            rw[j] = e[j] >= 0 ? bf2f(__ldcg(a.weights + t * a.top_k + k0 + j)) : 0.f;
+        }
         if (k0 == 0) {
             grid_dependency_wait();
             grid_dependency_trigger();
@@ -204,11 +212,11 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
             float part = 0.f;
             for (int c = lane * 16; c < a.inner; c += kChunk) {
                 const uint4 w = c == lane * 16 ? v[j] : ld_stream(row(j) + c);
-                float f[16];
-                unpack16(*reinterpret_cast<const uint4 *>(act + j * a.inner + c), f);
-                part = fmaf(dot16(w, f), ws[c / kGroup] * acts[j * gi + c / kGroup], part);
+                uint16_t f[16];
+                halves16(*reinterpret_cast<const uint4 *>(act + j * a.inner + c), f);
+                part = fmaf(dot16(w, f), (c == lane * 16 ? sc[j] : ws[c / kGroup]) * acts[j * gi + c / kGroup], part);
             }
-            acc = fmaf(part, bf2f(a.weights[t * a.top_k + k0 + j]), acc);
+            acc = fmaf(part, rw[j], acc);
         }
     }
     if (!live) return;

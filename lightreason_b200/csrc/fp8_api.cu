@@ -77,7 +77,7 @@ extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uin
                 "moe_linear_fp8: workspace of %zu bytes (256-byte aligned) required", need);
     if (int rc = require_sm100()) return rc;
     const LinearFp8 a{x, x_scales, w, w_scales, tokens, rows, cols, out, out_f32};
-    if (tokens <= kGemvTokens) return launch_linear_fp8_gemv(a, as_stream(stream));
+    if (plan_linear_fp8(tokens, rows, cols).gemv) return launch_linear_fp8_gemv(a, as_stream(stream));
     return launch_linear_fp8_tiles(a, status, as_stream(stream));
 }
 

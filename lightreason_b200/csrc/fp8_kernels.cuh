@@ -52,6 +52,13 @@ struct ExpertsFp8Scratch {
 int experts_fp8_tile(int routes, int experts);
 // Whether a route's down row is kept in FP32 until the weighted sum.
 bool experts_fp8_wide_rows(int routes);
+// How a plain product is cut: rows of x per tile, CTAs that share a tile's
+// columns of x, or the GEMV kernel.
+struct LinearFp8Plan {
+    int tile, split;
+    bool gemv;
+};
+LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols);
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream);
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream);
 

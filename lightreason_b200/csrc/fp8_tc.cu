@@ -41,6 +41,7 @@
 // launch, 64,512 a CTA either way).  Every wait is bounded; a timeout raises
 // *status, drains what is in flight and returns.
 #include <algorithm>
+#include <cmath>
 
 #include "fp8_kernels.cuh"
 #include "sm100.cuh"
@@ -92,6 +93,7 @@ struct Params {
     int rows, n, k;                    // T, weight rows, columns
     void *out;                         // [T, n]
     int out_f32;
+    int split;                         // CTAs of a cluster that share an item's groups
     // experts
     const float *act_scales_in, *down_scales;  // phase 2: [R, I / 128], [E, blocks, I / 128]
     const int32_t *offsets;                    // [E + 1]
@@ -227,12 +229,13 @@ __device__ __forceinline__ void store32(void *p, const uint32_t *v) {
 // tm_x: linear, the row tiles; experts, the token rows (gathered).  tm_r, tm_r16:
 // full and 16-row boxes of the rows of linear or phase 2.  tm_w, tm_w2: weights
 // of linear or phase 1, and of phase 2.  tm_out: linear's BF16 output.
-template <bool LIN, int BN>
+template <bool LIN, int BN, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_r,
                     const __grid_constant__ CUtensorMap tm_r16, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ CUtensorMap tm_out,
                     const Params P) {
+    static_assert(LIN || !SPLIT, "only the plain product is split");
     using S = Shape<LIN, BN>;
     constexpr bool kSwap = S::kSwap;
     constexpr int kRows = S::kRows;
@@ -324,6 +327,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         items1 = nt1 * tail->tiles[P.experts];
         total = items1 + nt2 * tail->tiles[P.experts];
     }
+    // SPLIT: this CTA's groups of its cluster's one item; else all of an item's
+    const int rank = SPLIT ? static_cast<int>(sm100::cluster_ctarank()) : 0;
+    const int split0 = SPLIT ? kbs2 * rank / P.split : 0, split1 = SPLIT ? kbs2 * (rank + 1) / P.split : kbs2;
     auto decode = [&](int item) {
         Item r;
         if (item >= total) {
@@ -358,11 +364,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // The item after the last one this warp took: linear, the CTA's next of a
     // fixed order; experts, from the ring that warp 0 fills.
-    int take_at = LIN ? blockIdx.x : 0;
+    int take_at = SPLIT ? blockIdx.x / P.split : LIN ? blockIdx.x : 0;
     auto take_item = [&]() {
         if constexpr (LIN) {
             const Item r = decode(take_at);
-            take_at += gridDim.x;
+            take_at += SPLIT ? total : gridDim.x;
             return r;
         } else {
             const int slot = take_at % kRing;
@@ -422,9 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 const bool p1 = !LIN && it.phase == 1;
                 const uint64_t policy = it.mt > 1 ? keep : once;  // other tiles read the same weight rows
-                const int kbs = p1 ? kbs1 : kbs2;
+                const int kbs = p1 ? kbs1 : split1;
                 const int r0 = it.n * (p1 ? kGroup : kBN), r1 = p1 ? P.inner + r0 : r0 + 128;
-                for (int kb = 0; kb < kbs; ++kb) {
+                for (int kb = split0; kb < kbs; ++kb) {
                     ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
                     if (!ok) break;
                     uint8_t *b = smem + stage * S::kStage;
@@ -452,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t buf = 0, bphase = 0;
             bool ok = true, any = false;
             for (Item it = take_item(); ok && it.phase; it = take_item()) {
-                const int kbs = !LIN && it.phase == 1 ? kbs1 : kbs2;
+                const int kbs = !LIN && it.phase == 1 ? kbs1 : split1 - split0;
                 const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kSwap ? (it.count + 15) & ~15 : kBN);
                 for (int kb = 0; kb < kbs; ++kb) {
                     ok = wait_bar(&tail->tempty[buf], bphase ^ 1, abort) && wait_bar(&tail->full[stage], phase, abort);
@@ -543,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int kbs = p1 ? kbs1 : kbs2;
                 const float *rs = LIN || p1 ? P.x_scales : P.act_scales_in;
                 const float *bs = LIN || p1 ? P.w_scales : P.down_scales;
-                const bool quads = kbs % 4 == 0 && ((reinterpret_cast<uintptr_t>(rs) | reinterpret_cast<uintptr_t>(bs)) & 15) == 0;
+                const bool quads = kbs % 4 == 0 && ((reinterpret_cast<uintptr_t>(rs) | reinterpret_cast<uintptr_t>(bs)) & 15) == 0 &&
+                                   (!SPLIT || split0 % 4 == 0);
                 if (!LIN && !p1) {
                     // the expert's activations: every epilogue warp of its phase-1 items
                     const int need = 8 * nt1 * it.mt;
@@ -564,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int boxes = p1 ? min(kPerWarp / 4, (max(0, it.count - kPerWarp * (warp - 2)) + 3) / 4)
                                      : it.count == kRows ? 1 : (it.count + 15) / 16;
                 const int box_bytes = p1 ? 4 * kGroup : it.count == kRows ? S::kATile : 16 * kGroup;
-                for (int kb = 0; kb < kbs; ++kb) {
-                    if (warp == 3 && (kb & 3) == 0) {
+                for (int kb = split0; kb < (p1 ? kbs1 : split1); ++kb) {
+                    if (warp == 3 && ((kb - split0) & 3) == 0) {
                         // the scales of groups kb .. kb + 3, on their way from here
                         ok = wait_warp(&tail->sempty[slot], sphase ^ 1, abort);
                         if (!ok) break;
@@ -616,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int q = warp & 3, h = warp >= 8;  // TMEM lanes 32q..; half of the columns
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * q) << 16);
+        float *partial = reinterpret_cast<float *>(smem);  // SPLIT: the stages, when all of them are used
         uint32_t slot = 0, sphase = 0, buf = 0, bphase = 0, iphase = 0;
         auto next_buf = [&] {
             sm100::tc_fence_before();
@@ -648,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int j0 = NJ * h;
             for (Item it = take_item(); it.phase; it = take_item()) {
                 const bool p1 = !LIN && it.phase == 1;
-                const int kbs = p1 ? kbs1 : kbs2;
+                const int kbs = p1 ? kbs1 : split1 - split0;
                 const bool active = j0 < it.count;
                 float acc0[NJ], acc1[NJ];
 #pragma unroll
@@ -712,6 +720,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         iphase ^= 1;
                     }
                     count_in(it);
+                } else if (SPLIT) {
+                    // partial sums [row][weight row] for the cluster
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        partial[(j0 + j) * kBN + 32 * q + lane] = acc0[j];
+                        partial[(j0 + j) * kBN + 128 + 32 * q + lane] = acc1[j];
+                    }
                 } else if (active) {
                     const int c0 = it.n * kBN + 32 * q + lane;
                     const bool f32 = LIN ? P.out_f32 : P.y_f32;
@@ -754,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             while (next.phase) {
                 const Item it = next;
                 const bool p1 = !LIN && it.phase == 1;
-                const int kbs = p1 ? kbs1 : kbs2;
+                const int kbs = p1 ? kbs1 : split1 - split0;
                 const bool active = 32 * q < it.count;  // the warp has rows of the tile
                 float acc[128];
 #pragma unroll
@@ -824,6 +839,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (h == 0 && lane < rows) P.act_scales[(first + lane) * nt1 + it.n] = fp8::scale_of(top);
                     }
                     count_in(it);
+                } else if (SPLIT) {
+                    // partial sums [weight row][row] for the cluster
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) partial[(128 * h + i) * kBM + r] = acc[i];
                 } else if (active) {
                     const int n0 = it.n * kBN + 128 * h;
                     const bool f32 = LIN && P.out_f32;
@@ -889,6 +908,80 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         sm100::tc_fence_before();
+    }
+    if constexpr (SPLIT) {
+        // Every CTA has its partial sums in shared memory; each adds up and
+        // stores an equal part of the tile's columns, in rank order.
+        __syncwarp();
+        sm100::cluster_sync();
+        if (warp >= 4) {
+            const Item it = decode(blockIdx.x / P.split);
+            const int tid = threadIdx.x - 128, cols = kBN / P.split;
+            const uint32_t base = sm100::smem_u32(smem);
+            // sums of N places, `step` apart, of every CTA: a CTA's N loads in flight together
+            auto sums = [&](auto &v, int at, int step) {
+#pragma unroll
+                for (float &x : v) x = 0.f;
+                for (int c = 0; c < P.split; ++c) {
+                    const uint32_t from = sm100::mapa_u32(base, c) + 4 * at;
+                    constexpr int N = sizeof(v) / sizeof(float);
+                    float w[N];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) w[i] = sm100::ld_cluster_f32(from + 4 * i * step);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[i] += w[i];
+                }
+            };
+            uint16_t *y = static_cast<uint16_t *>(P.out);
+            float *z = static_cast<float *>(P.out);
+            if constexpr (kSwap) {
+                // column tid % cols of this CTA's; rows tid / cols, + step, ...
+                const int step = 256 / cols, c = tid % cols + rank * cols, n = it.n * kBN + c;
+                for (int j = tid / cols; j < it.count; j += 4 * step) {
+                    float v[4];  // places past the tile's rows are still in the stages, and not stored
+                    sums(v, j * kBN + c, step * kBN);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t o = static_cast<int64_t>(it.row0 + j + i * step) * n2 + n;
+                        if (n >= n2 || j + i * step >= it.count) continue;
+                        if (P.out_f32) z[o] = v[i];
+                        else y[o] = f2bf(v[i]);
+                    }
+                }
+            } else {
+                const int r = tid & 127;
+                const bool vec = n2 % (P.out_f32 ? 4 : 8) == 0;
+                for (int c = rank * cols + (tid >> 7) * (cols / 2), end = c + cols / 2; c < end; c += 16) {
+                    const int n = it.n * kBN + c;
+                    if (r >= it.count || n >= n2) continue;
+                    float v[16];
+                    sums(v, c * kBM + r, kBM);
+                    const int64_t o = static_cast<int64_t>(it.row0 + r) * n2 + n;
+                    if (vec && P.out_f32) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            if (n + i < n2)
+                                *reinterpret_cast<float4 *>(z + o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    } else if (vec) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8)
+                            if (n + i < n2)
+                                *reinterpret_cast<uint4 *>(y + o + i) =
+                                    make_uint4(fp8::pack_bf16(v[i], v[i + 1]), fp8::pack_bf16(v[i + 2], v[i + 3]),
+                                               fp8::pack_bf16(v[i + 4], v[i + 5]), fp8::pack_bf16(v[i + 6], v[i + 7]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            if (n + i >= n2) continue;
+                            if (P.out_f32) z[o + i] = v[i];
+                            else y[o + i] = f2bf(v[i]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        sm100::cluster_sync();  // no CTA leaves while another reads its sums
     }
     if (*abort && warp < 4) {
         // loads may be in flight whose barriers will never complete: give them
@@ -1033,8 +1126,33 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const Y *__restrict__ 
 template <bool LIN, int BN>
 int launch_tile(const CUtensorMap (&m)[6], const Params &P, int64_t items, cudaStream_t stream) {
     constexpr int smem = Shape<LIN, BN>::kSmem;
-    if (int rc = ensure_dynamic_smem(fp8_tile_kernel<LIN, BN>, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
-    return launch_pdl(fp8_tile_kernel<LIN, BN>, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
+    if constexpr (LIN) {
+        if (P.split > 1) {
+            static_assert(Shape<LIN, BN>::kStages * Shape<LIN, BN>::kStage >= Shape<LIN, BN>::kRows * kBN * 4,
+                          "the partial sums fit the stages");
+            auto kernel = fp8_tile_kernel<LIN, BN, true>;
+            if (int rc = ensure_dynamic_smem(kernel, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(items * P.split));
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = P.split;
+            attr[1].val.clusterDim.y = 1;
+            attr[1].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], m[4], m[5], P);
+            return err == cudaSuccess ? MOE_OK : cuda_error(err, "fp8_tile_kernel");
+        }
+    }
+    auto kernel = fp8_tile_kernel<LIN, BN, false>;
+    if (int rc = ensure_dynamic_smem(kernel, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
                       dim3(kThreads), smem, stream, "fp8_tile_kernel", m[0], m[1], m[2], m[3], m[4], m[5], P);
 }
 
@@ -1075,10 +1193,55 @@ int out_map(CUtensorMap *m, const void *base, int rows, int cols) {
 
 }  // namespace
 
+// The least of a few estimates, in microseconds, fitted to graph replays on a
+// B200 (weights of 1024 x 2048, 1000 x 1040, 2048 x 512, 4096 x 4096, 8192 x
+// 8192 and 512 x 8192, 1 to 512 rows; off by a fifth at most):
+//  - tiles: 5.5, plus a group's time for every group in a CTA's row of items, plus
+//    what the tile's epilogue and, with a split, the cluster's sum take; and no
+//    less than the tiles' traffic at 9 TB/s from L2.  Clusters of eight are
+//    limited to eight of them: sixteen do not all fit at once.
+//  - a warp per weight row, up to four rows of x: 4.2 plus the longest of the
+//    multiplications, the weights from HBM, and a warp's chain of loads.
+// At 77 rows of 1040 against 1000: tiles of 16 in one piece 9.1, of 128 12.7; at
+// 64 of 8192 against 512: tiles of 16 split eight ways 11.1, of 64 in one piece
+// 38.3; at 16 of 512 against 2048: in one piece 6.5, split in two 8.6.
+LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols) {
+    constexpr int kTiles[4] = {16, 32, 64, kBM};
+    constexpr double kGroupUs[4] = {0.33, 0.36, 0.45, 0.55}, kEndUs[4] = {0, 0.4, 1.6, 1.7},
+                     kSplitUs[4] = {2.8, 2.9, 3.3, 4.5};
+    constexpr int kMostCtas[4] = {148, 148, 128, 64};  // of a split 1, 2, 4, 8
+    const double kbs = fp8::groups(cols), nt = (rows + kBN - 1) / kBN;
+    LinearFp8Plan best{kBM, 1, false};
+    double least = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const double items = nt * ((tokens + kTiles[i] - 1) / kTiles[i]);
+        const double floor = items * kbs * kGroup * (kBN + kTiles[i]) / 9e6;
+        for (int p = 0; p < 4; ++p) {
+            const int split = 1 << p;
+            if (p && (kbs < 2 * split || items * split > kMostCtas[p])) break;
+            const double waves = std::ceil(items * split / 148);
+            const double us = std::max(floor, waves * std::ceil(kbs / split) * kGroupUs[i]) + 5.5 +
+                              (p ? kSplitUs[i] : kEndUs[i]);
+            if (us < least) {
+                least = us;
+                best = LinearFp8Plan{kTiles[i], split, false};
+            }
+        }
+    }
+    if (tokens <= kGemvTokens) {
+        const double macs = static_cast<double>(rows) * cols;
+        const double us = 4.2 + std::max(std::max(macs * tokens * 1.05e-7, macs / 6.4e6),
+                                         cols / 2048.0 * (0.5 + 0.45 * tokens));
+        best.gemv = us < least;
+    }
+    return best;
+}
+
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream) {
-    const int bn = a.tokens <= 16 ? 16 : a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : 0;
+    const LinearFp8Plan plan = plan_linear_fp8(a.tokens, a.rows, a.cols);
+    const int tile = plan.tile, bn = tile == kBM ? 0 : tile;
     CUtensorMap m[6]{};
-    if (int rc = row_maps(&m[1], &m[2], a.x, a.tokens, a.cols, bn ? bn : kBM)) return rc;
+    if (int rc = row_maps(&m[1], &m[2], a.x, a.tokens, a.cols, tile)) return rc;
     m[0] = m[1];
     const uint64_t dims[2] = {static_cast<uint64_t>(a.cols), static_cast<uint64_t>(a.rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(a.cols)};
@@ -1096,7 +1259,7 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
     P.out = a.out;
     P.out_f32 = a.out_f32;
     P.status = status;
-    const int tile = bn ? bn : kBM;
+    P.split = plan.split;
     const int64_t items = static_cast<int64_t>((a.tokens + tile - 1) / tile) * ((a.rows + kBN - 1) / kBN);
     LRB_REQUIRE(items < (1ll << 31), "moe_linear_fp8: too many tiles");
     switch (bn) {

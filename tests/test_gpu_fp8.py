@@ -234,6 +234,11 @@ LINEAR_SHAPES = [(1, 1, 16), (1, 1024, 2048), (2, 100, 144), (3, 130, 2064), (4,
                  (300, 72, 1024), (513, 1024, 1168), (1000, 511, 2048), (2048, 2048, 512), (1, 8200, 16),
                  (300, 3, 48), (6, 20000, 128)]
 
+# every row tile with every split over the columns, and widths that end inside a 16-byte unit
+LINEAR_SHAPES += [(5, 2500, 7488), (5, 17000, 2064), (50, 2048, 3552), (129, 1000, 2096), (257, 2048, 6192),
+                  (65, 2048, 10720), (200, 4097, 2240), (400, 4097, 1056), (257, 4097, 2560), (65, 4097, 3280),
+                  (257, 2052, 5120), (3000, 1001, 256), (2500, 2052, 272), (2, 8192, 8192), (4, 512, 8192)]
+
 
 @pytest.mark.parametrize("tokens,rows,cols", LINEAR_SHAPES)
 def test_linear(dev, tokens, rows, cols):

@@ -21,29 +21,40 @@ the caller keeps.
 
 from __future__ import annotations
 
+import ctypes
+import importlib.util
 from functools import lru_cache
 
 import torch
 
-from lightreason_b200 import native
+from lightreason_b200 import build, native
 from lightreason_b200.native import _require
 
 GROUP = 128
 E4M3 = torch.float8_e4m3fn
 _BF16, _F32 = torch.bfloat16, torch.float32
 
-# These calls sit in decode loops that may run uncaptured, where a few
-# microseconds of Python a call show: the stream comes from torch's raw getter,
-# sizes of workspaces are remembered per shape, and a tensor is checked in one
-# expression.
+# These calls sit in decode loops that may run uncaptured, where the checks of a
+# call's tensors in Python would take longer than its launch.  Each goes to its
+# namesake in _fp8_bind (csrc/fp8_bind.cpp), which makes the same checks and the
+# call.  What it does not take comes back as None: the Python below then goes
+# through the checks one by one and raises at the first that fails.
 
 
-def _device() -> int:
-    return torch._C._cuda_getDevice()
-
-
-def _stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+@lru_cache(maxsize=1)
+def _bind():
+    """The module, with the C ABI's addresses in the loaded library."""
+    path = str(build.BIND)
+    if not build.BIND.exists():
+        raise RuntimeError(f"{path} is missing: build it with `python -m lightreason_b200.build`")
+    spec = importlib.util.spec_from_file_location("_fp8_bind", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    so = native.lib()
+    module.bind(*(ctypes.cast(getattr(so, name), ctypes.c_void_p).value for name in (
+        "moe_rmsnorm_fp8", "moe_quantize_fp8_blocks", "moe_linear_fp8", "moe_linear_fp8_workspace_bytes",
+        "moe_experts_fp8", "moe_experts_fp8_workspace_bytes")))
+    return module
 
 
 def _groups(n: int) -> int:
@@ -56,24 +67,11 @@ def _check(t, name: str, dtype: torch.dtype, shape: tuple, index: int) -> None:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on cuda:{index}")
 
 
-def _check_all(checks, index: int) -> None:
-    """_check of every (tensor, name, dtype, shape), in one loop."""
-    for t, name, dtype, shape in checks:
-        if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
-            _check(t, name, dtype, shape, index)
-
-
-def _call(name: str, index: int, args: tuple) -> None:
-    """Entry point `name` on device `index` and its current stream (the last
-    argument of every entry point)."""
-    fn = getattr(native.lib(), name)
-    if _device() == index:
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
-    if rc:
-        native.check(rc, name)
+def _refused(name: str, status) -> None:
+    """The end of a call that _fp8_bind did not answer with a result."""
+    if status is None:
+        raise ValueError(f"{name}: arguments out of range")
+    native.check(status, name)
 
 
 def _no_grad(*tensors) -> None:
@@ -97,18 +95,19 @@ def _rows(t: torch.Tensor, name: str) -> int:
 def quantize_rows(x: torch.Tensor, *, out=None):
     """BF16 rows [T, H] (any row stride) -> (q e4m3 [T, H], scales f32
     [T, ceil(H / 128)]).  out: the same pair, to be written."""
-    stride = _rows(x, "x")
+    if out is None and isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_cuda:
+        out = (torch.empty(x.shape, dtype=E4M3, device=x.device),
+               torch.empty((x.shape[0], _groups(x.shape[1])), dtype=_F32, device=x.device))
+    q, scales = out if out is not None else (None, None)
+    done = _bind().rows(x, None, None, 0.0, 0.0, q, scales, None, None)
+    if done is True:
+        return q, scales
+    _rows(x, "x")
     _no_grad(x)
-    tokens, hidden = x.shape
-    index, groups = x.get_device(), _groups(hidden)
-    if out is None:
-        out = (torch.empty((tokens, hidden), dtype=E4M3, device=x.device),
-               torch.empty((tokens, groups), dtype=_F32, device=x.device))
-    q, scales = out
-    _check_all(((q, "out[0]", E4M3, x.shape), (scales, "out[1]", _F32, (tokens, groups))), index)
-    _call("moe_rmsnorm_fp8", index, (x.data_ptr(), stride, None, 0, None, 0.0, 0.0, tokens, hidden, q.data_ptr(),
-                                     scales.data_ptr(), None, None))
-    return q, scales
+    index = x.get_device()
+    _check(q, "out[0]", E4M3, x.shape, index)
+    _check(scales, "out[1]", _F32, (x.shape[0], _groups(x.shape[1])), index)
+    _refused("moe_rmsnorm_fp8", done)
 
 
 def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -119,70 +118,51 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     (None without a residual).  weight_offset: 1 for Qwen3_5MoeRMSNorm, whose
     weight is stored around zero; 0 for plain norms.  out: the same four, to be
     written; its residual_out may be `residual` itself and its normed `x`."""
-    stride = _rows(x, "x")
-    tokens, hidden = shape = x.shape
-    index, groups = x.get_device(), _groups(hidden)
-    _no_grad(x, weight, residual)
-    rstride = 0
-    if residual is not None:
-        rstride = _rows(residual, "residual")
-        _require(residual.shape == shape and residual.get_device() == index,
-                 "residual must have x's shape and device")
-    if out is None:
-        dev = x.device
-        out = (torch.empty(shape, dtype=E4M3, device=dev), torch.empty((tokens, groups), dtype=_F32, device=dev),
+    if out is None and isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_cuda:
+        shape, dev = x.shape, x.device
+        out = (torch.empty(shape, dtype=E4M3, device=dev),
+               torch.empty((shape[0], _groups(shape[1])), dtype=_F32, device=dev),
                torch.empty(shape, dtype=_BF16, device=dev) if normed else None,
                torch.empty(shape, dtype=_BF16, device=dev) if residual is not None else None)
-    q, scales, y, r = out
-    _check_all(((weight, "weight", _BF16, (hidden,)), (q, "out[0]", E4M3, shape),
-                (scales, "out[1]", _F32, (tokens, groups))), index)
+    q, scales, y, r = out if out is not None else (None, None, None, None)
+    done = _bind().rows(x, weight, residual, eps, weight_offset, q, scales, y, r) if weight is not None else None
+    if done is True:
+        return q, scales, y, r
+    _rows(x, "x")
+    tokens, hidden = shape = x.shape
+    index = x.get_device()
+    _check(weight, "weight", _BF16, (hidden,), index)
+    _no_grad(x, weight, residual)
+    if residual is not None:
+        _rows(residual, "residual")
+        _require(residual.shape == shape and residual.get_device() == index,
+                 "residual must have x's shape and device")
+    _check(q, "out[0]", E4M3, shape, index)
+    _check(scales, "out[1]", _F32, (tokens, _groups(hidden)), index)
     if y is not None:
         _check(y, "out[2]", _BF16, shape, index)
     if r is not None:
         _require(residual is not None, "out[3] without a residual")
         _check(r, "out[3]", _BF16, shape, index)
-    _call("moe_rmsnorm_fp8", index,
-          (x.data_ptr(), stride, None if residual is None else residual.data_ptr(), rstride, weight.data_ptr(),
-           weight_offset, eps, tokens, hidden, q.data_ptr(), scales.data_ptr(), None if y is None else y.data_ptr(),
-           None if r is None else r.data_ptr()))
-    return out
+    _refused("moe_rmsnorm_fp8", done)
 
 
 def quantize_blocks(w: torch.Tensor, *, out=None):
     """BF16 weights [N, K] or [banks, N, K] -> (q e4m3, scales f32 [(banks,)
     ceil(N / 128), ceil(K / 128)])."""
-    if not (w.is_cuda and w.dtype is _BF16 and w.dim() in (2, 3) and w.is_contiguous()):
-        raise ValueError("w must be a contiguous CUDA BF16 [N, K] or [banks, N, K] tensor")
+    q, scales = out if out is not None else (None, None)
+    done = _bind().blocks(w, q, scales)
+    if isinstance(done, tuple):
+        return done
+    _require(isinstance(w, torch.Tensor) and w.is_cuda and w.dtype is _BF16 and w.dim() in (2, 3)
+             and w.is_contiguous(), "w must be a contiguous CUDA BF16 [N, K] or [banks, N, K] tensor")
     _no_grad(w)
     shape = w.shape
-    rows, cols = shape[-2], shape[-1]
-    banks = shape[0] if len(shape) == 3 else 1
-    _require(rows >= 1 and cols >= 1, "w has no rows or columns")
-    index = w.get_device()
-    blocks = (_groups(rows), _groups(cols)) if len(shape) == 2 else (banks, _groups(rows), _groups(cols))
-    if out is None:
-        out = (torch.empty(shape, dtype=E4M3, device=w.device), torch.empty(blocks, dtype=_F32, device=w.device))
-    else:
-        _check(out[0], "out[0]", E4M3, shape, index)
-        _check(out[1], "out[1]", _F32, blocks, index)
-    _call("moe_quantize_fp8_blocks", index, (w.data_ptr(), banks, rows, cols, out[0].data_ptr(), out[1].data_ptr()))
-    return out
-
-
-@lru_cache(maxsize=4096)
-def _linear_workspace(*sizes) -> int:
-    return native.lib().moe_linear_fp8_workspace_bytes(*sizes)
-
-
-@lru_cache(maxsize=4096)
-def _experts_workspace(*sizes) -> int:
-    return native.lib().moe_experts_fp8_workspace_bytes(*sizes)
-
-
-def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    """Scratch from torch's allocator for one call: calls never share it, and a
-    captured graph keeps its own in the graph's pool."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _require(shape[-2] >= 1 and shape[-1] >= 1, "w has no rows or columns")
+    if out is not None:
+        _check(q, "out[0]", E4M3, shape, w.get_device())
+        _check(scales, "out[1]", _F32, (*shape[:-2], _groups(shape[-2]), _groups(shape[-1])), w.get_device())
+    _refused("moe_quantize_fp8_blocks", done)
 
 
 def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *,
@@ -192,29 +172,27 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
     scales stand for -> [T, N] in BF16 or FP32 (out_dtype, or out's).  K must be
     a multiple of 16.  status: a device int32 [1] that becomes 1 if a bounded
     wait inside a kernel gave up (the output is then not valid)."""
-    if not (x.is_cuda and x.dim() == 2 and w.dim() == 2):
-        raise ValueError("x and w must be CUDA [T, K] and [N, K] tensors")
-    tokens, cols = x.shape
-    rows, index, groups = w.shape[0], x.get_device(), _groups(cols)
-    if rows < 1 or cols < 16 or cols % 16:
-        raise ValueError("K must be a positive multiple of 16 and N positive")
-    _check_all(((x, "x", E4M3, (tokens, cols)), (x_scales, "x_scales", _F32, (tokens, groups)),
-                (w, "w", E4M3, (rows, cols)), (w_scales, "w_scales", _F32, (_groups(rows), groups))), index)
     if out is None:
         _require(out_dtype in (_BF16, _F32), "out_dtype must be BF16 or FP32")
-        out = torch.empty((tokens, rows), dtype=out_dtype, device=x.device)
-    else:
+    done = _bind().linear(x, x_scales, w, w_scales, out, out_dtype is _F32, status)
+    if isinstance(done, torch.Tensor):
+        return done
+    _require(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.is_cuda and x.dim() == 2
+             and w.dim() == 2, "x and w must be CUDA [T, K] and [N, K] tensors")
+    tokens, cols = x.shape
+    rows, index, groups = w.shape[0], x.get_device(), _groups(cols)
+    _require(rows >= 1 and cols >= 16 and cols % 16 == 0, "K must be a positive multiple of 16 and N positive")
+    _check(x, "x", E4M3, (tokens, cols), index)
+    _check(x_scales, "x_scales", _F32, (tokens, groups), index)
+    _check(w, "w", E4M3, (rows, cols), index)
+    _check(w_scales, "w_scales", _F32, (_groups(rows), groups), index)
+    if out is not None:
         _require(out.dtype in (_BF16, _F32), "out must be BF16 or FP32")
         _check(out, "out", out.dtype, (tokens, rows), index)
     if status is not None:
         _check(status, "status", torch.int32, (1,), index)
-    nbytes = _linear_workspace(tokens, rows, cols)
-    ws = _workspace(nbytes, x.device)
-    _call("moe_linear_fp8", index,
-          (x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), tokens, rows, cols, out.data_ptr(),
-           out.dtype is _F32, None if ws is None else ws.data_ptr(), nbytes,
-           None if status is None else status.data_ptr()))
-    return out
+    _no_grad(x, x_scales, w, w_scales, out)
+    _refused("moe_linear_fp8", done)
 
 
 def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate_up_scales: torch.Tensor,
@@ -224,31 +202,29 @@ def experts(x: torch.Tensor, x_scales: torch.Tensor, gate_up: torch.Tensor, gate
     [E, 2I, H] and down [E, H, I] with their block scales, idx int64 [T, K]
     (ids outside [0, E) contribute nothing), weights BF16 [T, K] -> BF16 [T, H].
     H is a multiple of 16, I of 128.  status as in linear."""
-    if not (x.is_cuda and x.dim() == 2 and gate_up.dim() == 3 and down.dim() == 3 and idx.dim() == 2):
-        raise ValueError("expected x [T, H], gate_up [E, 2I, H], down [E, H, I] and idx [T, K] on a CUDA device")
+    done = _bind().experts(x, x_scales, gate_up, gate_up_scales, down, down_scales, idx, weights, out, status)
+    if isinstance(done, torch.Tensor):
+        return done
+    _require(all(isinstance(t, torch.Tensor) for t in (x, gate_up, down, idx)) and x.is_cuda and x.dim() == 2
+             and gate_up.dim() == 3 and down.dim() == 3 and idx.dim() == 2,
+             "expected x [T, H], gate_up [E, 2I, H], down [E, H, I] and idx [T, K] on a CUDA device")
     tokens, hidden = shape = x.shape
     index, groups = x.get_device(), _groups(hidden)
     count, inner, top_k = gate_up.shape[0], down.shape[2], idx.shape[1]
-    _check_all(((x, "x", E4M3, shape), (x_scales, "x_scales", _F32, (tokens, groups)),
-                (gate_up, "gate_up", E4M3, (count, 2 * inner, hidden)),
-                (gate_up_scales, "gate_up_scales", _F32, (count, _groups(2 * inner), groups)),
-                (down, "down", E4M3, (count, hidden, inner)),
-                (down_scales, "down_scales", _F32, (count, groups, _groups(inner))),
-                (idx, "idx", torch.int64, (tokens, top_k)), (weights, "weights", _BF16, (tokens, top_k))), index)
-    if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=x.device)
-    else:
+    _check(x, "x", E4M3, shape, index)
+    _check(x_scales, "x_scales", _F32, (tokens, groups), index)
+    _check(gate_up, "gate_up", E4M3, (count, 2 * inner, hidden), index)
+    _check(gate_up_scales, "gate_up_scales", _F32, (count, _groups(2 * inner), groups), index)
+    _check(down, "down", E4M3, (count, hidden, inner), index)
+    _check(down_scales, "down_scales", _F32, (count, groups, _groups(inner)), index)
+    _check(idx, "idx", torch.int64, (tokens, top_k), index)
+    _check(weights, "weights", _BF16, (tokens, top_k), index)
+    if out is not None:
         _check(out, "out", _BF16, shape, index)
     if status is not None:
         _check(status, "status", torch.int32, (1,), index)
-    nbytes = _experts_workspace(tokens, count, top_k, hidden, inner)
-    ws = _workspace(nbytes, x.device)
-    _call("moe_experts_fp8", index,
-          (x.data_ptr(), x_scales.data_ptr(), gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(),
-           down_scales.data_ptr(), idx.data_ptr(), weights.data_ptr(), tokens, count, top_k, hidden, inner,
-           out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-           None if status is None else status.data_ptr()))
-    return out
+    _no_grad(x_scales, gate_up_scales, down_scales, weights, out)
+    _refused("moe_experts_fp8", done)
 
 
 class ExpertBanks:

@@ -527,7 +527,8 @@ int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, ui
  * [T, cols] and w [rows, cols] stand for, products summed in FP32.  cols must
  * be a multiple of 16; x, w and out are 16-byte aligned.  The workspace query
  * may return 0: workspace may then be NULL.  status (device int32, or NULL) is
- * set to 1 if a bounded wait inside a kernel gave up; out is then not valid. */
+ * set to 1 if a bounded wait inside a kernel gave up; out then holds NaN (a
+ * linear: in the tiles concerned). */
 size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols);
 int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
                    int rows, int cols, void *out, int out_f32, void *workspace, size_t workspace_bytes,

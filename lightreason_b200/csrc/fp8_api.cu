@@ -44,7 +44,7 @@ Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
     l.offsets = take(sizeof(int32_t) * (experts + 1));
     l.row_token = take(sizeof(int32_t) * routes);
     l.route_pos = take(sizeof(int32_t) * routes);
-    l.counters = take(sizeof(int32_t) * (experts + 1));
+    l.counters = take(sizeof(int32_t) * (experts + 2));
     l.act = take(routes * inner);
     l.act_scales = take(routes * (inner / fp8::kGroup) * sizeof(float));
     l.y = take(routes * hidden * (experts_fp8_wide_rows(static_cast<int>(routes)) ? 4 : 2));

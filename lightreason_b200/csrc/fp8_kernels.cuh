@@ -43,7 +43,7 @@ struct ExpertsFp8Scratch {
     int32_t *offsets;    // [E + 1]
     int32_t *row_token;  // [T * K]
     int32_t *route_pos;  // [T, K]
-    int32_t *counters;   // [E + 1]: items handed out, and per expert the finished parts of gate/up items
+    int32_t *counters;   // [E + 2]: items handed out, per expert the finished parts of gate/up items, a wait gave up
     uint8_t *act;        // [T * K, I]
     float *act_scales;   // [T * K, I / 128]
     void *y;             // [T * K, H], BF16 or (experts_fp8_wide_rows) FP32

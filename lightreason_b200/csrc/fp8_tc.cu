@@ -39,9 +39,12 @@
 // groups at a time, up to four such requests in flight), 4-11 epilogue; the
 // first four hand registers to the others (104 and 200 a thread of 168 at
 // launch, 64,512 a CTA either way).  Every wait is bounded; a timeout raises
-// *status, drains what is in flight and returns.
+// *status, drains what is in flight and returns, and leaves NaN: in a linear's
+// tiles of that CTA, in all of an experts call's output.
 #include <algorithm>
 #include <cmath>
+
+#include <math_constants.h>
 
 #include "fp8_kernels.cuh"
 #include "sm100.cuh"
@@ -105,6 +108,7 @@ struct Params {
     int y_f32;
     int32_t *work;      // items handed out so far (zero at launch)
     int32_t *done;      // [E] epilogue warps that finished an item of phase 1 (zero at launch)
+    int32_t *gave_up;   // set to 1 when a wait gave up (zero at launch)
     int32_t *status;
 };
 
@@ -690,6 +694,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     next_buf();
                     if ((kb & 3) == 3 || kb + 1 == kbs) next_slot();
                 }
+                if (LIN && *abort) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc0[j] = acc1[j] = CUDART_NAN_F;
+                }
                 const int left = it.count - j0;  // rows of this warp, if below NJ
                 if (p1) {
                     if (active) {
@@ -812,6 +820,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (next.phase && (LIN || next.phase == it.phase)) {
                     take_scales(!LIN && next.phase == 1);
                     ready = true;
+                }
+                if (LIN && *abort) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) acc[i] = CUDART_NAN_F;
                 }
                 const int rows = it.count - 32 * q;  // of this warp, if below 32
                 const int64_t first = static_cast<int64_t>(it.row0) + 32 * q;
@@ -994,7 +1006,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tc_fence_after();
         sm100::tmem_dealloc(tmem, 512);
     }
-    if (threadIdx.x == 0 && *abort && P.status) atomicExch(P.status, 1);
+    if (threadIdx.x == 0 && *abort) {
+        if (P.status) atomicExch(P.status, 1);
+        if (!LIN) atomicExch(P.gave_up, 1);
+    }
 }
 
 // The experts' plan, by one CTA or a cluster of eight with an equal share of
@@ -1016,7 +1031,7 @@ __global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restric
     grid_dependency_wait();
     grid_dependency_trigger();
     if (cta == 0)
-        for (int i = x; i <= experts; i += threads) counters[i] = 0;
+        for (int i = x; i < experts + 2; i += threads) counters[i] = 0;
     __syncthreads();
     const int per = (routes + ctas - 1) / ctas, r0 = cta * per, r1 = min(routes, r0 + per);
     constexpr int kU = 4;  // routes of a thread in flight
@@ -1071,39 +1086,51 @@ __global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restric
 }
 
 // out[t] = sum over the token's routes, in slot order, of weight * row, in
-// FP32.  A thread per 8 columns of a token, eight (BF16) or four rows in flight.
+// FP32.  A thread per 8 columns of a token, eight rows in flight.  The first
+// routes' places and weights are there before the wait: the plan kernel and
+// whatever wrote the weights were complete when the tile kernel let this one
+// start.
 template <class Y>
-__global__ void __launch_bounds__(256) fp8_combine_kernel(const Y *__restrict__ y,
-                                                          const int32_t *__restrict__ route_pos,
-                                                          const uint16_t *__restrict__ weights, int tokens, int top_k,
-                                                          int hidden, uint16_t *__restrict__ out) {
-    constexpr bool kWide = sizeof(Y) == 4;
-    constexpr int kU = kWide ? 4 : 8;
-    grid_dependency_wait();
-    grid_dependency_trigger();
+__global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *__restrict__ y, const int32_t *route_pos,
+                                                          const uint16_t *weights, const int32_t *gave_up, int tokens,
+                                                          int top_k, int hidden, uint16_t *__restrict__ out) {
+    constexpr int kU = 8, kParts = sizeof(Y) / 2;  // 16-byte parts of 8 columns
     const int units = hidden / 8;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
     const int64_t t = i / units;
-    if (t >= tokens) return;
     const int c = static_cast<int>(i % units) * 8;
-    float acc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int k0 = 0; k0 < top_k; k0 += kU) {
-        uint4 v[kU][kWide ? 2 : 1];
-        float w[kU];
+    int pos[kU];
+    float w[kU];
+    auto routes = [&](int k0) {
 #pragma unroll
         for (int k = 0; k < kU; ++k) {
             const int64_t at = t * top_k + k0 + k;
-            const int p = k0 + k < top_k ? route_pos[at] : -1;
-            w[k] = p >= 0 ? bf2f(weights[at]) : 0.f;
-#pragma unroll
-            for (int h = 0; h < (kWide ? 2 : 1); ++h)
-                v[k][h] = p >= 0 ? ld_stream(y + static_cast<int64_t>(p) * hidden + c + 4 * h) : make_uint4(0, 0, 0, 0);
+            const bool there = t < tokens && k0 + k < top_k;
+            pos[k] = there ? __ldcg(route_pos + at) : -1;
+            w[k] = there ? bf2f(__ldcg(weights + at)) : 0.f;
         }
+    };
+    routes(0);
+    grid_dependency_wait();
+    grid_dependency_trigger();
+    if (t >= tokens) return;
+    const float zero = __ldcg(gave_up) ? CUDART_NAN_F : 0.f;
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = zero;
+    for (int k0 = 0; k0 < top_k; k0 += kU) {
+        if (k0) routes(k0);
+        uint4 v[kU][kParts];
+#pragma unroll
+        for (int k = 0; k < kU; ++k)
+#pragma unroll
+            for (int h = 0; h < kParts; ++h)
+                v[k][h] = pos[k] >= 0 ? ld_stream(y + static_cast<int64_t>(pos[k]) * hidden + c + 4 * h)
+                                      : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < kU; ++k) {
-            if constexpr (kWide) {
+            if (pos[k] < 0) continue;  // a weight of a dropped route may be anything
+            if constexpr (kParts == 2) {
                 const uint32_t u[8] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w,
                                        v[k][1].x, v[k][1].y, v[k][1].z, v[k][1].w};
 #pragma unroll
@@ -1321,6 +1348,7 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     P.y_f32 = experts_fp8_wide_rows(routes);
     P.work = s.counters;
     P.done = s.counters + 1;
+    P.gave_up = s.counters + 1 + a.experts;
     P.status = status;
     int rc = MOE_OK;
     switch (bn) {
@@ -1329,14 +1357,14 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
         default: rc = launch_tile<false, 0>(m, P, items, stream); break;
     }
     if (rc) return rc;
-    const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 255) / 256;
-    const dim3 grid(static_cast<unsigned>(ctas)), block(256);
-    const int32_t *pos = s.route_pos;
+    const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 127) / 128;
+    const dim3 grid(static_cast<unsigned>(ctas)), block(128);
+    const int32_t *pos = s.route_pos, *gave_up = P.gave_up;
     if (!P.y_f32)
         return launch_pdl(fp8_combine_kernel<uint16_t>, grid, block, 0, stream, "fp8_combine_kernel",
-                          static_cast<const uint16_t *>(s.y), pos, a.weights, a.tokens, a.top_k, a.hidden, a.out);
+                          static_cast<const uint16_t *>(s.y), pos, a.weights, gave_up, a.tokens, a.top_k, a.hidden, a.out);
     return launch_pdl(fp8_combine_kernel<float>, grid, block, 0, stream, "fp8_combine_kernel",
-                      static_cast<const float *>(s.y), pos, a.weights, a.tokens, a.top_k, a.hidden, a.out);
+                      static_cast<const float *>(s.y), pos, a.weights, gave_up, a.tokens, a.top_k, a.hidden, a.out);
 }
 
 }  // namespace lrb

@@ -171,7 +171,7 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
     """x [T, K] . w [N, K]^T on the values that the e4m3 tensors and their
     scales stand for -> [T, N] in BF16 or FP32 (out_dtype, or out's).  K must be
     a multiple of 16.  status: a device int32 [1] that becomes 1 if a bounded
-    wait inside a kernel gave up (the output is then not valid)."""
+    wait inside a kernel gave up (the output then holds NaN)."""
     if out is None:
         _require(out_dtype in (_BF16, _F32), "out_dtype must be BF16 or FP32")
     done = _bind().linear(x, x_scales, w, w_scales, out, out_dtype is _F32, status)

@@ -293,7 +293,9 @@ def experts_case(dev, tokens, count, top_k, hidden, inner, seed=0, routes="rando
 EXPERT_SHAPES = [(1, 8, 2, 256, 128), (1, 32, 8, 2048, 512), (2, 4, 4, 144, 128), (3, 16, 5, 400, 256),
                  (5, 64, 8, 2048, 512), (16, 32, 8, 1024, 256), (17, 16, 8, 2048, 512), (33, 4, 2, 16, 128),
                  (64, 1, 1, 128, 128), (65, 3, 3, 2064, 384), (130, 8, 2, 272, 256), (300, 6, 4, 1104, 128),
-                 (700, 5, 2, 512, 640), (1500, 12, 8, 512, 256), (12, 40, 12, 640, 128), (1, 40, 32, 256, 256)]
+                 (700, 5, 2, 512, 640), (1500, 12, 8, 512, 256), (12, 40, 12, 640, 128), (1, 40, 32, 256, 256),
+                 # two passes over the routes of one token; as many experts as there may be; the cluster plan
+                 (1, 40, 12, 640, 128), (20, 1024, 8, 128, 128), (260, 64, 8, 256, 256), (1100, 300, 2, 144, 128)]
 
 
 @pytest.mark.parametrize("tokens,count,top_k,hidden,inner", EXPERT_SHAPES)
@@ -332,6 +334,43 @@ def test_experts_nan_row_keeps_to_itself(dev, tokens):
     assert not torch.isfinite(got[tokens // 2]).any()
     keep = torch.arange(tokens, device=dev) != tokens // 2
     assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 60, 400])
+def test_experts_weights_of_dropped_routes_do_not_matter(dev, tokens):
+    """A dropped route's weight may hold anything, NaN too."""
+    c = list(experts_case(dev, tokens, 8, 4, 256, 128))
+    idx, weights = c[6].clone(), c[7].clone()
+    idx[:, 1], idx[:, 3] = -1, 8
+    weights[:, 1::2] = 0
+    want = fp8.experts(*c[:6], idx, weights)
+    weights[:, 1], weights[:, 3] = float("nan"), float("inf")
+    assert torch.equal(fp8.experts(*c[:6], idx, weights), want)
+
+
+def test_experts_and_linear_past_32_bit_rows(dev):
+    """Route rows and outputs of more than 2^32 bytes: the last rows against 64 bits."""
+    tokens, hidden, inner = 140_000, 2048, 128
+    c = experts_case(dev, 64, 8, 8, hidden, inner)
+    x, xs = (t.repeat(tokens // 64 + 1, 1)[:tokens].contiguous() for t in c[:2])
+    idx, weights = (t.repeat(tokens // 64 + 1, 1)[:tokens].contiguous() for t in c[6:])
+    got = fp8.experts(x, xs, *c[2:6], idx, weights)
+    want, bound = R.experts(*c)
+    last = slice(tokens - 96, tokens)
+    at = torch.arange(tokens, device=dev)[last] % 64
+    within(got[last], want[at], bound[at], "experts")
+    within(got[:64], want, bound, "experts, first")
+    del got, x, xs
+    rows, cols = 1_100_000, 128
+    x, xs, w, ws = linear_case(dev, 64, 2056, cols)
+    xl, xsl = (t.repeat(rows // 64 + 1, 1)[:rows].contiguous() for t in (x, xs))
+    got = fp8.linear(xl, xsl, w, ws)
+    want, bound = R.linear(x, xs, w, ws)
+    bound = bound + R.BF * (want.abs() + bound)
+    at = torch.arange(rows, device=dev)[rows - 96:] % 64
+    within(got[rows - 96:], want[at], bound[at], "linear")
+    del got, xl, xsl
+    torch.cuda.empty_cache()
 
 
 def test_experts_bank_past_32_bit_offsets(dev):

@@ -694,10 +694,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     next_buf();
                     if ((kb & 3) == 3 || kb + 1 == kbs) next_slot();
                 }
-                if (LIN && *abort) {
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc0[j] = acc1[j] = CUDART_NAN_F;
-                }
                 const int left = it.count - j0;  // rows of this warp, if below NJ
                 if (p1) {
                     if (active) {
@@ -820,10 +816,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (next.phase && (LIN || next.phase == it.phase)) {
                     take_scales(!LIN && next.phase == 1);
                     ready = true;
-                }
-                if (LIN && *abort) {
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) acc[i] = CUDART_NAN_F;
                 }
                 const int rows = it.count - 32 * q;  // of this warp, if below 32
                 const int64_t first = static_cast<int64_t>(it.row0) + 32 * q;
@@ -1005,6 +997,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 1) {
         sm100::tc_fence_after();
         sm100::tmem_dealloc(tmem, 512);
+    }
+    if (LIN && *abort) {
+        // NaN in place of this CTA's tiles (here, and not in the items' own
+        // path, where the test alone cost a twentieth of the time)
+        for (int item = SPLIT ? blockIdx.x / P.split : blockIdx.x; item < total; item += SPLIT ? total : gridDim.x) {
+            const Item it = decode(item);
+            for (int i = threadIdx.x; i < it.count * kBN; i += kThreads) {
+                const int n = it.n * kBN + i % kBN;
+                const int64_t o = static_cast<int64_t>(it.row0 + i / kBN) * n2 + n;
+                if (n >= n2) continue;
+                if (P.out_f32) static_cast<float *>(P.out)[o] = CUDART_NAN_F;
+                else static_cast<uint16_t *>(P.out)[o] = 0x7fff;
+            }
+        }
     }
     if (threadIdx.x == 0 && *abort) {
         if (P.status) atomicExch(P.status, 1);

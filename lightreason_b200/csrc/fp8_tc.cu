@@ -37,8 +37,8 @@
 //
 // Warps: 0 items and weight tiles, 1 MMA, 2 and 3 row tiles and scales (four
 // groups at a time, up to four such requests in flight), 4-11 epilogue; the
-// first four hand registers to the others (104 and 200 a thread of 168 at
-// launch, 64,512 a CTA either way).  Every wait is bounded; a timeout raises
+// first four hand registers to the others (72 and 216, the experts' 104 and
+// 200, a thread of 168 at launch: 64,512 a CTA either way).  Every wait is bounded; a timeout raises
 // *status, drains what is in flight and returns, and leaves NaN: in a linear's
 // tiles of that CTA, in all of an experts call's output.
 #include <algorithm>
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LIN ? 72 : 104));
         uint32_t stage = 0, phase = 0;
         auto next_stage = [&] {
             if (++stage == S::kStages) {
@@ -624,15 +624,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ----------------------------------------------------------- epilogue
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(LIN ? 216 : 200));
         const int q = warp & 3, h = warp >= 8;  // TMEM lanes 32q..; half of the columns
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * q) << 16);
         float *partial = reinterpret_cast<float *>(smem);  // SPLIT: the stages, when all of them are used
         uint32_t slot = 0, sphase = 0, buf = 0, bphase = 0, iphase = 0;
-        auto next_buf = [&] {
+        auto release_buf = [&] {
             sm100::tc_fence_before();
             __syncwarp();
             sm100::mbar_arrive_if(&tail->tempty[buf], lane == 0);
+        };
+        auto next_buf = [&] {
             if (++buf == S::kBufs) {
                 buf = 0;
                 bphase ^= 1;
@@ -691,6 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
+                    release_buf();
                     next_buf();
                     if ((kb & 3) == 3 || kb + 1 == kbs) next_slot();
                 }
@@ -800,12 +803,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             if (c < 7) load_cols<16>(base + 16 * (c + 1) + (c >= 3 ? skip : 0), t[(c + 1) & 1]);
+                            else release_buf();  // all of it is in registers
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 acc[16 * c + i] = fmaf(t[c & 1][i], c < 4 ? g0 : g1, acc[16 * c + i]);
                             if (c < 7) wait_cols(t[(c + 1) & 1]);
                         }
                     }
+                    if (!active) release_buf();
                     next_buf();
                     // behind the buffer's release: the products go on meanwhile
                     if ((kb & 3) == 3 && kb + 1 < kbs) take_scales(p1);

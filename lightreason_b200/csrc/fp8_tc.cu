@@ -1097,7 +1097,7 @@ __global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restric
 }
 
 // out[t] = sum over the token's routes, in slot order, of weight * row, in
-// FP32.  A thread per 8 columns of a token, eight rows in flight.  The first
+// FP32.  A thread per 16 bytes of a row, eight rows in flight.  The first
 // routes' places and weights are there before the wait: the plan kernel and
 // whatever wrote the weights were complete when the tile kernel let this one
 // start.
@@ -1105,11 +1105,11 @@ template <class Y>
 __global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *__restrict__ y, const int32_t *route_pos,
                                                           const uint16_t *weights, const int32_t *gave_up, int tokens,
                                                           int top_k, int hidden, uint16_t *__restrict__ out) {
-    constexpr int kU = 8, kParts = sizeof(Y) / 2;  // 16-byte parts of 8 columns
-    const int units = hidden / 8;
+    constexpr int kU = 8, kCols = 16 / sizeof(Y);
+    const int units = hidden / kCols;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
     const int64_t t = i / units;
-    const int c = static_cast<int>(i % units) * 8;
+    const int c = static_cast<int>(i % units) * kCols;
     int pos[kU];
     float w[kU];
     auto routes = [&](int k0) {
@@ -1126,39 +1126,37 @@ __global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *__restrict__ 
     grid_dependency_trigger();
     if (t >= tokens) return;
     const float zero = __ldcg(gave_up) ? CUDART_NAN_F : 0.f;
-    float acc[8];
+    float acc[kCols];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = zero;
+    for (int j = 0; j < kCols; ++j) acc[j] = zero;
     for (int k0 = 0; k0 < top_k; k0 += kU) {
         if (k0) routes(k0);
-        uint4 v[kU][kParts];
+        uint4 v[kU];
 #pragma unroll
         for (int k = 0; k < kU; ++k)
-#pragma unroll
-            for (int h = 0; h < kParts; ++h)
-                v[k][h] = pos[k] >= 0 ? ld_stream(y + static_cast<int64_t>(pos[k]) * hidden + c + 4 * h)
-                                      : make_uint4(0, 0, 0, 0);
+            v[k] = pos[k] >= 0 ? ld_stream(y + static_cast<int64_t>(pos[k]) * hidden + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < kU; ++k) {
             if (pos[k] < 0) continue;  // a weight of a dropped route may be anything
-            if constexpr (kParts == 2) {
-                const uint32_t u[8] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w,
-                                       v[k][1].x, v[k][1].y, v[k][1].z, v[k][1].w};
+            const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[j] = fmaf(__uint_as_float(u[j]), w[k], acc[j]);
-            } else {
-                const uint32_t u[4] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (kCols == 4) {
+                    acc[j] = fmaf(__uint_as_float(u[j]), w[k], acc[j]);
+                } else {
                     acc[2 * j] = fmaf(bf16_lo(u[j]), w[k], acc[2 * j]);
                     acc[2 * j + 1] = fmaf(bf16_hi(u[j]), w[k], acc[2 * j + 1]);
                 }
             }
         }
     }
-    *reinterpret_cast<uint4 *>(out + t * hidden + c) =
-        make_uint4(fp8::pack_bf16(acc[0], acc[1]), fp8::pack_bf16(acc[2], acc[3]), fp8::pack_bf16(acc[4], acc[5]),
-                   fp8::pack_bf16(acc[6], acc[7]));
+    if constexpr (kCols == 4)
+        *reinterpret_cast<uint2 *>(out + t * hidden + c) =
+            make_uint2(fp8::pack_bf16(acc[0], acc[1]), fp8::pack_bf16(acc[2], acc[3]));
+    else
+        *reinterpret_cast<uint4 *>(out + t * hidden + c) =
+            make_uint4(fp8::pack_bf16(acc[0], acc[1]), fp8::pack_bf16(acc[2], acc[3]),
+                       fp8::pack_bf16(acc[4], acc[5]), fp8::pack_bf16(acc[6], acc[7]));
 }
 
 template <bool LIN, int BN>
@@ -1368,7 +1366,7 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
         default: rc = launch_tile<false, 0>(m, P, items, stream); break;
     }
     if (rc) return rc;
-    const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / 8) + 127) / 128;
+    const int64_t ctas = (static_cast<int64_t>(a.tokens) * (a.hidden / (P.y_f32 ? 4 : 8)) + 127) / 128;
     const dim3 grid(static_cast<unsigned>(ctas)), block(128);
     const int32_t *pos = s.route_pos, *gave_up = P.gave_up;
     if (!P.y_f32)

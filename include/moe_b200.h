@@ -525,14 +525,11 @@ int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, ui
 
 /* out[T, rows] (BF16, or FP32 with out_f32 = 1) = x . w^T on the values that x
  * [T, cols] and w [rows, cols] stand for, products summed in FP32.  cols must
- * be a multiple of 16; x, w and out are 16-byte aligned.  The workspace query
- * may return 0: workspace may then be NULL.  status (device int32, or NULL) is
- * set to 1 if a bounded wait inside a kernel gave up; out then holds NaN (a
- * linear: in the tiles concerned). */
-size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols);
+ * be a multiple of 16; x, w and out are 16-byte aligned; no size is above 2^30.
+ * status (device int32, or NULL) is set to 1 if a bounded wait inside a kernel
+ * gave up; out then holds NaN (a linear: in the tiles concerned). */
 int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
-                   int rows, int cols, void *out, int out_f32, void *workspace, size_t workspace_bytes,
-                   int32_t *status, void *stream);
+                   int rows, int cols, void *out, int out_f32, int32_t *status, void *stream);
 
 /* The routed experts (the Qwen3_5MoeExperts.forward contract of
  * moe_layer_forward with route_in) on e4m3 banks gate_up [E, 2I, H] and down

@@ -57,24 +57,18 @@ Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
 
 using namespace lrb;
 
-extern "C" size_t moe_linear_fp8_workspace_bytes(int tokens, int rows, int cols) {
-    (void)tokens, (void)rows, (void)cols;
-    return 0;
-}
-
 extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales,
-                              int tokens, int rows, int cols, void *out, int out_f32, void *workspace,
-                              size_t workspace_bytes, int32_t *status, void *stream) {
-    LRB_REQUIRE(tokens >= 0 && rows >= 1, "moe_linear_fp8: bad tokens %d / rows %d", tokens, rows);
-    LRB_REQUIRE(cols >= 16 && cols % 16 == 0, "moe_linear_fp8: cols %d must be a positive multiple of 16", cols);
+                              int tokens, int rows, int cols, void *out, int out_f32, int32_t *status,
+                              void *stream) {
+    LRB_REQUIRE(tokens >= 0 && tokens <= (1 << 30) && rows >= 1 && rows <= (1 << 30),
+                "moe_linear_fp8: bad tokens %d / rows %d", tokens, rows);
+    LRB_REQUIRE(cols >= 16 && cols % 16 == 0 && cols <= (1 << 30),
+                "moe_linear_fp8: cols %d must be a positive multiple of 16 up to 2^30", cols);
     LRB_REQUIRE(out_f32 == 0 || out_f32 == 1, "moe_linear_fp8: out_f32 must be 0 or 1");
     if (tokens == 0) return MOE_OK;
     LRB_REQUIRE(x && x_scales && w && w_scales && out, "moe_linear_fp8: null tensor");
     LRB_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scales, 4) && aligned(w_scales, 4) && aligned(out, 16),
                 "moe_linear_fp8: x, w and out must be 16-byte aligned");
-    const size_t need = moe_linear_fp8_workspace_bytes(tokens, rows, cols);
-    LRB_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need),
-                "moe_linear_fp8: workspace of %zu bytes (256-byte aligned) required", need);
     if (int rc = require_sm100()) return rc;
     const LinearFp8 a{x, x_scales, w, w_scales, tokens, rows, cols, out, out_f32};
     if (plan_linear_fp8(tokens, rows, cols).gemv) return launch_linear_fp8_gemv(a, as_stream(stream));

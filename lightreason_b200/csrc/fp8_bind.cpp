@@ -20,7 +20,6 @@ namespace {
 decltype(&moe_rmsnorm_fp8) g_rows;
 decltype(&moe_quantize_fp8_blocks) g_blocks;
 decltype(&moe_linear_fp8) g_linear;
-decltype(&moe_linear_fp8_workspace_bytes) g_linear_workspace;
 decltype(&moe_experts_fp8) g_experts;
 decltype(&moe_experts_fp8_workspace_bytes) g_experts_workspace;
 
@@ -57,17 +56,28 @@ T *ptr(const at::Tensor *t) {
     return t ? static_cast<T *>(t->data_ptr()) : nullptr;
 }
 
-// Runs f(stream) on device `index` without the interpreter's lock.
+// Runs f(stream) on device `index` without the interpreter's lock.  f may throw
+// (a tensor without memory of its own has no data_ptr): device and lock are
+// back before the exception is turned into Python's.
 template <class F>
 int on(int index, F &&f) {
-    const auto before = c10::cuda::current_device();
-    if (before != index) c10::cuda::set_device(index);
-    void *stream = c10::cuda::getCurrentCUDAStream(index).stream();
-    PyThreadState *state = PyEval_SaveThread();
-    const int rc = f(stream);
-    PyEval_RestoreThread(state);
-    if (before != index) c10::cuda::set_device(before);
-    return rc;
+    struct Device {
+        const c10::DeviceIndex before;
+        const bool changed;
+        explicit Device(int i) : before(c10::cuda::current_device()), changed(before != i) {
+            if (changed) c10::cuda::set_device(static_cast<c10::DeviceIndex>(i));
+        }
+        ~Device() {
+            if (changed) c10::cuda::MaybeSetDevice(before);
+        }
+    } device(index);
+    struct Unlocked {
+        PyThreadState *state = PyEval_SaveThread();
+        ~Unlocked() { PyEval_RestoreThread(state); }
+    };
+    void *stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream();
+    Unlocked unlocked;
+    return f(stream);
 }
 
 PyObject *none() { Py_RETURN_NONE; }
@@ -159,14 +169,10 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
                !fits(out, out->scalar_type(), {tokens, nr}, index)) {
         return none();
     }
-    const size_t bytes = g_linear_workspace(static_cast<int>(tokens), static_cast<int>(nr), static_cast<int>(cols));
-    at::Tensor ws_t;
-    if (bytes) ws_t = make({static_cast<int64_t>(bytes)}, at::kByte, *x);
     const int rc = on(index, [&](void *stream) {
         return g_linear(ptr<uint8_t>(x), ptr<float>(xs), ptr<uint8_t>(w), ptr<float>(ws), static_cast<int>(tokens),
                         static_cast<int>(nr), static_cast<int>(cols), ptr<void>(out),
-                        out->scalar_type() == at::kFloat, bytes ? ws_t.data_ptr() : nullptr, bytes,
-                        ptr<int32_t>(status), stream);
+                        out->scalar_type() == at::kFloat, ptr<int32_t>(status), stream);
     });
     if (rc) return PyLong_FromLong(rc);
     return own(a[4], made);
@@ -219,16 +225,15 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(rows, blocks, linear, linear_workspace, experts, experts_workspace): addresses in the loaded library
+// bind(rows, blocks, linear, experts, experts_workspace): addresses in the loaded library
 PyObject *bind(PyObject *, PyObject *args) {
-    unsigned long long p[6];
-    if (!PyArg_ParseTuple(args, "KKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5])) return nullptr;
+    unsigned long long p[5];
+    if (!PyArg_ParseTuple(args, "KKKKK", &p[0], &p[1], &p[2], &p[3], &p[4])) return nullptr;
     g_rows = reinterpret_cast<decltype(g_rows)>(p[0]);
     g_blocks = reinterpret_cast<decltype(g_blocks)>(p[1]);
     g_linear = reinterpret_cast<decltype(g_linear)>(p[2]);
-    g_linear_workspace = reinterpret_cast<decltype(g_linear_workspace)>(p[3]);
-    g_experts = reinterpret_cast<decltype(g_experts)>(p[4]);
-    g_experts_workspace = reinterpret_cast<decltype(g_experts_workspace)>(p[5]);
+    g_experts = reinterpret_cast<decltype(g_experts)>(p[3]);
+    g_experts_workspace = reinterpret_cast<decltype(g_experts_workspace)>(p[4]);
     Py_RETURN_NONE;
 }
 

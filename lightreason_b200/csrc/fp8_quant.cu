@@ -6,8 +6,6 @@
 // (transformers modeling_qwen3_5_moe.py): r = bf16(x + residual),
 // y = r * rsqrt(mean(r^2) + eps) * (offset + weight), the sum of squares in
 // FP32; q and the scales are those of y before it is rounded to BF16.
-#include <algorithm>
-
 #include "fp8.cuh"
 #include "kernels.cuh"
 
@@ -303,8 +301,8 @@ extern "C" int moe_rmsnorm_fp8(const uint16_t *x, int64_t x_stride, const uint16
                                int64_t residual_stride, const uint16_t *weight, float weight_offset, float eps,
                                int tokens, int hidden, uint8_t *q, float *scales, uint16_t *normed,
                                uint16_t *residual_out, void *stream) {
-    LRB_REQUIRE(tokens >= 0 && hidden >= 1 && hidden <= (1 << 20), "moe_rmsnorm_fp8: bad tokens %d / hidden %d",
-                tokens, hidden);
+    LRB_REQUIRE(tokens >= 0 && tokens <= (1 << 30) && hidden >= 1 && hidden <= (1 << 20),
+                "moe_rmsnorm_fp8: bad tokens %d / hidden %d", tokens, hidden);
     LRB_REQUIRE(weight || (!residual && !normed && !residual_out),
                 "moe_rmsnorm_fp8: without a norm weight there is no residual, normed or residual_out");
     LRB_REQUIRE(!residual_out || residual, "moe_rmsnorm_fp8: residual_out without residual");
@@ -321,8 +319,8 @@ extern "C" int moe_rmsnorm_fp8(const uint16_t *x, int64_t x_stride, const uint16
 
 extern "C" int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, uint8_t *q, float *scales,
                                        void *stream) {
-    LRB_REQUIRE(banks >= 0 && rows >= 1 && cols >= 1, "moe_quantize_fp8_blocks: bad shape [%d, %d, %d]", banks, rows,
-                cols);
+    LRB_REQUIRE(banks >= 0 && rows >= 1 && rows <= (1 << 30) && cols >= 1 && cols <= (1 << 30),
+                "moe_quantize_fp8_blocks: bad shape [%d, %d, %d]", banks, rows, cols);
     const int64_t blocks = static_cast<int64_t>(banks) * lrb::fp8::groups(rows) * lrb::fp8::groups(cols);
     LRB_REQUIRE(blocks < (1ll << 31), "moe_quantize_fp8_blocks: too many blocks");
     LRB_REQUIRE(banks == 0 || (w && q && scales), "moe_quantize_fp8_blocks: null tensor");

@@ -1200,7 +1200,7 @@ int row_maps(CUtensorMap *m, CUtensorMap *m16, const void *base, int rows, int c
     return make_map_u8(m16, base, 2, dims, str, 16);
 }
 
-// One CTA up to 2048 routes; eight (6 us at 32,768 routes) above.
+// One CTA up to 2048 routes; eight (9 us at 32,768 routes) above.
 int launch_plan(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int routes, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(routes <= 2048 ? 1 : 8);

@@ -52,8 +52,8 @@ def _bind():
     spec.loader.exec_module(module)
     so = native.lib()
     module.bind(*(ctypes.cast(getattr(so, name), ctypes.c_void_p).value for name in (
-        "moe_rmsnorm_fp8", "moe_quantize_fp8_blocks", "moe_linear_fp8", "moe_linear_fp8_workspace_bytes",
-        "moe_experts_fp8", "moe_experts_fp8_workspace_bytes")))
+        "moe_rmsnorm_fp8", "moe_quantize_fp8_blocks", "moe_linear_fp8", "moe_experts_fp8",
+        "moe_experts_fp8_workspace_bytes")))
     return module
 
 

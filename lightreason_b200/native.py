@@ -96,8 +96,7 @@ _SIGNATURES = {
     "moe_rmsnorm_fp8": ([_p, ctypes.c_int64, _p, ctypes.c_int64, _p, ctypes.c_float, ctypes.c_float, _i, _i, _p, _p,
                          _p, _p, _p], _i),
     "moe_quantize_fp8_blocks": ([_p, _i, _i, _i, _p, _p, _p], _i),
-    "moe_linear_fp8_workspace_bytes": ([_i, _i, _i], _sz),
-    "moe_linear_fp8": ([_p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _sz, _p, _p], _i),
+    "moe_linear_fp8": ([_p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _p], _i),
     "moe_experts_fp8_workspace_bytes": ([_i, _i, _i, _i, _i], _sz),
     "moe_experts_fp8": ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _sz, _p, _p], _i),
     "moe_grouped_paired": ([_i, _i, _i], _i),

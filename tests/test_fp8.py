@@ -32,6 +32,8 @@ def test_rows_refusals(so):
 
     refused(so, call(hidden=0), "bad tokens")
     refused(so, call(tokens=-1), "bad tokens")
+    refused(so, call(tokens=2**31 - 1), "bad tokens")
+    refused(so, call(hidden=(1 << 20) + 1), "bad tokens")
     refused(so, call(xs=255), "row strides")
     refused(so, call(res=ok, rs=8), "row strides")
     refused(so, call(r=ok), "residual_out without residual")
@@ -47,6 +49,8 @@ def test_blocks_refusals(so):
     ok = P(1 << 20)
     refused(so, so.moe_quantize_fp8_blocks(ok, 1, 0, 4, ok, ok, None), "bad shape")
     refused(so, so.moe_quantize_fp8_blocks(ok, -1, 4, 4, ok, ok, None), "bad shape")
+    refused(so, so.moe_quantize_fp8_blocks(ok, 1, 2**31 - 1, 4, ok, ok, None), "bad shape")
+    refused(so, so.moe_quantize_fp8_blocks(ok, 1, 4, 2**31 - 1, ok, ok, None), "bad shape")
     refused(so, so.moe_quantize_fp8_blocks(None, 1, 4, 4, ok, ok, None), "null tensor")
     refused(so, so.moe_quantize_fp8_blocks(ok, 1 << 30, 1024, 1024, ok, ok, None), "too many blocks")
     assert so.moe_quantize_fp8_blocks(None, 0, 4, 4, None, None, None) == native.MOE_OK
@@ -54,10 +58,9 @@ def test_blocks_refusals(so):
 
 def test_linear_refusals(so):
     ok, bad = P(1 << 20), P((1 << 20) + 8)
-    ws = so.moe_linear_fp8_workspace_bytes
 
-    def call(x=ok, w=ok, tokens=3, rows=64, cols=256, out=ok, f32=0, work=ok, nbytes=1 << 30):
-        return so.moe_linear_fp8(x, ok, w, ok, tokens, rows, cols, out, f32, work, nbytes, None, None)
+    def call(x=ok, w=ok, tokens=3, rows=64, cols=256, out=ok, f32=0):
+        return so.moe_linear_fp8(x, ok, w, ok, tokens, rows, cols, out, f32, None, None)
 
     refused(so, call(cols=24), "multiple of 16")
     refused(so, call(cols=0), "multiple of 16")
@@ -67,9 +70,10 @@ def test_linear_refusals(so):
     refused(so, call(x=None), "null tensor")
     for k in ("x", "w", "out"):
         refused(so, call(**{k: bad}), "16-byte aligned")
-    for shape in ((64, 1024, 2048), (8, 512, 4096)):
-        if ws(*shape):
-            refused(so, call(tokens=shape[0], rows=shape[1], cols=shape[2], nbytes=ws(*shape) - 1), "workspace")
+    # past 2^30, where a size rounded up to a tile no longer fits 32 bits
+    refused(so, call(tokens=2**31 - 1), "bad tokens")
+    refused(so, call(rows=2**31 - 1), "bad tokens")
+    refused(so, call(cols=2**31 - 16), "multiple of 16")
     assert call(tokens=0, x=None, out=None) == native.MOE_OK
 
 

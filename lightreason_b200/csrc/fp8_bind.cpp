@@ -53,11 +53,14 @@ at::Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &li
 }
 template <class T>
 T *ptr(const at::Tensor *t) {
-    return t ? static_cast<T *>(t->data_ptr()) : nullptr;
+    if (!t) return nullptr;
+    void *p = t->data_ptr();
+    TORCH_CHECK(p || t->numel() == 0, "the FP8 operators need tensors with storage");
+    return static_cast<T *>(p);
 }
 
 // Runs f(stream) on device `index` without the interpreter's lock.  f may throw
-// (a tensor without memory of its own has no data_ptr): device and lock are
+// (a fake tensor has no storage): device and lock are
 // back before the exception is turned into Python's.
 template <class F>
 int on(int index, F &&f) {

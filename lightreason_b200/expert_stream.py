@@ -136,14 +136,26 @@ class ExpertPool:
         slots = min(share // layer.row_bytes, layer.module.num_experts, 1024)
         return slots if slots >= routed else 0
 
-    def _fp8_banks(self, layer: "_Layer", owner=None, shared=None) -> fp8.ExpertBanks:
-        """The FP8 banks of one patched module (with its shared expert, for a
-        whole-block patch), made on first use."""
+    def _fp8_banks(self, layer: "_Layer", owner=None, shared=(), extra=()) -> fp8.ExpertBanks:
+        """The FP8 banks of one patched module (with its shared expert and its
+        router, for a whole-block patch), made on first use, and again where the
+        module's weights have changed since."""
         key = (id(owner if owner is not None else layer.module), layer.residency, 0)
         banks = self._layers.get(key)
-        if banks is None:
-            banks = self._layers[key] = fp8.ExpertBanks(layer.gate_up, layer.down, self.device, shared=shared)
-            self.stats.resident_bytes += banks.nbytes()
+        if banks is not None:
+            if banks.holds(layer.gate_up, layer.down, *shared, *extra):
+                return banks
+            if (banks.experts, banks.hidden, banks.inner) == (
+                    layer.module.num_experts, layer.module.hidden_dim, layer.module.intermediate_dim):
+                banks.load(layer.gate_up, layer.down, shared=shared, extra=extra)
+                return banks
+            # another module's, gone, under the same id: its captured calls go too
+            self.stats.resident_bytes -= banks.nbytes()
+            graphs = getattr(self, "replay_graphs", {})
+            for old in [k for k in graphs if k[:2] == key[:2]]:
+                del graphs[old]
+        banks = self._layers[key] = fp8.ExpertBanks(layer.gate_up, layer.down, self.device, shared=shared, extra=extra)
+        self.stats.resident_bytes += banks.nbytes()
         return banks
 
     def _native_layer(self, layer: "_Layer", top_k: int, owner=None, extra=None, cache: int = 0) -> native.Layer:
@@ -220,7 +232,7 @@ class _Layer:
         if self.residency in HOST_RESIDENCIES and self.gate_up.device.type != "cpu":
             raise ValueError(f"{name}: host residency needs CPU expert parameters")
         if self.residency == "b200-fp8":
-            fp8.check_widths(module.hidden_dim, module.intermediate_dim)
+            fp8.check_widths(module.hidden_dim, module.intermediate_dim, module.num_experts)
         self.row_bytes = (self.gate_up.numel() + self.down.numel()) * 2 // module.num_experts
 
     def _check_sources(self):

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import weakref
 from functools import lru_cache
 
 import torch
@@ -233,37 +234,61 @@ class ExpertBanks:
     gate_up [E, 2I, H] and down [E, H, I] may live on the CPU or on the device;
     they are brought over and quantised a few experts at a time, so the BF16
     bank is never whole on the device because of this.  shared: a further
-    expert (gate [I, H], up [I, H], down [H, I]), kept as expert id E."""
+    expert (gate [I, H], up [I, H], down [H, I]), kept as expert id E.  extra:
+    tensors that go with the layer, copied to the device as they are."""
 
     CHUNK = 16  # experts quantised at once
 
-    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, device, *, shared=None):
+    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, device, *, shared=(), extra=()):
         count, rows, hidden = gate_up.shape
         inner = rows // 2
         _require(tuple(down.shape) == (count, hidden, inner), "gate_up must be [E, 2I, H] and down [E, H, I]")
-        check_widths(hidden, inner)
-        total = count + (shared is not None)
+        total = count + bool(shared)
+        check_widths(hidden, inner, total)
         self.experts, self.hidden, self.inner, self.device = count, hidden, inner, torch.device(device)
         make = lambda n, k: (torch.empty((total, n, k), dtype=E4M3, device=self.device),  # noqa: E731
                              torch.empty((total, _groups(n), _groups(k)), dtype=_F32, device=self.device))
         self.gate_up, self.gate_up_scales = make(rows, hidden)
         self.down, self.down_scales = make(hidden, inner)
+        self.extra = tuple(torch.empty_like(t, device=self.device, memory_format=torch.contiguous_format)
+                           for t in extra)
+        self.load(gate_up, down, shared=shared, extra=extra)
+
+    def load(self, gate_up: torch.Tensor, down: torch.Tensor, *, shared=(), extra=()) -> None:
+        """Brings these weights into the banks' memory, where captured graphs
+        that read it find them too."""
+        _require(not (self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()),
+                 "FP8 banks cannot be made during a graph capture: call the layer once before it")
+        count, hidden, inner = self.experts, self.hidden, self.inner
+        _require(tuple(gate_up.shape) == (count, 2 * inner, hidden) and tuple(down.shape) == (count, hidden, inner)
+                 and self.gate_up.shape[0] == count + bool(shared) and len(extra) == len(self.extra),
+                 "the weights do not have the banks' shapes")
         parts = [(a, min(a + self.CHUNK, count)) for a in range(0, count, self.CHUNK)]
         with torch.no_grad():
             for source, q, scales in ((gate_up, self.gate_up, self.gate_up_scales),
                                       (down, self.down, self.down_scales)):
                 for a, b in parts:
                     quantize_blocks(source[a:b].detach().to(self.device).contiguous(), out=(q[a:b], scales[a:b]))
-            if shared is not None:
+            if shared:
                 gate, up, last = (t.detach().to(self.device) for t in shared)
                 _require(tuple(gate.shape) == tuple(up.shape) == (inner, hidden)
                          and tuple(last.shape) == (hidden, inner), "the shared expert must have the experts' widths")
                 quantize_blocks(torch.cat([gate, up])[None], out=(self.gate_up[count:], self.gate_up_scales[count:]))
                 quantize_blocks(last[None].contiguous(), out=(self.down[count:], self.down_scales[count:]))
+            for held, t in zip(self.extra, extra):
+                held.copy_(t)
+        self._sources = [(weakref.ref(t), _version(t)) for t in (gate_up, down, *shared, *extra)]
+
+    def holds(self, *sources: torch.Tensor) -> bool:
+        """Whether these are the tensors last loaded (in load's order), unchanged
+        since.  Changes made behind autograd's version counter (through .data, or
+        to tensors made in inference mode) are not seen."""
+        return len(sources) == len(self._sources) and all(
+            ref() is t and version == _version(t) for (ref, version), t in zip(self._sources, sources))
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size()
-                   for t in (self.gate_up, self.gate_up_scales, self.down, self.down_scales))
+                   for t in (self.gate_up, self.gate_up_scales, self.down, self.down_scales, *self.extra))
 
     def release(self) -> None:
         """Part of the pool's layer interface; the banks go with their tensors."""
@@ -274,7 +299,14 @@ class ExpertBanks:
         return experts(q, scales, self.gate_up, self.gate_up_scales, self.down, self.down_scales, idx, weights)
 
 
-def check_widths(hidden: int, inner: int) -> None:
-    """The widths the expert kernels take."""
+def _version(t: torch.Tensor) -> int:
+    return -1 if t.is_inference() else t._version
+
+
+def check_widths(hidden: int, inner: int, experts: int = 1) -> None:
+    """The widths and numbers of experts that the expert kernels take."""
     _require(hidden % 16 == 0 and inner % 128 == 0,
              f"FP8 experts need hidden a multiple of 16 and inner of 128, got {hidden} and {inner}")
+    _require(16 <= hidden <= 65536 and 128 <= inner <= 16384 and 1 <= experts <= 1024,
+             f"FP8 experts take hidden up to 65536, inner up to 16384 and 1024 experts (a shared one counts), got "
+             f"{hidden}, {inner} and {experts}")

@@ -20,7 +20,7 @@ from contextlib import contextmanager
 
 import torch
 
-from lightreason_b200 import native
+from lightreason_b200 import fp8, native
 from lightreason_b200.expert_stream import MODES, _Layer
 
 
@@ -35,10 +35,10 @@ class _Block:
                 block.experts.num_experts, block.experts.hidden_dim):
             raise ValueError(f"{name}: expected a BF16 router [experts, hidden]")
         self.top_k = gate.top_k
-        self._route = None   # router and shared gate weights on the device (FP8 blocks)
-        if self.experts.residency == "b200-fp8" and \
-                block.shared_expert.gate_proj.weight.shape[0] != block.experts.intermediate_dim:
-            raise ValueError(f"{name}: FP8 blocks need a shared expert of the experts' width")
+        if self.experts.residency == "b200-fp8":
+            if block.shared_expert.gate_proj.weight.shape[0] != block.experts.intermediate_dim:
+                raise ValueError(f"{name}: FP8 blocks need a shared expert of the experts' width")
+            fp8.check_widths(block.experts.hidden_dim, block.experts.intermediate_dim, block.experts.num_experts + 1)
 
     def _extra(self):
         dev = self.pool.device
@@ -71,14 +71,13 @@ class _Block:
 
     def _fp8(self, x):
         """The block on FP8 banks: the shared expert is expert E, its weight the sigmoid gate."""
-        b, dev = self.block, self.pool.device
+        b = self.block
         shared = b.shared_expert
-        banks = self.pool._fp8_banks(self.experts, owner=b, shared=(
-            shared.gate_proj.weight, shared.up_proj.weight, shared.down_proj.weight))
-        if self._route is None:
-            self._route = (b.gate.weight.detach().to(dev).contiguous(),
-                           b.shared_expert_gate.weight.reshape(-1).detach().to(dev).contiguous())
-        idx, _, scores, _, sig = native.router_topk(x, self._route[0], None, self._route[1], self.top_k)
+        banks = self.pool._fp8_banks(
+            self.experts, owner=b, shared=(shared.gate_proj.weight, shared.up_proj.weight, shared.down_proj.weight),
+            extra=(b.gate.weight, b.shared_expert_gate.weight))
+        router, gate = banks.extra
+        idx, _, scores, _, sig = native.router_topk(x, router, None, gate.view(-1), self.top_k)
         idx = torch.nn.functional.pad(idx, (0, 1), value=banks.experts)
         return banks(x, idx, torch.cat([scores, sig[:, None]], 1))
 

@@ -70,6 +70,8 @@ def replay_experts(pool, *, max_tokens: int = 16):
         if layer.pool is not pool or not 0 < tokens <= max_tokens or torch.cuda.is_current_stream_capturing():
             return original(layer, hidden, indices, weights)
         key = (id(layer.module), layer.residency, tokens, indices.shape[1])
+        if layer.residency == "b200-fp8":
+            pool._fp8_banks(layer)  # weights changed since are brought to the banks that the graphs read
         entry = pool.replay_graphs.get(key)
         if entry is None:
             entry = pool.replay_graphs[key] = _Replay(layer, original, hidden, indices, weights,

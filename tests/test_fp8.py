@@ -132,3 +132,45 @@ def test_patch_refuses_widths_without_kernels():
         expert_stream._Layer("e", experts, pool, "b200-fp8")
     with pytest.raises(ValueError, match="inner of 128"):
         fp8.check_widths(256, 192)
+
+
+def test_widths_and_numbers_of_experts():
+    fp8.check_widths(16, 128)
+    fp8.check_widths(65536, 16384, 1024)
+    for bad in ((65552, 128, 4), (256, 16512, 4), (256, 128, 1025), (0, 128, 4)):
+        with pytest.raises(ValueError, match="1024 experts"):
+            fp8.check_widths(*bad)
+
+
+def test_banks_follow_their_sources(monkeypatch):
+    """ExpertBanks.holds: the tensors last loaded, unchanged; load writes into
+    the memory that the banks already have."""
+    quantised = []
+
+    def fake(w, out):
+        quantised.append(tuple(w.shape))
+        out[0].copy_(w.to(E4M3))
+        out[1].fill_(float(w.flatten()[0]))
+
+    monkeypatch.setattr(fp8, "quantize_blocks", fake)
+    gu, dn = (torch.full(s, 1.0, dtype=torch.bfloat16) for s in ((20, 256, 64), (20, 64, 128)))
+    shared = [torch.full(s, 2.0, dtype=torch.bfloat16) for s in ((128, 64), (128, 64), (64, 128))]
+    router = torch.full((20, 64), 3.0, dtype=torch.bfloat16)
+    banks = fp8.ExpertBanks(gu, dn, "cpu", shared=shared, extra=(router,))
+    assert quantised == [(16, 256, 64), (4, 256, 64), (16, 64, 128), (4, 64, 128), (1, 256, 64), (1, 64, 128)]
+    assert banks.gate_up.shape == (21, 256, 64) and banks.down_scales.shape == (21, 1, 1)
+    sources = [gu, dn, *shared, router]
+    assert banks.holds(*sources) and not banks.holds(gu, dn) and not banks.holds(gu.clone(), dn, *shared, router)
+    places = [t.data_ptr() for t in (banks.gate_up, banks.down_scales, banks.extra[0])]
+    for t in sources:
+        t.mul_(2)
+        assert not banks.holds(*sources)
+        banks.load(gu, dn, shared=shared, extra=(router,))
+        assert banks.holds(*sources)
+    assert places == [t.data_ptr() for t in (banks.gate_up, banks.down_scales, banks.extra[0])]
+    assert banks.extra[0].eq(6).all() and banks.down_scales[:20].eq(2).all() and banks.down_scales[20:].eq(4).all()
+    with pytest.raises(ValueError, match="banks' shapes"):
+        banks.load(gu, dn)
+    with pytest.raises(ValueError, match="1024 experts"):
+        fp8.ExpertBanks(torch.zeros(1024, 256, 16, dtype=torch.bfloat16), torch.zeros(1024, 16, 128,
+                        dtype=torch.bfloat16), "cpu", shared=[torch.zeros(1)] * 3)

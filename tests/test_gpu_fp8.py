@@ -470,6 +470,99 @@ def test_back_to_back_calls_with_new_weights(dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_python_names_the_argument_it_refuses(dev):
+    """What the C++ module does not take is named by the Python behind it."""
+    c = experts_case(dev, 3, 4, 2, 256, 128)
+    x, xs, gu, gus, dn, dns, idx, wt = c
+    b = torch.zeros(3, 256, dtype=torch.bfloat16, device=dev)
+    w = torch.zeros(256, dtype=torch.bfloat16, device=dev)
+    grad = b.clone().requires_grad_()
+    cases = [
+        (lambda: fp8.quantize_rows(b.float()), ValueError, "x must be a CUDA BF16"),
+        (lambda: fp8.quantize_rows(b[:, ::2]), ValueError, "dense rows"),
+        (lambda: fp8.quantize_rows(b[:1].expand(3, 256)), ValueError, "dense rows"),
+        (lambda: fp8.quantize_rows(b, out=(x, xs[:2])), ValueError, r"out\[1\]"),
+        (lambda: fp8.quantize_rows(b, out=(b, xs)), ValueError, r"out\[0\]"),
+        (lambda: fp8.quantize_rows(grad), RuntimeError, "no gradient"),
+        (lambda: fp8.rmsnorm_quantize(b, w[:128]), ValueError, "weight"),
+        (lambda: fp8.rmsnorm_quantize(b, w, b[:2]), ValueError, "residual"),
+        (lambda: fp8.rmsnorm_quantize(b, w.cpu()), ValueError, "weight"),
+        (lambda: fp8.rmsnorm_quantize(b, w, out=(x, xs, None, b.clone())), ValueError, "without a residual"),
+        (lambda: fp8.rmsnorm_quantize(b, w, eps=2.0), ValueError, "eps"),
+        (lambda: fp8.rmsnorm_quantize(grad, w), RuntimeError, "no gradient"),
+        (lambda: fp8.quantize_blocks(b.t()), ValueError, "w must be"),
+        (lambda: fp8.quantize_blocks(grad), RuntimeError, "no gradient"),
+        (lambda: fp8.quantize_blocks(b, out=(x, xs)), ValueError, r"out\[1\]"),
+        (lambda: fp8.linear(x, xs[:, :1], gu[0], gus[0]), ValueError, "x_scales"),
+        (lambda: fp8.linear(x, xs, gu[0], gus[0][:1]), ValueError, "w_scales"),
+        (lambda: fp8.linear(x, xs, gu[0], gus[0], out_dtype=torch.float16), ValueError, "out_dtype"),
+        (lambda: fp8.linear(x, xs, gu[0], gus[0], out=b[:2]), ValueError, "out"),
+        (lambda: fp8.linear(x, xs, gu[0], gus[0], status=idx), ValueError, "status"),
+        (lambda: fp8.linear(x, xs.clone().requires_grad_(), gu[0], gus[0]), RuntimeError, "no gradient"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn, dns, idx.int(), wt), ValueError, "idx"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn, dns, idx, wt.float()), ValueError, "weights"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn[:3], dns, idx, wt), ValueError, "down"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn, dns[:, :1], idx, wt), ValueError, "down_scales"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn, dns, idx, wt, out=b.float()), ValueError, "out"),
+        (lambda: fp8.experts(x, xs, gu, gus, dn, dns, idx, wt.clone().requires_grad_()), RuntimeError, "no gradient"),
+    ]
+    for call, error, text in cases:
+        with pytest.raises(error, match=text):
+            call()
+    with torch.no_grad():  # nothing to be tracked here
+        assert fp8.quantize_rows(grad)[0].shape == (3, 256)
+
+
+def test_tensors_without_memory_raise(dev):
+    """A tensor with no data pointer is an exception, and the device and the
+    interpreter are as they were."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        fake = torch.empty(4, 256, dtype=torch.bfloat16, device=dev)
+    out = (torch.empty(4, 256, dtype=torch.float8_e4m3fn, device=dev), torch.empty(4, 2, device=dev))
+    for _ in range(3):
+        with pytest.raises(Exception, match="(?i)fake|data pointer|storage"):
+            fp8.quantize_rows(fake, out=out)
+    assert torch.cuda.current_device() == torch.device(dev).index
+    assert fp8.quantize_rows(torch.ones(4, 256, dtype=torch.bfloat16, device=dev), out=out)[1].shape == (4, 2)
+
+
+@pytest.mark.parametrize("tokens", [1, 48, 400])
+def test_calls_from_two_threads_at_once(dev, tokens):
+    """The chain from two threads on streams of their own equals the calls one
+    after another, and no wait gives up."""
+    import threading
+
+    c = experts_case(dev, tokens, 8, 4, 512, 256)
+    g = gen(tokens + 1, dev)
+    w = randn(g, 512).to(torch.bfloat16)
+    ins = [(randn(g, tokens, 512).to(torch.bfloat16), randn(g, tokens, 512).to(torch.bfloat16)) for _ in range(2)]
+    want = [chain_of_calls(*i, w, c) for i in ins]
+    status = torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for _ in range(20):
+                    got[k] = chain_of_calls(*ins[k], w, c)
+                    fp8.experts(*got[k][:2], *c[2:], status=status[k])
+                torch.cuda.current_stream(dev).synchronize()
+        except Exception as error:  # noqa: BLE001 - shown by the main thread
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and status.sum() == 0
+    for a, b in zip(got, want):
+        assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(a, b))
+
+
 # ------------------------------------------------------------ in a model ---
 
 EXPERTS = 32
@@ -556,6 +649,59 @@ def test_patched_experts_fp8_replayed(dev, model):
         scheduled_graph.release_graphs(pool)
     assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
     pool.clear()
+
+
+def test_patched_experts_and_blocks_follow_changed_weights(dev):
+    """Weights changed in place between calls: the next call, eager or replayed,
+    is that of banks made from the new ones."""
+    from lightreason_b200 import expert_stream, moe_block, scheduled_graph
+    from tests.dropin_model import make_model
+
+    model = make_model(experts=16, layers=1, seed=41)[0]
+    layer = model.layers[0]
+    g = gen(3, dev)
+    x, weights = randn(g, 3, 2048).to(torch.bfloat16), torch.softmax(randn(g, 3, 8), -1).to(torch.bfloat16)
+    idx = torch.rand(3, 16, generator=g, device=dev).topk(8, -1)[1]
+
+    def change():
+        with torch.no_grad():
+            layer.experts.gate_up_proj[5].mul_(-1.5)
+            layer.experts.down_proj.mul_(0.7)
+            layer.gate.weight.copy_(layer.gate.weight.flip(0).clone())
+            layer.shared_expert.up_proj.weight.mul_(3)
+
+    def fresh(block):
+        pool = expert_stream.ExpertPool(dev)
+        with (moe_block.patch_moe_blocks if block else expert_stream.patch_experts)(model, mode="b200-fp8", pool=pool):
+            return layer(x[None]) if block else layer.experts(x, idx, weights)
+
+    with torch.no_grad():
+        pool = expert_stream.ExpertPool(dev)
+        with expert_stream.patch_experts(model, mode="b200-fp8", pool=pool), scheduled_graph.replay_experts(pool):
+            first = layer.experts(x, idx, weights).clone()
+            resident = pool.stats.resident_bytes
+            change()
+            second = layer.experts(x, idx, weights).clone()
+            assert pool.stats.resident_bytes == resident
+        scheduled_graph.release_graphs(pool)
+        assert not torch.equal(first, second) and torch.equal(second, fresh(False))
+        pool = expert_stream.ExpertPool(dev)
+        with moe_block.patch_moe_blocks(model, mode="b200-fp8", pool=pool):
+            first = layer(x[None])
+            change()
+            second = layer(x[None])
+        assert not torch.equal(first, second) and torch.equal(second, fresh(True))
+
+
+def test_banks_are_not_made_in_a_capture(dev):
+    """Where the first call would be recorded instead of run, it is refused."""
+    c = torch.zeros(2, 256, 64, dtype=torch.bfloat16, device=dev), torch.zeros(2, 64, 128, dtype=torch.bfloat16,
+                                                                              device=dev)
+    with pytest.raises(ValueError, match="graph capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fp8.ExpertBanks(*c, dev)
+    torch.cuda.synchronize()
+    assert fp8.ExpertBanks(*c, dev).experts == 2
 
 
 def test_layer_as_a_decoder_would_run_it(dev):

@@ -651,10 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // this warp's part of a phase-1 item is stored
         auto count_in = [&](const Item &it) {
             __syncwarp();
-            if (lane == 0) {
-                __threadfence();
-                atomicAdd(P.done + it.e, 1);
-            }
+            if (lane == 0)
+                asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(P.done + it.e) : "memory");
         };
         if constexpr (kSwap) {
             // This warp: weight rows 32q + lane of both blocks, rows NJ h .. of the tile.

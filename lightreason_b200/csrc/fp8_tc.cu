@@ -1305,12 +1305,13 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
 }
 
 // The row tile by the average rows of an expert (256 experts of 2048 x 512,
-// top-8, us at 32 / 128 / 256 / 512 / 1024 tokens, so 1 / 4 / 8 / 16 / 32 rows:
-// tiles of 16 86 / 125 / 154 / 190 / 268, of 32 88 / 123 / 148 / 168 / 205, rows
-// as M 94 / 133 / 156 / 168 / 178).
+// top-8, us at 96 / 256 / 384 / 512 / 768 / 896 / 1024 tokens, so 3 / 8 / 12 /
+// 16 / 24 / 28 / 32 rows: tiles of 16 140 / 150 / 156 / 168 / 210 / 227 / 246, of
+// 32 144 / 152 / 148 / 152 / 164 / 172 / 188, rows as M 152 / 158 / 158 / 162 /
+// 166 / 168 / 168; 128 experts of 2048 x 768 cross at the same places).
 int experts_fp8_tile(int routes, int experts) {
     const int mean = routes / experts;
-    return mean < 4 ? 16 : mean < 16 ? 32 : 0;
+    return mean < 10 ? 16 : mean <= 24 ? 32 : 0;
 }
 
 // FP32 rows cost nothing beside the weights on small batches; above 2048 routes

@@ -295,7 +295,9 @@ EXPERT_SHAPES = [(1, 8, 2, 256, 128), (1, 32, 8, 2048, 512), (2, 4, 4, 144, 128)
                  (64, 1, 1, 128, 128), (65, 3, 3, 2064, 384), (130, 8, 2, 272, 256), (300, 6, 4, 1104, 128),
                  (700, 5, 2, 512, 640), (1500, 12, 8, 512, 256), (12, 40, 12, 640, 128), (1, 40, 32, 256, 256),
                  # two passes over the routes of one token; as many experts as there may be; the cluster plan
-                 (1, 40, 12, 640, 128), (20, 1024, 8, 128, 128), (260, 64, 8, 256, 256), (1100, 300, 2, 144, 128)]
+                 (1, 40, 12, 640, 128), (20, 1024, 8, 128, 128), (260, 64, 8, 256, 256), (1100, 300, 2, 144, 128),
+                 # 9 to 25 rows an expert
+                 (300, 128, 4, 272, 256), (290, 30, 1, 1040, 128), (100, 32, 8, 512, 384), (1900, 1024, 8, 144, 128)]
 
 
 @pytest.mark.parametrize("tokens,count,top_k,hidden,inner", EXPERT_SHAPES)

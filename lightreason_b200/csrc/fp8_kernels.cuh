@@ -56,7 +56,7 @@ bool experts_fp8_wide_rows(int routes);
 // columns of x, or the GEMV kernel.
 struct LinearFp8Plan {
     int tile, split;
-    bool gemv;
+    bool gemv, pair;
 };
 LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols);
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream);

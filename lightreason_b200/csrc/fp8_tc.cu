@@ -16,7 +16,12 @@
 //  * BN = 0, rows as M: tiles of 128 rows against N = 256 weight rows.  An
 //    accumulator lane is one row, so a group's factor is one number per thread,
 //    gate and up of a column meet in one thread, and warps without rows of a
-//    partial tile skip.
+//    partial tile skip.  A plain product of more than 128 rows runs them on CTA
+//    pairs (PAIR): each CTA holds 128 of an item's 256 rows and 128 of its
+//    weight rows, multiplied by tcgen05.mma.cta_group::2 (M = 256), a third less
+//    to load for the same work.  The first CTA issues the products; both CTAs'
+//    loads complete on its barriers, its commits arrive on both CTAs', and all
+//    sixteen epilogue warps hand its buffers back.
 //  * BN = 16, 32 (64 for a plain product), weights as M: the two blocks of 128 weight rows against
 //    N = BN rows.  A lane is one weight row and the tile's few rows are its
 //    columns: at a few rows per expert all eight warps share the epilogue
@@ -62,13 +67,14 @@ constexpr int kRing = 4;        // items on their way to the warps
 constexpr int kMaxExperts = 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-// LIN: the plain product; otherwise the experts.
-template <bool LIN, int BN>
+// LIN: the plain product; otherwise the experts.  PAIR: two CTAs share an item.
+template <bool LIN, int BN, bool PAIR = false>
 struct Shape {
     static constexpr bool kSwap = BN != 0;
     static constexpr int kRows = kSwap ? BN : kBM;  // rows of a tile
-    static constexpr int kATile = kRows * kGroup, kStage = kATile + kBTile;
-    static constexpr int kStages = kSwap ? (BN == 64 ? 5 : 6) : LIN ? 3 : 4;
+    static constexpr int kB = PAIR ? kBTile / 2 : kBTile;  // a CTA's weight bytes of a stage
+    static constexpr int kATile = kRows * kGroup, kStage = kATile + kB;
+    static constexpr int kStages = kSwap ? (BN == 64 ? 5 : 6) : LIN && !PAIR ? 3 : 4;
     static constexpr int kBufs = kSwap ? 4 : 2;
     static constexpr int kBufCols = kSwap ? 2 * BN : kBN;
     // an epilogue warp's output buffer: 32 rows of 256 bytes (stored by TMA) or of 64
@@ -97,6 +103,7 @@ struct Params {
     void *out;                         // [T, n]
     int out_f32;
     int split;                         // CTAs of a cluster that share an item's groups
+    bool pair;                         // two CTAs share an item's 256 rows and its weights
     // experts
     const float *act_scales_in, *down_scales;  // phase 2: [R, I / 128], [E, blocks, I / 128]
     const int32_t *offsets;                    // [E + 1]
@@ -121,9 +128,12 @@ __device__ __forceinline__ uint64_t now_ns() {
 // leave on false: from then on their waits return at once and they run to the
 // end on whatever is there, together.  The clock (and the flag) are looked at
 // every 256th poll only: reading the global timer takes longer than most waits.
+// CLUSTER: what the other CTA of a cluster did before it arrived is seen too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort) {
     uint64_t t0 = 0;
-    for (uint32_t i = 1; !sm100::mbar_try_wait(bar, parity); ++i) {
+    for (uint32_t i = 1;
+         !(CLUSTER ? sm100::mbar_try_wait_cluster(bar, parity) : sm100::mbar_try_wait(bar, parity)); ++i) {
         if (i & 255) continue;
         if (*abort) return false;
         const uint64_t t = now_ns();
@@ -233,16 +243,17 @@ __device__ __forceinline__ void store32(void *p, const uint32_t *v) {
 // tm_x: linear, the row tiles; experts, the token rows (gathered).  tm_r, tm_r16:
 // full and 16-row boxes of the rows of linear or phase 2.  tm_w, tm_w2: weights
 // of linear or phase 1, and of phase 2.  tm_out: linear's BF16 output.
-template <bool LIN, int BN, bool SPLIT>
+template <bool LIN, int BN, bool SPLIT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_r,
                     const __grid_constant__ CUtensorMap tm_r16, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ CUtensorMap tm_out,
                     const Params P) {
     static_assert(LIN || !SPLIT, "only the plain product is split");
-    using S = Shape<LIN, BN>;
+    static_assert(!PAIR || (LIN && BN == 0 && !SPLIT), "pairs have 128 rows each of a plain product");
+    using S = Shape<LIN, BN, PAIR>;
     constexpr bool kSwap = S::kSwap;
-    constexpr int kRows = S::kRows;
+    constexpr int kRows = S::kRows, kItemRows = (PAIR ? 2 : 1) * kRows;  // rows of a CTA's part, of an item
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     // a stage: the weight tile, then the rows (both on 1024-byte boundaries)
@@ -260,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < S::kBufs; ++b) {
             sm100::mbar_init(&tail->tfull[b], 1);
-            sm100::mbar_init(&tail->tempty[b], 8);
+            sm100::mbar_init(&tail->tempty[b], PAIR ? 16 : 8);  // the epilogue warps, of both CTAs
         }
         for (int s = 0; s < kScaleSlots; ++s) {
             sm100::mbar_init(&tail->sfull[s], 32);  // the lanes of warp 3
@@ -283,11 +294,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tma_prefetch_map(&tm_r16);
     }
     if (warp == 1) {
-        sm100::tmem_alloc(&tail->tmem, 512);
-        sm100::tmem_relinquish();
+        if constexpr (PAIR) {
+            sm100::tmem_alloc_pair(&tail->tmem, 512);
+            sm100::tmem_relinquish_pair();
+        } else {
+            sm100::tmem_alloc(&tail->tmem, 512);
+            sm100::tmem_relinquish();
+        }
     }
     sm100::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) sm100::cluster_sync();  // the other CTA's barriers are there
     sm100::tc_fence_after();
     const uint32_t tmem = tail->tmem;
     grid_dependency_wait();
@@ -299,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nt1 = LIN ? 0 : P.inner / kGroup, nt2 = (n2 + kBN - 1) / kBN;
     int items1 = 0, total;
     if constexpr (LIN) {
-        total = nt2 * ((P.rows + kRows - 1) / kRows);
+        total = nt2 * ((P.rows + kItemRows - 1) / kItemRows);
     } else {
         // tiles[e]: an exclusive scan of the experts' row tiles, a few
         // neighbouring experts a thread
@@ -332,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         total = items1 + nt2 * tail->tiles[P.experts];
     }
     // SPLIT: this CTA's groups of its cluster's one item; else all of an item's
-    const int rank = SPLIT ? static_cast<int>(sm100::cluster_ctarank()) : 0;
+    const int rank = SPLIT || PAIR ? static_cast<int>(sm100::cluster_ctarank()) : 0;
     const int split0 = SPLIT ? kbs2 * rank / P.split : 0, split1 = SPLIT ? kbs2 * (rank + 1) / P.split : kbs2;
     auto decode = [&](int item) {
         Item r;
@@ -341,11 +358,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             return r;
         }
         if constexpr (LIN) {
-            r.mt = (P.rows + kRows - 1) / kRows;
+            r.mt = (P.rows + kItemRows - 1) / kItemRows;
             r.phase = 2;
             r.e = 0;
             r.n = item / r.mt;
-            r.row0 = (item % r.mt) * kRows;
+            // (of a pair's second CTA perhaps past the rows: count is then not positive)
+            r.row0 = (item % r.mt) * kItemRows + (PAIR ? rank * kRows : 0);
             r.count = min(kRows, P.rows - r.row0);
         } else {
             r.phase = item < items1 ? 1 : 2;
@@ -368,11 +386,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // The item after the last one this warp took: linear, the CTA's next of a
     // fixed order; experts, from the ring that warp 0 fills.
-    int take_at = SPLIT ? blockIdx.x / P.split : LIN ? blockIdx.x : 0;
+    int take_at = SPLIT ? blockIdx.x / P.split : PAIR ? blockIdx.x / 2 : LIN ? blockIdx.x : 0;
     auto take_item = [&]() {
         if constexpr (LIN) {
             const Item r = decode(take_at);
-            take_at += SPLIT ? total : gridDim.x;
+            take_at += SPLIT ? total : PAIR ? gridDim.x / 2 : gridDim.x;
             return r;
         } else {
             const int slot = take_at % kRing;
@@ -440,8 +458,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint8_t *b = smem + stage * S::kStage;
                     uint64_t *bar = &tail->full[stage];
                     if (one) {
-                        sm100::mbar_expect_tx(bar, kBTile);
-                        if constexpr (LIN) {
+                        // a pair's loads complete on the first CTA's barrier
+                        if (!PAIR || rank == 0) sm100::mbar_expect_tx(bar, kBTile);
+                        if constexpr (PAIR) {
+                            sm100::tma_load_2d_pair(b, &tm_w, sm100::mapa(bar, 0), kb * kGroup, r0 + 128 * rank, policy);
+                        } else if constexpr (LIN) {
                             sm100::tma_load_2d_hint(b, &tm_w, bar, kb * kGroup, r0, policy);
                             sm100::tma_load_2d_hint(b + kBTile / 2, &tm_w, bar, kb * kGroup, r1, policy);
                         } else if (p1) {
@@ -461,17 +482,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t one = sm100::elect_one();
             uint32_t buf = 0, bphase = 0;
             bool ok = true, any = false;
-            for (Item it = take_item(); ok && it.phase; it = take_item()) {
+            for (Item it = take_item(); ok && it.phase && (!PAIR || rank == 0); it = take_item()) {
                 const int kbs = !LIN && it.phase == 1 ? kbs1 : split1 - split0;
-                const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kSwap ? (it.count + 15) & ~15 : kBN);
+                const uint32_t idesc = sm100::idesc_e4m3_f32(PAIR ? 2 * kBM : kBM, kSwap ? (it.count + 15) & ~15 : kBN);
                 for (int kb = 0; kb < kbs; ++kb) {
-                    ok = wait_bar(&tail->tempty[buf], bphase ^ 1, abort) && wait_bar(&tail->full[stage], phase, abort);
+                    ok = wait_bar<PAIR>(&tail->tempty[buf], bphase ^ 1, abort) &&
+                         wait_bar<PAIR>(&tail->full[stage], phase, abort);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     sm100::tc_fence_after();
                     const uint32_t base = sm100::smem_u32(smem + stage * S::kStage), d = tmem + buf * S::kBufCols;
                     const uint64_t w = sm100::desc_kmajor_sw128(base), w1 = sm100::desc_kmajor_sw128(base + kBTile / 2);
-                    const uint64_t r = sm100::desc_kmajor_sw128(base + kBTile);
+                    const uint64_t r = sm100::desc_kmajor_sw128(base + S::kB);
                     if constexpr (kSwap) {
                         sm100::mma_e4m3<false>(d, w, r, idesc, one);
                         sm100::mma_e4m3<false>(d + BN, w1, r, idesc, one);
@@ -480,13 +502,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                             sm100::mma_e4m3<true>(d, w + 2 * kk, r + 2 * kk, idesc, one);
                             sm100::mma_e4m3<true>(d + BN, w1 + 2 * kk, r + 2 * kk, idesc, one);
                         }
+                    } else if constexpr (PAIR) {
+                        sm100::mma_e4m3_pair<false>(d, r, w, idesc, one);
+#pragma unroll
+                        for (int kk = 1; kk < 4; ++kk) sm100::mma_e4m3_pair<true>(d, r + 2 * kk, w + 2 * kk, idesc, one);
                     } else {
                         sm100::mma_e4m3<false>(d, r, w, idesc, one);
 #pragma unroll
                         for (int kk = 1; kk < 4; ++kk) sm100::mma_e4m3<true>(d, r + 2 * kk, w + 2 * kk, idesc, one);
                     }
-                    sm100::mma_commit_if(&tail->tfull[buf], one);
-                    sm100::mma_commit_if(&tail->empty[stage], one);
+                    if constexpr (PAIR) {
+                        sm100::mma_commit_pair_if(&tail->tfull[buf], one);
+                        sm100::mma_commit_pair_if(&tail->empty[stage], one);
+                    } else {
+                        sm100::mma_commit_if(&tail->tfull[buf], one);
+                        sm100::mma_commit_if(&tail->empty[stage], one);
+                    }
                     __syncwarp();
                     any = true;
                     next_stage();
@@ -497,7 +528,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (*abort && any) {
-                if (one) sm100::mma_commit(&tail->drain);
+                if (one) {
+                    if constexpr (PAIR) sm100::mma_commit_pair(&tail->drain, 1);
+                    else sm100::mma_commit(&tail->drain);
+                }
                 const uint64_t t0 = now_ns();
                 while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
                 }
@@ -510,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // with 128-row tiles gathers the second 64 rows: a warp's lanes
             // issue their gathers one after another, two warps halve that time.
             sm100::fence_proxy_async_global();
+            const uint64_t rows_policy = sm100::l2_evict_normal_policy();
             constexpr int kPerWarp = kRows / kGatherWarps;  // gathered rows of a warp
             const int g0 = kPerWarp * (warp - 2) + 4 * lane;
             uint32_t slot = 0, sphase = 0;
@@ -605,8 +640,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (warp == 3 && (LIN || kGatherWarps == 1)) continue;
                     ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
                     if (!ok) break;
-                    uint8_t *a = smem + stage * S::kStage + kBTile;
+                    uint8_t *a = smem + stage * S::kStage + S::kB;
                     uint64_t *bar = &tail->full[stage];
+                    if constexpr (PAIR) {
+                        if (lane == 0) {
+                            if (rank == 0) sm100::mbar_expect_tx(bar, 2 * S::kATile);
+                            sm100::tma_load_2d_pair(a, &tm_r, sm100::mapa(bar, 0), kb * kGroup, it.row0, rows_policy);
+                        }
+                        __syncwarp();
+                        next_stage();
+                        continue;
+                    }
                     if (lane == 0) {
                         if (loads) sm100::mbar_expect_tx(bar, boxes * box_bytes);
                         else sm100::mbar_arrive(bar);
@@ -632,7 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto release_buf = [&] {
             sm100::tc_fence_before();
             __syncwarp();
-            sm100::mbar_arrive_if(&tail->tempty[buf], lane == 0);
+            if constexpr (PAIR) sm100::mbar_arrive_cluster_if(sm100::mapa(&tail->tempty[buf], 0), lane == 0);
+            else sm100::mbar_arrive_if(&tail->tempty[buf], lane == 0);
         };
         auto next_buf = [&] {
             if (++buf == S::kBufs) {
@@ -997,14 +1042,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (now_ns() - t0 < 200000) __nanosleep(1000);
     }
     __syncthreads();
+    // a pair: no CTA leaves while the other may arrive on its barriers, or the
+    // products still write its TMEM
+    if constexpr (PAIR) sm100::cluster_sync();
     if (warp == 1) {
         sm100::tc_fence_after();
-        sm100::tmem_dealloc(tmem, 512);
+        if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem, 512);
+        else sm100::tmem_dealloc(tmem, 512);
     }
     if (LIN && *abort) {
         // NaN in place of this CTA's tiles (here, and not in the items' own
         // path, where the test alone cost a twentieth of the time)
-        for (int item = SPLIT ? blockIdx.x / P.split : blockIdx.x; item < total; item += SPLIT ? total : gridDim.x) {
+        const int step = SPLIT ? total : PAIR ? gridDim.x / 2 : gridDim.x;
+        for (int item = SPLIT ? blockIdx.x / P.split : PAIR ? blockIdx.x / 2 : blockIdx.x; item < total; item += step) {
             const Item it = decode(item);
             for (int i = threadIdx.x; i < it.count * kBN; i += kThreads) {
                 const int n = it.n * kBN + i % kBN;
@@ -1164,7 +1214,7 @@ int launch_tile(const CUtensorMap (&m)[6], const Params &P, int64_t items, cudaS
         if (P.split > 1) {
             static_assert(Shape<LIN, BN>::kStages * Shape<LIN, BN>::kStage >= Shape<LIN, BN>::kRows * kBN * 4,
                           "the partial sums fit the stages");
-            auto kernel = fp8_tile_kernel<LIN, BN, true>;
+            auto kernel = fp8_tile_kernel<LIN, BN, true, false>;
             if (int rc = ensure_dynamic_smem(kernel, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(static_cast<unsigned>(items * P.split));
@@ -1184,7 +1234,17 @@ int launch_tile(const CUtensorMap (&m)[6], const Params &P, int64_t items, cudaS
             return err == cudaSuccess ? MOE_OK : cuda_error(err, "fp8_tile_kernel");
         }
     }
-    auto kernel = fp8_tile_kernel<LIN, BN, false>;
+    if constexpr (LIN && BN == 0) {
+        if (P.pair) {
+            auto kernel = fp8_tile_kernel<true, 0, false, true>;
+            constexpr int pair_smem = Shape<true, 0, true>::kSmem;
+            if (int rc = ensure_dynamic_smem(kernel, pair_smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
+            const int clusters = static_cast<int>(std::min<int64_t>(items, grouped_pair_clusters()));
+            return launch_pdl_cluster2(kernel, dim3(2 * clusters), dim3(kThreads), pair_smem, stream, "fp8_tile_kernel",
+                                       m[0], m[1], m[2], m[3], m[4], m[5], P);
+        }
+    }
+    auto kernel = fp8_tile_kernel<LIN, BN, false, false>;
     if (int rc = ensure_dynamic_smem(kernel, smem, "cudaFuncSetAttribute(fp8_tile)")) return rc;
     return launch_pdl(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
                       dim3(kThreads), smem, stream, "fp8_tile_kernel", m[0], m[1], m[2], m[3], m[4], m[5], P);
@@ -1245,7 +1305,7 @@ LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols) {
                      kSplitUs[4] = {2.8, 2.9, 3.3, 4.5};
     constexpr int kMostCtas[4] = {148, 148, 128, 64};  // of a split 1, 2, 4, 8
     const double kbs = fp8::groups(cols), nt = (rows + kBN - 1) / kBN;
-    LinearFp8Plan best{kBM, 1, false};
+    LinearFp8Plan best{kBM, 1, false, false};
     double least = 1e300;
     for (int i = 0; i < 4; ++i) {
         const double items = nt * ((tokens + kTiles[i] - 1) / kTiles[i]);
@@ -1258,7 +1318,7 @@ LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols) {
                               (p ? kSplitUs[i] : kEndUs[i]);
             if (us < least) {
                 least = us;
-                best = LinearFp8Plan{kTiles[i], split, false};
+                best = LinearFp8Plan{kTiles[i], split, false, false};
             }
         }
     }
@@ -1268,6 +1328,11 @@ LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols) {
                                          cols / 2048.0 * (0.5 + 0.45 * tokens));
         best.gemv = us < least;
     }
+    // Pairs wherever a pair has more than one tile of rows: the cycles are the
+    // same, the power is not (8192 rows of 2048 against 4096, in a run of
+    // seconds at 1000 W: 90.6 us without, 87.3 with; of 8192 against 8192: 686 and
+    // 659; in short runs 75.6 and 73.4; 300 to 512 rows: alike).
+    best.pair = !best.gemv && best.tile == kBM && best.split == 1 && tokens > kBM && grouped_pair_clusters() > 0;
     return best;
 }
 
@@ -1294,7 +1359,9 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
     P.out_f32 = a.out_f32;
     P.status = status;
     P.split = plan.split;
-    const int64_t items = static_cast<int64_t>((a.tokens + tile - 1) / tile) * ((a.rows + kBN - 1) / kBN);
+    P.pair = plan.pair;
+    const int item_rows = plan.pair ? 2 * tile : tile;
+    const int64_t items = static_cast<int64_t>((a.tokens + item_rows - 1) / item_rows) * ((a.rows + kBN - 1) / kBN);
     LRB_REQUIRE(items < (1ll << 31), "moe_linear_fp8: too many tiles");
     switch (bn) {
         case 16: return launch_tile<true, 16>(m, P, items, stream);

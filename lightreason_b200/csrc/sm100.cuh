@@ -176,6 +176,28 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
         "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "r"(issue)
         : "memory");
 }
+// The same of a CTA pair: M = 256 and N split over both, issued by the leader.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "r"(issue)
+        : "memory");
+}
+// Arrives on `bar` in both CTAs of the pair.
+__device__ __forceinline__ void mma_commit_pair_if(uint64_t *bar, uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+            smem_u32(bar)),
+        "r"(issue), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
 __device__ __forceinline__ void mma_commit_if(uint64_t *bar, uint32_t issue) {
     asm volatile(
         "{\n\t.reg .pred q;\n\t"
@@ -289,6 +311,16 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
 // earlier writes at cluster scope
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// The arrival alone, in the lanes where `issue` is nonzero: what it orders is
+// TMEM reads (by tcgen05.fence), and a release at cluster scope would wait for
+// the thread's other memory work too (the 8192-row FP8 linear: 139 us, not 75).
+__device__ __forceinline__ void mbar_arrive_cluster_if(uint32_t addr, uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(addr),
+        "r"(issue)
+        : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
     uint32_t ok;

@@ -239,6 +239,10 @@ LINEAR_SHAPES += [(5, 2500, 7488), (5, 17000, 2064), (50, 2048, 3552), (129, 100
                   (65, 2048, 10720), (200, 4097, 2240), (400, 4097, 1056), (257, 4097, 2560), (65, 4097, 3280),
                   (257, 2052, 5120), (3000, 1001, 256), (2500, 2052, 272), (2, 8192, 8192), (4, 512, 8192)]
 
+# CTA pairs: the second CTA of the last pair with all its rows, some, one and none
+LINEAR_SHAPES += [(2048, 4096, 1024), (2300, 2304, 400), (2177, 2500, 144), (2100, 4104, 272), (130, 40000, 128),
+                  (4500, 257, 2064)]
+
 
 @pytest.mark.parametrize("tokens,rows,cols", LINEAR_SHAPES)
 def test_linear(dev, tokens, rows, cols):
@@ -262,6 +266,26 @@ def test_linear_rows_and_outside_are_left_alone(dev, tokens):
     assert got[tokens // 2].isnan().all()
     keep = torch.arange(tokens, device=dev) != tokens // 2
     assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,rows", [(2100, 4104), (2100, 4100), (2177, 2501)])
+def test_linear_pairs_leave_the_outside_alone(dev, tokens, rows, dtype):
+    """CTA pairs whose last rows fill part of one CTA: nothing beyond the output,
+    a row with NaN by itself, and the same values call after call."""
+    x, xs, w, ws = linear_case(dev, tokens, rows, 400)
+    pad = 16  # elements, so that the output stays on a 16-byte boundary
+    store = torch.full((tokens * rows + 2 * pad,), 7.0, dtype=dtype, device=dev)
+    out = store[pad:-pad].view(tokens, rows)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    fp8.linear(x, xs, w, ws, out=out, status=status)
+    want, bound = R.linear(x, xs, w, ws)
+    within(out, want, bound + (R.F32 * want.abs() if dtype is torch.float32 else R.BF * (want.abs() + bound)), "out")
+    assert store[:pad].eq(7).all() and store[-pad:].eq(7).all() and status.item() == 0
+    xs2 = xs.clone()
+    xs2[tokens - 1, 1] = float("nan")
+    got = fp8.linear(x, xs2, w, ws, out_dtype=dtype)
+    assert got[-1].isnan().all() and torch.equal(got[:-1], out[:-1])
 
 
 def test_linear_is_deterministic(dev):

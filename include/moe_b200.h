@@ -531,6 +531,13 @@ int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, ui
 int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
                    int rows, int cols, void *out, int out_f32, int32_t *status, void *stream);
 
+/* The longest that one wait inside the kernels of moe_linear_fp8 and
+ * moe_experts_fp8 may take before the kernel gives up, in nanoseconds: process-wide,
+ * 2 s at first, for the calls made from then on (a captured call keeps the limit it
+ * was captured with).  0: they give up before their first product.  Returns the
+ * limit before. */
+uint64_t moe_fp8_wait_limit(uint64_t ns);
+
 /* The routed experts (the Qwen3_5MoeExperts.forward contract of
  * moe_layer_forward with route_in) on e4m3 banks gate_up [E, 2I, H] and down
  * [E, H, I]: for each route (t, k) of expert e = idx[t, k]

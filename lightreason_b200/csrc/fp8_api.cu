@@ -57,6 +57,8 @@ Layout layout(int tokens, int experts, int top_k, int hidden, int inner) {
 
 using namespace lrb;
 
+extern "C" uint64_t moe_fp8_wait_limit(uint64_t ns) { return fp8_wait_limit(ns); }
+
 extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales,
                               int tokens, int rows, int cols, void *out, int out_f32, int32_t *status,
                               void *stream) {

@@ -59,6 +59,9 @@ struct LinearFp8Plan {
     bool gemv, pair;
 };
 LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols);
+// Sets the longest that one wait inside the tile kernel may take (ns, for the
+// launches from now on); returns what it was.
+uint64_t fp8_wait_limit(uint64_t ns);
 int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t stream);
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream);
 

@@ -47,6 +47,7 @@
 // *status, drains what is in flight and returns, and leaves NaN: in a linear's
 // tiles of that CTA, in all of an experts call's output.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include <math_constants.h>
@@ -65,7 +66,7 @@ constexpr int kThreads = 12 * 32;
 constexpr int kScaleSlots = 4;  // of four groups each
 constexpr int kRing = 4;        // items on their way to the warps
 constexpr int kMaxExperts = 1024;
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kDrainNs = 2000000000ull;  // for products in flight, when a wait gave up
 
 // LIN: the plain product; otherwise the experts.  PAIR: two CTAs share an item.
 template <bool LIN, int BN, bool PAIR = false>
@@ -117,6 +118,7 @@ struct Params {
     int32_t *done;      // [E] epilogue warps that finished an item of phase 1 (zero at launch)
     int32_t *gave_up;   // set to 1 when a wait gave up (zero at launch)
     int32_t *status;
+    uint64_t wait_ns;   // the longest that a wait may take; 0: give up before the first product
 };
 
 __device__ __forceinline__ uint64_t now_ns() {
@@ -124,29 +126,35 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
+// How long a wait may take, and the CTA's flag that one took longer.
+struct Patience {
+    volatile int *abort;
+    uint64_t ns;
+};
 // Bounded wait; false once the CTA has given up.  The epilogue warps do not
-// leave on false: from then on their waits return at once and they run to the
-// end on whatever is there, together.  The clock (and the flag) are looked at
-// every 256th poll only: reading the global timer takes longer than most waits.
-// CLUSTER: what the other CTA of a cluster did before it arrived is seen too.
+// leave on false: from then on their waits return after a few looks and they
+// run to the end on whatever is there, together.  A look that fails takes the
+// hardware 4 us; the flag and the clock are looked at after every eighth (after
+// each, the kernel is 2% slower where no look fails).  CLUSTER: what the other
+// CTA of a cluster did before it arrived is seen too.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort) {
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, const Patience &patience) {
     uint64_t t0 = 0;
     for (uint32_t i = 1;
          !(CLUSTER ? sm100::mbar_try_wait_cluster(bar, parity) : sm100::mbar_try_wait(bar, parity)); ++i) {
-        if (i & 255) continue;
-        if (*abort) return false;
+        if (i & 7) continue;
+        if (*patience.abort) return false;
         const uint64_t t = now_ns();
         if (t0 == 0) t0 = t;
-        if (t - t0 > kWaitNs) {
-            *abort = 1;
+        if (t - t0 > patience.ns) {
+            *patience.abort = 1;
             return false;
         }
     }
     return true;
 }
-__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, const Patience &patience) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, patience));
 }
 
 struct Item {
@@ -260,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *pieces = smem + S::kStages * S::kStage;
     typename S::Tail *tail = reinterpret_cast<typename S::Tail *>(pieces + 8 * S::kPiece);
     volatile int *abort = &tail->abort;
+    const Patience patience{abort, P.wait_ns};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // gate/up rows as M: two warps gather a tile's rows
     constexpr int kGatherWarps = kSwap ? 1 : 2;
@@ -283,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int q = 0; q < 4; ++q) sm100::mbar_init(&tail->half[q], kSwap ? 4 : 2);
         sm100::mbar_init(&tail->drain, 1);
-        tail->abort = 0;
+        tail->abort = P.wait_ns == 0;
         sm100::fence_barrier_init();
         sm100::tma_prefetch_map(&tm_x);
         sm100::tma_prefetch_map(&tm_w);
@@ -396,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int slot = take_at % kRing;
             Item r;
             r.phase = 0;
-            if (wait_warp(&tail->ifull[slot], (take_at / kRing) & 1, abort)) {
+            if (wait_warp(&tail->ifull[slot], (take_at / kRing) & 1, patience)) {
                 const int4 a = tail->ring[slot][0], b = tail->ring[slot][1];
                 r = Item{a.x, a.y, a.z, a.w, b.x, b.y};
             }
@@ -432,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fetched = __shfl_sync(0xffffffffu, fetched, 0);
                     const Item r = decode(fetched);
                     const int slot = put_at % kRing;
-                    ok = wait_warp(&tail->iempty[slot], ((put_at / kRing) & 1) ^ 1, abort);
+                    ok = wait_warp(&tail->iempty[slot], ((put_at / kRing) & 1) ^ 1, patience);
                     if (lane == 0) {
                         tail->ring[slot][0] = make_int4(r.phase, r.e, r.row0, r.count);
                         tail->ring[slot][1] = make_int4(r.n, r.mt, 0, 0);
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int kbs = p1 ? kbs1 : split1;
                 const int r0 = it.n * (p1 ? kGroup : kBN), r1 = p1 ? P.inner + r0 : r0 + 128;
                 for (int kb = split0; kb < kbs; ++kb) {
-                    ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
+                    ok = wait_warp(&tail->empty[stage], phase ^ 1, patience);
                     if (!ok) break;
                     uint8_t *b = smem + stage * S::kStage;
                     uint64_t *bar = &tail->full[stage];
@@ -481,13 +490,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ----------------------------------------------------- MMA issuer
             const uint32_t one = sm100::elect_one();
             uint32_t buf = 0, bphase = 0;
-            bool ok = true, any = false;
+            bool ok = !*abort, any = false;
             for (Item it = take_item(); ok && it.phase && (!PAIR || rank == 0); it = take_item()) {
                 const int kbs = !LIN && it.phase == 1 ? kbs1 : split1 - split0;
                 const uint32_t idesc = sm100::idesc_e4m3_f32(PAIR ? 2 * kBM : kBM, kSwap ? (it.count + 15) & ~15 : kBN);
                 for (int kb = 0; kb < kbs; ++kb) {
-                    ok = wait_bar<PAIR>(&tail->tempty[buf], bphase ^ 1, abort) &&
-                         wait_bar<PAIR>(&tail->full[stage], phase, abort);
+                    ok = wait_bar<PAIR>(&tail->tempty[buf], bphase ^ 1, patience) &&
+                         wait_bar<PAIR>(&tail->full[stage], phase, patience);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     sm100::tc_fence_after();
@@ -533,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     else sm100::mma_commit(&tail->drain);
                 }
                 const uint64_t t0 = now_ns();
-                while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kWaitNs) {
+                while (!sm100::mbar_try_wait(&tail->drain, 0) && now_ns() - t0 < kDrainNs) {
                 }
             }
             __syncwarp();
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int need = 8 * nt1 * it.mt;
                     const uint64_t t0 = now_ns();
                     while (sm100::ld_acquire(P.done + it.e) < need) {
-                        if (*abort || now_ns() - t0 > kWaitNs) {
+                        if (*abort || now_ns() - t0 >= P.wait_ns) {
                             *abort = 1;
                             break;
                         }
@@ -613,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kb = split0; kb < (p1 ? kbs1 : split1); ++kb) {
                     if (warp == 3 && ((kb - split0) & 3) == 0) {
                         // the scales of groups kb .. kb + 3, on their way from here
-                        ok = wait_warp(&tail->sempty[slot], sphase ^ 1, abort);
+                        ok = wait_warp(&tail->sempty[slot], sphase ^ 1, patience);
                         if (!ok) break;
 #pragma unroll
                         for (int j = 0; j < kScaleRows; ++j) {
@@ -638,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     if (warp == 3 && (LIN || kGatherWarps == 1)) continue;
-                    ok = wait_warp(&tail->empty[stage], phase ^ 1, abort);
+                    ok = wait_warp(&tail->empty[stage], phase ^ 1, patience);
                     if (!ok) break;
                     uint8_t *a = smem + stage * S::kStage + S::kB;
                     uint64_t *bar = &tail->full[stage];
@@ -711,10 +720,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) acc0[j] = acc1[j] = 0.f;
                 for (int kb = 0; kb < kbs; ++kb) {
-                    if ((kb & 3) == 0) wait_bar(&tail->sfull[slot], sphase, abort);
+                    if ((kb & 3) == 0) wait_bar(&tail->sfull[slot], sphase, patience);
                     const float b0 = reinterpret_cast<const float *>(&tail->block_scale[slot][0])[kb & 3];
                     const float b1 = reinterpret_cast<const float *>(&tail->block_scale[slot][1])[kb & 3];
-                    wait_bar(&tail->tfull[buf], bphase, abort);
+                    wait_bar(&tail->tfull[buf], bphase, patience);
                     sm100::tc_fence_after();
                     if (active) {
                         const uint32_t at = lanes + buf * S::kBufCols + j0;
@@ -753,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         __syncwarp();
                         sm100::mbar_arrive_if(&tail->half[h], lane == 0);
-                        wait_bar(&tail->half[h], iphase, abort);
+                        wait_bar(&tail->half[h], iphase, patience);
                         uint8_t *dst = P.act + static_cast<int64_t>(it.row0 + j0) * P.inner + it.n * kGroup + 32 * q + lane;
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) {
@@ -804,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the factors of the next four groups: row scale x weight scale (gate's and up's)
             float s0[4], s1[4];
             auto take_scales = [&](bool p1) {
-                wait_bar(&tail->sfull[slot], sphase, abort);
+                wait_bar(&tail->sfull[slot], sphase, patience);
                 const float4 rs = *reinterpret_cast<const float4 *>(&tail->row_scale[slot][4 * r]);
                 const float4 b0 = tail->block_scale[slot][p1 ? 0 : h];
                 s0[0] = rs.x * b0.x, s0[1] = rs.y * b0.y, s0[2] = rs.z * b0.z, s0[3] = rs.w * b0.w;
@@ -836,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         s0[i] = s0[i + 1];
                         if (!LIN) s1[i] = s1[i + 1];
                     }
-                    wait_bar(&tail->tfull[buf], bphase, abort);
+                    wait_bar(&tail->tfull[buf], bphase, patience);
                     sm100::tc_fence_after();
                     if (active) {
                         const uint32_t base = at + buf * kBN;
@@ -879,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tail->top[iphase][h][r] = top;
                         __syncwarp();
                         sm100::mbar_arrive_if(&tail->half[q], lane == 0);
-                        wait_bar(&tail->half[q], iphase, abort);
+                        wait_bar(&tail->half[q], iphase, patience);
                         top = fp8::max_nan(top, tail->top[iphase][h ^ 1][r]);
                         iphase ^= 1;
                         const fp8::Divisor f(top);
@@ -1035,13 +1044,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         sm100::cluster_sync();  // no CTA leaves while another reads its sums
     }
-    if (*abort && warp < 4) {
+    __syncthreads();  // no warp issues loads or products any more
+    const bool gave_up = *abort;
+    if (gave_up) {
         // loads may be in flight whose barriers will never complete: give them
         // a time far above any load's before the CTA leaves
         const uint64_t t0 = now_ns();
         while (now_ns() - t0 < 200000) __nanosleep(1000);
+        __syncwarp();
     }
-    __syncthreads();
     // a pair: no CTA leaves while the other may arrive on its barriers, or the
     // products still write its TMEM
     if constexpr (PAIR) sm100::cluster_sync();
@@ -1050,7 +1061,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem, 512);
         else sm100::tmem_dealloc(tmem, 512);
     }
-    if (LIN && *abort) {
+    if (LIN && gave_up) {
         // NaN in place of this CTA's tiles (here, and not in the items' own
         // path, where the test alone cost a twentieth of the time)
         const int step = SPLIT ? total : PAIR ? gridDim.x / 2 : gridDim.x;
@@ -1065,7 +1076,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
-    if (threadIdx.x == 0 && *abort) {
+    if (threadIdx.x == 0 && gave_up) {
         if (P.status) atomicExch(P.status, 1);
         if (!LIN) atomicExch(P.gave_up, 1);
     }
@@ -1285,7 +1296,11 @@ int out_map(CUtensorMap *m, const void *base, int rows, int cols) {
     return make_map_bf16(m, base, 2, dims, str, 32);
 }
 
+std::atomic<uint64_t> g_wait_ns{2000000000ull};
+
 }  // namespace
+
+uint64_t fp8_wait_limit(uint64_t ns) { return g_wait_ns.exchange(ns, std::memory_order_relaxed); }
 
 // The least of a few estimates, in microseconds, fitted to graph replays on a
 // B200 (weights of 1024 x 2048, 1000 x 1040, 2048 x 512, 4096 x 4096, 8192 x
@@ -1358,6 +1373,7 @@ int launch_linear_fp8_tiles(const LinearFp8 &a, int32_t *status, cudaStream_t st
     P.out = a.out;
     P.out_f32 = a.out_f32;
     P.status = status;
+    P.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     P.split = plan.split;
     P.pair = plan.pair;
     const int item_rows = plan.pair ? 2 * tile : tile;
@@ -1425,6 +1441,7 @@ int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, in
     P.done = s.counters + 1;
     P.gave_up = s.counters + 1 + a.experts;
     P.status = status;
+    P.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     int rc = MOE_OK;
     switch (bn) {
         case 16: rc = launch_tile<false, 16>(m, P, items, stream); break;

@@ -97,6 +97,7 @@ _SIGNATURES = {
                          _p, _p, _p], _i),
     "moe_quantize_fp8_blocks": ([_p, _i, _i, _i, _p, _p, _p], _i),
     "moe_linear_fp8": ([_p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _p], _i),
+    "moe_fp8_wait_limit": ([ctypes.c_uint64], ctypes.c_uint64),
     "moe_experts_fp8_workspace_bytes": ([_i, _i, _i, _i, _i], _sz),
     "moe_experts_fp8": ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _sz, _p, _p], _i),
     "moe_grouped_paired": ([_i, _i, _i], _i),

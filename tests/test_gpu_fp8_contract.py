@@ -1,0 +1,100 @@
+"""What the FP8 operators promise at their edges, on the GPU: waits that run
+out, weights that change under a model, values across the borders where a
+product changes its kernel."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lightreason_b200 import fp8, native
+from tests import fp8_reference as R
+from tests.test_gpu_fp8 import dev, experts_case, gen, linear_case, randn, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------ bounded waits ---
+
+@pytest.fixture
+def no_patience(dev):  # noqa: F811
+    """No product is made: every wait for one runs out."""
+    before = native.lib().moe_fp8_wait_limit(0)
+    yield
+    native.lib().moe_fp8_wait_limit(before)
+
+
+# a tile of each kind, in one piece and split over the columns
+GIVE_UP_LINEAR = [(5, 257, 272), (200, 2050, 336), (5, 2500, 7488), (33, 129, 4096), (513, 1024, 1168), (65, 4097, 3280),
+                  (129, 1000, 2096), (64, 1024, 2048), (400, 4097, 1056), (200, 4097, 2240), (1000, 511, 2048),
+                  (50, 2048, 3552), (2048, 2048, 512), (3000, 1001, 256), (257, 4097, 2560), (257, 2048, 6192),
+                  (65, 2048, 10720)]
+
+
+def give_up_linear(dev, tokens, rows, cols, dtype):  # noqa: F811
+    """A product whose waits run out: NaN throughout, status 1, nothing beyond
+    the output; then the same call with patience."""
+    x, xs, w, ws = linear_case(dev, tokens, rows, cols)
+    pad = 16  # elements, so that the output stays on a 16-byte boundary
+    store = torch.full((tokens * rows + 2 * pad,), 7.0, dtype=dtype, device=dev)
+    out = store[pad:-pad].view(tokens, rows)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    fp8.linear(x, xs, w, ws, out=out, status=status)
+    torch.cuda.synchronize()
+    assert status.item() == 1 and out.isnan().all()
+    assert store[:pad].eq(7).all() and store[-pad:].eq(7).all()
+    limit = native.lib().moe_fp8_wait_limit(2_000_000_000)
+    status.zero_()
+    fp8.linear(x, xs, w, ws, out=out, status=status)
+    native.lib().moe_fp8_wait_limit(limit)
+    want, bound = R.linear(x, xs, w, ws)
+    within(out, want, bound + (R.F32 * want.abs() if dtype is torch.float32 else R.BF * (want.abs() + bound)), "out")
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("tokens,rows,cols", GIVE_UP_LINEAR)
+def test_linear_that_gives_up_holds_nan(dev, no_patience, tokens, rows, cols):  # noqa: F811
+    give_up_linear(dev, tokens, rows, cols, torch.bfloat16 if rows % 2 else torch.float32)
+
+
+@pytest.mark.parametrize("tokens,count,top_k,hidden,inner", [(17, 16, 2, 272, 128), (40, 16, 8, 512, 256),
+                                                             (300, 6, 4, 1104, 128), (600, 40, 8, 256, 128)])
+def test_experts_that_give_up_hold_nan(dev, no_patience, tokens, count, top_k, hidden, inner):  # noqa: F811
+    """Tiles of 16, 32 and 128 rows, route rows in FP32 and BF16."""
+    c = experts_case(dev, tokens, count, top_k, hidden, inner)
+    store = torch.full((tokens + 2, hidden), 7.0, dtype=torch.bfloat16, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    fp8.experts(*c, out=store[1:-1], status=status)
+    torch.cuda.synchronize()
+    assert status.item() == 1 and store[1:-1].isnan().all()
+    assert store[0].eq(7).all() and store[-1].eq(7).all()
+    native.lib().moe_fp8_wait_limit(2_000_000_000)
+    status.zero_()
+    got = fp8.experts(*c, status=status)
+    want, bound = R.experts(*c)
+    within(got, want, bound, "out")
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("tokens,count,top_k,hidden,inner", [(40, 64, 8, 1024, 512), (600, 40, 8, 1024, 512)])
+def test_experts_that_give_up_half_way(dev, tokens, count, top_k, hidden, inner):  # noqa: F811
+    """With a limit of a nanosecond the down items give up where their rows are
+    not there yet: NaN throughout and status 1, or, if none had to wait, the values."""
+    c = experts_case(dev, tokens, count, top_k, hidden, inner)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    want, bound = R.experts(*c)
+    before = native.lib().moe_fp8_wait_limit(1)
+    try:
+        outs = []
+        for _ in range(5):
+            status.zero_()
+            outs.append((fp8.experts(*c, status=status), status.clone()))
+        torch.cuda.synchronize()
+    finally:
+        native.lib().moe_fp8_wait_limit(before)
+    for out, status in outs:
+        if status.item():
+            assert out.isnan().all()
+        else:
+            within(out, want, bound, "out")
+    within(fp8.experts(*c), want, bound, "afterwards")

@@ -45,7 +45,7 @@
 // first four hand registers to the others (72 and 216, the experts' 104 and
 // 200, a thread of 168 at launch: 64,512 a CTA either way).  Every wait is bounded; a timeout raises
 // *status, drains what is in flight and returns, and leaves NaN: in a linear's
-// tiles of that CTA, in all of an experts call's output.
+// tiles of that CTA or pair, in all of an experts call's output.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -88,7 +88,7 @@ struct Shape {
         int4 ring[kRing][2];
         uint64_t full[kStages], empty[kStages], tfull[kBufs], tempty[kBufs], sfull[kScaleSlots], sempty[kScaleSlots],
             ifull[kRing], iempty[kRing], half[4], drain;
-        int abort;
+        int abort, other_abort;  // this CTA, the other of its pair gave up
         uint32_t tmem;
         int32_t scan[16];
         int32_t tiles[LIN ? 1 : kMaxExperts + 1];  // row tiles of the experts before e
@@ -293,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 4; ++q) sm100::mbar_init(&tail->half[q], kSwap ? 4 : 2);
         sm100::mbar_init(&tail->drain, 1);
         tail->abort = P.wait_ns == 0;
+        tail->other_abort = 0;
         sm100::fence_barrier_init();
         sm100::tma_prefetch_map(&tm_x);
         sm100::tma_prefetch_map(&tm_w);
@@ -1045,17 +1046,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::cluster_sync();  // no CTA leaves while another reads its sums
     }
     __syncthreads();  // no warp issues loads or products any more
-    const bool gave_up = *abort;
+    if constexpr (PAIR) {
+        // A pair gives up together: once one of its CTAs has, its epilogue warps
+        // hand buffers back unread, and those count for the other's.  Nor does a
+        // CTA leave while the other may arrive on its barriers.
+        if (threadIdx.x == 0 && *abort) sm100::st_cluster_u32(sm100::mapa(&tail->other_abort, rank ^ 1), 1);
+        __syncwarp();
+        sm100::cluster_sync();
+    }
+    const bool gave_up = *abort || (PAIR && *static_cast<volatile int *>(&tail->other_abort));
     if (gave_up) {
-        // loads may be in flight whose barriers will never complete: give them
-        // a time far above any load's before the CTA leaves
+        // loads and products may be in flight whose barriers will never
+        // complete: give them a time far above any load's before the CTA leaves
         const uint64_t t0 = now_ns();
         while (now_ns() - t0 < 200000) __nanosleep(1000);
         __syncwarp();
     }
-    // a pair: no CTA leaves while the other may arrive on its barriers, or the
-    // products still write its TMEM
-    if constexpr (PAIR) sm100::cluster_sync();
     if (warp == 1) {
         sm100::tc_fence_after();
         if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem, 512);

@@ -31,6 +31,12 @@ GIVE_UP_LINEAR = [(5, 257, 272), (200, 2050, 336), (5, 2500, 7488), (33, 129, 40
                   (65, 2048, 10720)]
 
 
+# CTA pairs (at least 64 groups of columns a CTA): the second CTA of the last pair with all
+# its rows, some, one and none; widths on and off 16-byte units
+PAIR_SHAPES = [(1024, 5001, 4000), (2560, 1000, 8128), (2198, 2052, 3984), (385, 5001, 8176), (1153, 4104, 4000),
+               (2049, 2052, 4000), (1025, 4104, 3984), (1044, 4097, 4016)]
+
+
 def give_up_linear(dev, tokens, rows, cols, dtype):  # noqa: F811
     """A product whose waits run out: NaN throughout, status 1, nothing beyond
     the output; then the same call with patience."""
@@ -55,6 +61,12 @@ def give_up_linear(dev, tokens, rows, cols, dtype):  # noqa: F811
 @pytest.mark.parametrize("tokens,rows,cols", GIVE_UP_LINEAR)
 def test_linear_that_gives_up_holds_nan(dev, no_patience, tokens, rows, cols):  # noqa: F811
     give_up_linear(dev, tokens, rows, cols, torch.bfloat16 if rows % 2 else torch.float32)
+
+
+@pytest.mark.parametrize("tokens,rows,cols", PAIR_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_pairs_that_give_up_hold_nan_in_both_halves(dev, no_patience, tokens, rows, cols, dtype):  # noqa: F811
+    give_up_linear(dev, tokens, rows, cols, dtype)
 
 
 @pytest.mark.parametrize("tokens,count,top_k,hidden,inner", [(17, 16, 2, 272, 128), (40, 16, 8, 512, 256),

@@ -487,6 +487,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     next_stage();
                 }
             }
+            // the first CTA's products read this CTA's stages and arrive on its
+            // barriers: all of them have before it may leave
+            if constexpr (PAIR)
+                for (int i = 0; ok && i < S::kStages; ++i) {
+                    ok = wait_warp(&tail->empty[stage], phase ^ 1, patience);
+                    next_stage();
+                }
         } else if (warp == 1) {
             // ----------------------------------------------------- MMA issuer
             const uint32_t one = sm100::elect_one();

@@ -110,3 +110,16 @@ def test_experts_that_give_up_half_way(dev, tokens, count, top_k, hidden, inner)
         else:
             within(out, want, bound, "out")
     within(fp8.experts(*c), want, bound, "afterwards")
+
+
+def test_linear_pairs_back_to_back(dev):  # noqa: F811
+    """Pairs right behind other pairs and single CTAs on the same SMs, on both
+    dtypes: the same values every time, no wait gives up."""
+    shapes = [(1025, 4104, 3984, torch.bfloat16), (2198, 2052, 3984, torch.float32), (5, 2500, 7488, torch.bfloat16),
+              (1044, 4097, 4016, torch.bfloat16)]
+    cases = [(linear_case(dev, *s[:3]), s[3]) for s in shapes]
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    first = [fp8.linear(*c, out_dtype=d) for c, d in cases]
+    torch.cuda.synchronize()
+    again = [[fp8.linear(*c, out_dtype=d, status=status) for c, d in cases] for _ in range(8)]
+    assert all(torch.equal(a, b) for outs in again for a, b in zip(outs, first)) and status.item() == 0

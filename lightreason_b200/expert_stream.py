@@ -109,7 +109,9 @@ class ExpertPool:
         self.stats = TransferStats(resident_bytes=self.stats.resident_bytes, pinned_bytes=self.stats.pinned_bytes)
 
     def clear(self):
-        """Release device copies, host mappings and packed banks."""
+        """Release device copies, host mappings and packed banks, and the
+        captured expert calls (scheduled_graph.replay_experts) that read them."""
+        getattr(self, "replay_graphs", {}).clear()
         for layer in self._layers.values():
             layer.release()
         self._layers.clear()
@@ -149,11 +151,11 @@ class ExpertPool:
                     layer.module.num_experts, layer.module.hidden_dim, layer.module.intermediate_dim):
                 banks.load(layer.gate_up, layer.down, shared=shared, extra=extra)
                 return banks
-            # another module's, gone, under the same id: its captured calls go too
-            self.stats.resident_bytes -= banks.nbytes()
-            graphs = getattr(self, "replay_graphs", {})
-            for old in [k for k in graphs if k[:2] == key[:2]]:
-                del graphs[old]
+            self.stats.resident_bytes -= banks.nbytes()  # another module's, gone, under the same id
+        # calls captured on other banks under this key go with those
+        graphs = getattr(self, "replay_graphs", {})
+        for old in [k for k in graphs if k[:2] == key[:2]]:
+            del graphs[old]
         banks = self._layers[key] = fp8.ExpertBanks(layer.gate_up, layer.down, self.device, shared=shared, extra=extra)
         self.stats.resident_bytes += banks.nbytes()
         return banks

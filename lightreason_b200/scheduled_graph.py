@@ -14,8 +14,8 @@ the ordinary path.
 As in the reference, the returned tensor is the graph's static output: it is
 valid until the next replay of the same layer at the same width.  Graphs
 persist on the pool (`pool.replay_graphs`) across contexts; `pool.clear()`
-releases the native layers they use, so clear the graphs first
-(`release_graphs(pool)`).
+releases the layers they use and drops them too, `release_graphs(pool)` drops
+them alone.
 """
 
 from __future__ import annotations

@@ -123,3 +123,40 @@ def test_linear_pairs_back_to_back(dev):  # noqa: F811
     torch.cuda.synchronize()
     again = [[fp8.linear(*c, out_dtype=d, status=status) for c, d in cases] for _ in range(8)]
     assert all(torch.equal(a, b) for outs in again for a, b in zip(outs, first)) and status.item() == 0
+
+
+# ------------------------------------------------------------ in a model ---
+
+def small_model(seed):
+    from tests.dropin_model import make_model
+
+    return make_model(experts=16, layers=1, seed=seed)[0]
+
+
+def model_inputs(dev, tokens, seed):  # noqa: F811
+    g = gen(seed, dev)
+    idx = torch.rand(tokens, 16, generator=g, device=dev).topk(8, -1)[1]
+    return randn(g, tokens, 2048).to(torch.bfloat16), idx, torch.softmax(randn(g, tokens, 8), -1).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("mode", ["b200-fp8", "b200"])
+def test_clear_between_replayed_calls(dev, mode):  # noqa: F811
+    """After pool.clear() a replayed call is captured on new banks, with the
+    values of weights changed where nothing sees it."""
+    from lightreason_b200 import expert_stream, scheduled_graph
+
+    model = small_model(43)
+    layer, args = model.layers[0], model_inputs(dev, 3, 5)
+    pool = expert_stream.ExpertPool(dev)
+    with torch.no_grad(), expert_stream.patch_experts(model, mode=mode, pool=pool):
+        with scheduled_graph.replay_experts(pool):
+            first = layer.experts(*args).clone()
+            layer.experts.down_proj.data.mul_(2)
+            pool.clear()
+            taken = [torch.full((64 << 20,), 0x7f, dtype=torch.uint8, device=dev) for _ in range(4)]  # the banks' old memory
+            second = layer.experts(*args).clone()
+            third = layer.experts(*args).clone()
+            del taken
+        eager = layer.experts(*args)
+    assert torch.equal(second, 2 * first) and torch.equal(third, second) and torch.equal(eager, second)
+    pool.clear()

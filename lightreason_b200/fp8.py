@@ -261,8 +261,12 @@ class ExpertBanks:
                  "FP8 banks cannot be made during a graph capture: call the layer once before it")
         count, hidden, inner = self.experts, self.hidden, self.inner
         _require(tuple(gate_up.shape) == (count, 2 * inner, hidden) and tuple(down.shape) == (count, hidden, inner)
-                 and self.gate_up.shape[0] == count + bool(shared) and len(extra) == len(self.extra),
+                 and self.gate_up.shape[0] == count + bool(shared)
+                 and [t.shape for t in extra] == [t.shape for t in self.extra],
                  "the weights do not have the banks' shapes")
+        _require(not shared or [tuple(t.shape) for t in shared] == [(inner, hidden)] * 2 + [(hidden, inner)],
+                 "the shared expert must have the experts' widths")
+        self._sources = []  # held only once all of them are there
         parts = [(a, min(a + self.CHUNK, count)) for a in range(0, count, self.CHUNK)]
         with torch.no_grad():
             for source, q, scales in ((gate_up, self.gate_up, self.gate_up_scales),
@@ -271,8 +275,6 @@ class ExpertBanks:
                     quantize_blocks(source[a:b].detach().to(self.device).contiguous(), out=(q[a:b], scales[a:b]))
             if shared:
                 gate, up, last = (t.detach().to(self.device) for t in shared)
-                _require(tuple(gate.shape) == tuple(up.shape) == (inner, hidden)
-                         and tuple(last.shape) == (hidden, inner), "the shared expert must have the experts' widths")
                 quantize_blocks(torch.cat([gate, up])[None], out=(self.gate_up[count:], self.gate_up_scales[count:]))
                 quantize_blocks(last[None].contiguous(), out=(self.down[count:], self.down_scales[count:]))
             for held, t in zip(self.extra, extra):

@@ -49,3 +49,57 @@ def test_captured_calls_go_with_the_banks_they_read(monkeypatch):
     pool.replay_graphs[key] = "captured"
     pool.clear()
     assert pool.replay_graphs == {} and pool.stats.resident_bytes == 0
+
+
+@pytest.fixture
+def quantised(monkeypatch):
+    """quantize_blocks on the CPU (values alone); the list of its calls' shapes, and one to fail at."""
+    calls = SimpleNamespace(shapes=[], fail_at=None)
+
+    def fake(w, out):
+        if len(calls.shapes) == calls.fail_at:
+            raise RuntimeError("out of memory")
+        calls.shapes.append(tuple(w.shape))
+        out[0].copy_(w.to(E4M3))
+        out[1].fill_(float(w.flatten()[0]))
+
+    monkeypatch.setattr(fp8, "quantize_blocks", fake)
+    return calls
+
+
+def bank_weights(value=1.0):
+    """Experts' gate_up and down, a shared expert, a router."""
+    full = lambda *s: torch.full(s, value, dtype=torch.bfloat16)  # noqa: E731
+    return full(20, 256, 64), full(20, 64, 128), [full(128, 64), full(128, 64), full(64, 128)], full(20, 64)
+
+
+def test_banks_half_loaded_hold_nothing(quantised):
+    """A load that fails on its way leaves banks that hold no weights, those
+    of before the call neither."""
+    gu, dn, shared, router = bank_weights()
+    banks = fp8.ExpertBanks(gu, dn, "cpu", shared=shared, extra=(router,))
+    assert banks.holds(gu, dn, *shared, router)
+    other = bank_weights(2.0)
+    for at in range(6):
+        quantised.shapes.clear()
+        quantised.fail_at = at
+        with pytest.raises(RuntimeError, match="out of memory"):
+            banks.load(*other[:2], shared=other[2], extra=(other[3],))
+        assert not banks.holds(gu, dn, *shared, router) and not banks.holds(*other[:2], *other[2], other[3])
+        quantised.fail_at = None
+        banks.load(gu, dn, shared=shared, extra=(router,))
+        assert banks.holds(gu, dn, *shared, router)
+
+
+def test_banks_check_every_shape_before_they_write(quantised):
+    gu, dn, shared, router = bank_weights()
+    banks = fp8.ExpertBanks(gu, dn, "cpu", shared=shared, extra=(router,))
+    quantised.shapes.clear()
+    gu2, dn2, shared2, router2 = bank_weights(2.0)
+    for wrong in ([shared2[0], shared2[1][:64], shared2[2]], [*shared2[:2], shared2[2][:, :64]], shared2[:2]):
+        with pytest.raises(ValueError, match="widths"):
+            banks.load(gu2, dn2, shared=wrong, extra=(router2,))
+    for extra in ((router2[:1],), (router2, router2), ()):
+        with pytest.raises(ValueError, match="shapes"):
+            banks.load(gu2, dn2, shared=shared2, extra=extra)
+    assert quantised.shapes == [] and banks.extra[0].eq(1).all() and banks.holds(gu, dn, *shared, router)

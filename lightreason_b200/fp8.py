@@ -248,10 +248,10 @@ class ExpertBanks:
         self.experts, self.hidden, self.inner, self.device = count, hidden, inner, torch.device(device)
         make = lambda n, k: (torch.empty((total, n, k), dtype=E4M3, device=self.device),  # noqa: E731
                              torch.empty((total, _groups(n), _groups(k)), dtype=_F32, device=self.device))
-        self.gate_up, self.gate_up_scales = make(rows, hidden)
-        self.down, self.down_scales = make(hidden, inner)
-        self.extra = tuple(torch.empty_like(t, device=self.device, memory_format=torch.contiguous_format)
-                           for t in extra)
+        with torch.inference_mode(False):  # a later load may come from outside inference mode
+            self.gate_up, self.gate_up_scales = make(rows, hidden)
+            self.down, self.down_scales = make(hidden, inner)
+            self.extra = tuple(torch.empty(t.shape, dtype=t.dtype, device=self.device) for t in extra)
         self.load(gate_up, down, shared=shared, extra=extra)
 
     def load(self, gate_up: torch.Tensor, down: torch.Tensor, *, shared=(), extra=()) -> None:

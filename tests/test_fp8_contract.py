@@ -103,3 +103,16 @@ def test_banks_check_every_shape_before_they_write(quantised):
         with pytest.raises(ValueError, match="shapes"):
             banks.load(gu2, dn2, shared=shared2, extra=extra)
     assert quantised.shapes == [] and banks.extra[0].eq(1).all() and banks.holds(gu, dn, *shared, router)
+
+
+@pytest.mark.parametrize("first,then", [(torch.inference_mode, torch.no_grad), (torch.no_grad, torch.inference_mode)])
+def test_banks_made_and_loaded_in_either_mode(quantised, first, then):
+    """Banks made in inference mode are loaded again outside it, and the other way round."""
+    gu, dn, shared, router = bank_weights()
+    with first():
+        banks = fp8.ExpertBanks(gu, dn, "cpu", shared=shared, extra=(router,))
+    router.mul_(3)
+    with then():
+        assert not banks.holds(gu, dn, *shared, router)
+        banks.load(gu, dn, shared=shared, extra=(router,))
+        assert banks.holds(gu, dn, *shared, router) and banks.extra[0].eq(3).all()

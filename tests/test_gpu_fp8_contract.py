@@ -160,3 +160,28 @@ def test_clear_between_replayed_calls(dev, mode):  # noqa: F811
         eager = layer.experts(*args)
     assert torch.equal(second, 2 * first) and torch.equal(third, second) and torch.equal(eager, second)
     pool.clear()
+
+
+def test_block_made_in_inference_mode_and_called_outside_it(dev):  # noqa: F811
+    """Router, shared expert and experts changed between a call in inference
+    mode and one under no_grad: the second has the new values."""
+    from lightreason_b200 import expert_stream, moe_block
+
+    model = small_model(44)
+    layer, x = model.layers[0], model_inputs(dev, 3, 6)[0][None]
+
+    def fresh():
+        with torch.no_grad(), moe_block.patch_moe_blocks(model, mode="b200-fp8", pool=expert_stream.ExpertPool(dev)):
+            return layer(x)
+
+    pool = expert_stream.ExpertPool(dev)
+    with moe_block.patch_moe_blocks(model, mode="b200-fp8", pool=pool):
+        with torch.inference_mode():
+            first = layer(x)
+        with torch.no_grad():
+            layer.gate.weight.copy_(layer.gate.weight.flip(0).clone())
+            layer.experts.down_proj.mul_(0.5)
+            second = layer(x)
+        with torch.inference_mode():
+            third = layer(x)
+    assert not torch.equal(first, second) and torch.equal(second, fresh()) and torch.equal(third, second)

@@ -547,7 +547,8 @@ uint64_t moe_fp8_wait_limit(uint64_t ns);
  * routes keep each route's row as BF16 before the weighted sum.  Ids
  * outside [0, E) contribute nothing (a token with none left is 0).  hidden is
  * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024.
- * status as in moe_linear_fp8. */
+ * status as in moe_linear_fp8.  The workspace of a number of tokens also does for
+ * any smaller one (0 bytes: arguments that are refused, or no tokens). */
 size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner);
 int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up, const float *gate_up_scales,
                     const uint8_t *down, const float *down_scales, const int64_t *idx, const uint16_t *weights,

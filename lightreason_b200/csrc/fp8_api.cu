@@ -1,5 +1,7 @@
 // C entry points of the FP8 products: argument checks, workspaces and the
 // choice of kernel by size.
+#include <algorithm>
+
 #include "fp8_kernels.cuh"
 
 namespace lrb {
@@ -79,7 +81,12 @@ extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uin
 
 extern "C" size_t moe_experts_fp8_workspace_bytes(int tokens, int experts, int top_k, int hidden, int inner) {
     if (check_experts(tokens, experts, top_k, hidden, inner) != MOE_OK) return 0;
-    return layout(tokens, experts, top_k, hidden, inner).bytes;
+    // A layout grows with the tokens up to where the next one, perhaps smaller,
+    // takes over: the largest of all up to `tokens`.
+    size_t bytes = 0;
+    for (const int most : {tokens, kGemvRoutes / top_k, kWideRoutes / top_k})
+        bytes = std::max(bytes, layout(std::min(tokens, most), experts, top_k, hidden, inner).bytes);
+    return bytes;
 }
 
 extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const uint8_t *gate_up,
@@ -94,13 +101,12 @@ extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const ui
     LRB_REQUIRE(aligned(x, 16) && aligned(gate_up, 16) && aligned(down, 16) && aligned(x_scales, 4) &&
                     aligned(gate_up_scales, 4) && aligned(down_scales, 4) && aligned(out, 16),
                 "moe_experts_fp8: x, the banks and out must be 16-byte aligned");
-    const size_t need = moe_experts_fp8_workspace_bytes(tokens, experts, top_k, hidden, inner);
-    LRB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need,
-                "moe_experts_fp8: workspace of %zu bytes (256-byte aligned) required", need);
+    const Layout l = layout(tokens, experts, top_k, hidden, inner);
+    LRB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes,
+                "moe_experts_fp8: workspace of %zu bytes (256-byte aligned) required", l.bytes);
     if (int rc = require_sm100()) return rc;
     const ExpertsFp8 a{x, x_scales, gate_up, down, gate_up_scales, down_scales, idx, weights, tokens, experts, top_k,
                        hidden, inner, out};
-    const Layout l = layout(tokens, experts, top_k, hidden, inner);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     if (l.gemv) return launch_experts_fp8_gemv(a, reinterpret_cast<float *>(ws), as_stream(stream));
     auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(ws + at); };

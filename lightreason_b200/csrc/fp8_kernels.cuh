@@ -50,7 +50,9 @@ struct ExpertsFp8Scratch {
 };
 // Rows of the experts' tiles: 16, 32 (weights as M) or 0 for 128 (rows as M).
 int experts_fp8_tile(int routes, int experts);
-// Whether a route's down row is kept in FP32 until the weighted sum.
+// Whether a route's down row is kept in FP32 until the weighted sum: up to so
+// many routes of a call.
+constexpr int kWideRoutes = 2048;
 bool experts_fp8_wide_rows(int routes);
 // How a plain product is cut: rows of x per tile, CTAs that share a tile's
 // columns of x, or the GEMV kernel.

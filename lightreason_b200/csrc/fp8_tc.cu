@@ -1413,7 +1413,7 @@ int experts_fp8_tile(int routes, int experts) {
 // FP32 rows cost nothing beside the weights on small batches; above 2048 routes
 // they are rounded to BF16, half the traffic of what then takes a tenth of the
 // time.
-bool experts_fp8_wide_rows(int routes) { return routes <= 2048; }
+bool experts_fp8_wide_rows(int routes) { return routes <= kWideRoutes; }
 
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream) {
     const int routes = a.tokens * a.top_k;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+import re
 from types import SimpleNamespace
 
 import pytest
@@ -116,3 +118,20 @@ def test_banks_made_and_loaded_in_either_mode(quantised, first, then):
         assert not banks.holds(gu, dn, *shared, router)
         banks.load(gu, dn, shared=shared, extra=(router,))
         assert banks.holds(gu, dn, *shared, router) and banks.extra[0].eq(3).all()
+
+
+@pytest.mark.parametrize("experts,top_k,hidden,inner", [(256, 8, 2048, 512), (256, 1, 2048, 512), (8, 2, 16, 16384),
+                                                        (64, 12, 272, 128), (1024, 32, 4096, 1024), (3, 5, 65536, 128)])
+def test_experts_workspace_does_for_fewer_tokens(so, experts, top_k, hidden, inner):
+    """A caller that sizes the workspace once, for its largest batch, has enough
+    for every smaller one: across 12 and 13 routes, 2048 and 2049."""
+    need = lambda t: so.moe_experts_fp8_workspace_bytes(t, experts, top_k, hidden, inner)  # noqa: E731
+    edges = {r // top_k + d for r in (12, 2048) for d in (-1, 0, 1, 2)}
+    counts = sorted({t for t in (*range(1, 30), *range(30, 5000, 61), *edges) if t > 0})
+    sizes = [need(t) for t in counts]
+    assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
+    P = ctypes.c_void_p(1 << 20)
+    for t in counts:  # what each call itself asks for (none gets past that: the pointers are not memory)
+        rc = so.moe_experts_fp8(P, P, P, P, P, P, P, P, t, experts, top_k, hidden, inner, P, P, 0, None, None)
+        asked = re.search(rb"workspace of (\d+) bytes", so.moe_last_error())
+        assert rc == native.MOE_EINVAL and 0 < int(asked[1]) <= need(t) <= sizes[-1], t

@@ -19,6 +19,26 @@ constexpr float kTiny = 1e-10f;   // a group's maximum counts as at least this
 
 __host__ __device__ constexpr int groups(int n) { return (n + kGroup - 1) / kGroup; }
 
+// 16 bytes that a kernel before this one may have written.  Kernels of a stream
+// overlap here (programmatic dependent launch), so such data changes while this
+// kernel is already running, before its griddepcontrol.wait: the read-only path
+// (ld.global.nc, __ldg), which is for data that nobody writes until the kernel
+// ends, is not for it.  ld_once: for what is read once.
+__device__ __forceinline__ uint4 ld_once(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 ld_again(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 // The larger of two magnitudes, NaN if either is: a group that holds a NaN
 // must not come out as numbers.
 __device__ __forceinline__ float max_nan(float a, float b) {

@@ -12,6 +12,8 @@ namespace {
 using fp8::dot16;
 using fp8::kGroup;
 using fp8::halves16;
+using fp8::ld_again;
+using fp8::ld_once;
 
 constexpr int kWarps = 8;
 constexpr int kChunk = 32 * 16;  // weight bytes a warp reads per load
@@ -41,7 +43,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_gemv_kernel(LinearFp8 a) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int c = c0 + u * kChunk;
-                v[u] = c < a.cols ? ld_cached(w + c) : make_uint4(0, 0, 0, 0);
+                v[u] = c < a.cols ? ld_again(w + c) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
@@ -52,7 +54,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_gemv_kernel(LinearFp8 a) {
                 for (int m = 0; m < MT; ++m) {
                     const int t = min(m0 + m, a.tokens - 1);
                     uint16_t x[16];
-                    halves16(ld_cached(a.x + static_cast<int64_t>(t) * a.cols + c), x);
+                    halves16(ld_again(a.x + static_cast<int64_t>(t) * a.cols + c), x);
                     acc[m] = fmaf(dot16(v[u], x), s * a.x_scales[static_cast<int64_t>(t) * gk + c / kGroup], acc[m]);
                 }
             }
@@ -102,14 +104,14 @@ __global__ void __launch_bounds__(kWarps * 32) gate_up_gemv_kernel(ExpertsFp8 a,
         for (int u = 0; u < kUnroll; ++u) {
             const int c = c0 + u * kChunk;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[u][i] = c < a.hidden ? ld_stream(w[i] + c) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 4; ++i) v[u][i] = c < a.hidden ? ld_once(w[i] + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int c = c0 + u * kChunk;
             if (c >= a.hidden) break;
             uint16_t f[16];
-            halves16(ld_cached(x + c), f);
+            halves16(ld_again(x + c), f);
             const float s = xs[c / kGroup], g = s * gs[c / kGroup], up = s * us[c / kGroup];
             acc[0] = fmaf(dot16(v[u][0], f), g, acc[0]);
             acc[1] = fmaf(dot16(v[u][1], f), g, acc[1]);
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
         auto row = [&](int j) { return a.down + (static_cast<int64_t>(e[j]) * a.hidden + n) * a.inner; };
 #pragma unroll
         for (int j = 0; j < kRoutes; ++j)
-            v[j] = live && e[j] >= 0 && lane * 16 < a.inner ? ld_stream(row(j) + lane * 16) : make_uint4(0, 0, 0, 0);
+            v[j] = live && e[j] >= 0 && lane * 16 < a.inner ? ld_once(row(j) + lane * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < kRoutes; ++j) {
             sc[j] = live && e[j] >= 0 && lane * 16 < a.inner
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
             const float *ws = a.down_scales + (static_cast<int64_t>(e[j]) * gn + n / kGroup) * gi;
             float part = 0.f;
             for (int c = lane * 16; c < a.inner; c += kChunk) {
-                const uint4 w = c == lane * 16 ? v[j] : ld_stream(row(j) + c);
+                const uint4 w = c == lane * 16 ? v[j] : ld_once(row(j) + c);
                 uint16_t f[16];
                 halves16(*reinterpret_cast<const uint4 *>(act + j * a.inner + c), f);
                 part = fmaf(dot16(w, f), (c == lane * 16 ? sc[j] : ws[c / kGroup]) * acts[j * gi + c / kGroup], part);

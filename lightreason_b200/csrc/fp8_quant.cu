@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) row_kernel(RowArgs a) {
         unpack8(v[j], y);
         if constexpr (NORM) {
             float w[8];
-            unpack8(u < units ? ld_cached(a.weight + u * 8) : make_uint4(0, 0, 0, 0), w);
+            unpack8(u < units ? fp8::ld_again(a.weight + u * 8) : make_uint4(0, 0, 0, 0), w);
 #pragma unroll
             for (int c = 0; c < 8; ++c) y[c] = y[c] * inv * (a.offset + w[c]);
             if (a.normed && row && u < units)
@@ -233,7 +233,7 @@ int rows_for(const RowArgs &a, cudaStream_t stream) {
 // where the 98 registers it would take allow two: one layer's gate/up bank
 // (1.6 GB moved) 285 us, 5.65 TB/s, against 336.
 template <bool VEC>
-__global__ void __launch_bounds__(256, VEC ? 4 : 1) block_kernel(const uint16_t *__restrict__ w, int rows, int cols,
+__global__ void __launch_bounds__(256, VEC ? 4 : 1) block_kernel(const uint16_t *w, int rows, int cols,
                                                     uint8_t *__restrict__ q, float *__restrict__ scales) {
     __shared__ float part[8];
     grid_dependency_wait();
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 1) block_kernel(const uint16_t 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = r0 + 16 * j;
-            v[j] = r < rows && c < cols ? ld_stream(w + base + static_cast<int64_t>(r) * cols + c)
+            v[j] = r < rows && c < cols ? fp8::ld_once(w + base + static_cast<int64_t>(r) * cols + c)
                                         : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll

@@ -1101,7 +1101,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // per expert.  The rows of an expert come in no fixed order; no result depends
 // on it, since a row's products are its own and the weighted sum goes by
 // route_pos.  Also zeroes the tile kernel's counters.
-__global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restrict__ idx, int routes, int top_k,
+__global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *idx, int routes, int top_k,
                                                                 int experts, int32_t *__restrict__ offsets,
                                                                 int32_t *__restrict__ row_token,
                                                                 int32_t *__restrict__ route_pos,
@@ -1174,7 +1174,7 @@ __global__ void __launch_bounds__(1024) fp8_plan_kernel(const int64_t *__restric
 // whatever wrote the weights were complete when the tile kernel let this one
 // start.
 template <class Y>
-__global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *__restrict__ y, const int32_t *route_pos,
+__global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *y, const int32_t *route_pos,
                                                           const uint16_t *weights, const int32_t *gave_up, int tokens,
                                                           int top_k, int hidden, uint16_t *__restrict__ out) {
     constexpr int kU = 8, kCols = 16 / sizeof(Y);
@@ -1206,7 +1206,7 @@ __global__ void __launch_bounds__(128) fp8_combine_kernel(const Y *__restrict__ 
         uint4 v[kU];
 #pragma unroll
         for (int k = 0; k < kU; ++k)
-            v[k] = pos[k] >= 0 ? ld_stream(y + static_cast<int64_t>(pos[k]) * hidden + c) : make_uint4(0, 0, 0, 0);
+            v[k] = pos[k] >= 0 ? fp8::ld_once(y + static_cast<int64_t>(pos[k]) * hidden + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < kU; ++k) {
             if (pos[k] < 0) continue;  // a weight of a dropped route may be anything

@@ -185,3 +185,45 @@ def test_block_made_in_inference_mode_and_called_outside_it(dev):  # noqa: F811
         with torch.inference_mode():
             third = layer(x)
     assert not torch.equal(first, second) and torch.equal(second, fresh()) and torch.equal(third, second)
+
+
+# --------------------------------------------------- kernels that overlap ---
+
+@pytest.mark.parametrize("tokens", [2, 5, 64, 300])
+def test_each_kernel_reads_what_the_one_before_wrote(dev, tokens):  # noqa: F811
+    """Rows and weights quantised into the same memory again and again, right
+    before the products that read them, and route ids written right before the
+    experts: every call sees its own inputs."""
+    g = gen(tokens, dev)
+    rows = [randn(g, tokens, 1024).to(torch.bfloat16) for _ in range(5)]
+    mats = [(0.05 * randn(g, 512, 1024)).to(torch.bfloat16) for _ in range(5)]
+    norms = [randn(g, 1024).to(torch.bfloat16) for _ in range(5)]
+    banks = [((0.05 * randn(g, 4, 256, 1024)).to(torch.bfloat16), (0.05 * randn(g, 4, 1024, 128)).to(torch.bfloat16))
+             for _ in range(5)]
+    routers = [randn(g, 4, 1024).to(torch.bfloat16) for _ in range(5)]
+
+    def step(k, q, s, w, gu, dn, norm, wait):
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        norm.copy_(norms[k])
+        pause()
+        fp8.rmsnorm_quantize(rows[k], norm, out=(q, s, None, None))
+        pause()
+        fp8.quantize_blocks(mats[k], out=w)
+        pause()
+        a = fp8.linear(q, s, *w)
+        pause()
+        idx, _, scores, _, _ = native.router_topk(rows[k], routers[k], top_k=2)
+        pause()
+        fp8.quantize_blocks(banks[k][0], out=gu)
+        pause()
+        fp8.quantize_blocks(banks[k][1], out=dn)
+        pause()
+        return a, fp8.experts(q, s, *gu, *dn, idx, scores), fp8.quantize_rows(a)[0]
+
+    memory = (*fp8.quantize_rows(rows[0]), fp8.quantize_blocks(mats[0]), *map(fp8.quantize_blocks, banks[0]),
+              norms[0].clone())
+    want = [step(k, *memory, True) for k in range(5)]
+    got = [step(k % 5, *memory, False) for k in range(20)]
+    torch.cuda.synchronize()
+    for k, outs in enumerate(got):
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(outs, want[k % 5])), k

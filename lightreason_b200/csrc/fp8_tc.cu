@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (warp == 0) {
             // ---------------------------------------------- items, weight tiles
+            sm100::fence_proxy_async_global();  // the weights may have been written by the kernel before
             const uint64_t once = sm100::l2_evict_first_policy(), keep = sm100::l2_evict_normal_policy();
             const uint32_t one = sm100::elect_one();
             bool ok = true;

@@ -8,6 +8,7 @@
 // current stream.  It returns the result; None where a check fails, for
 // fp8.py to find the fault and name it; or the status of a failed call.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -31,15 +32,19 @@ int64_t groups(int64_t n) { return (n + kGroup - 1) / kGroup; }
 // An argument as a tensor; null if it is None or something else.
 const at::Tensor *tensor(PyObject *o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-// A dense CUDA tensor of this type and shape on device `index` without a gradient to be tracked.
+// No gradient to be tracked and no forward-mode tangent to be carried on.
+bool plain(const at::Tensor &t) {
+    if (t.requires_grad() && c10::GradMode::is_enabled()) return false;
+    return !(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+}
+// A dense plain CUDA tensor of this type and shape on device `index`.
 bool fits(const at::Tensor *t, at::ScalarType type, at::IntArrayRef shape, int index) {
     return t && t->scalar_type() == type && t->is_cuda() && t->get_device() == index && t->sizes() == shape &&
-           t->is_contiguous() && !(t->requires_grad() && c10::GradMode::is_enabled());
+           t->is_contiguous() && plain(*t);
 }
 // BF16 rows [T, H], dense within a row.
 bool fits_rows(const at::Tensor *t, int64_t *stride) {
-    if (!t || t->scalar_type() != at::kBFloat16 || !t->is_cuda() || t->dim() != 2 ||
-        (t->requires_grad() && c10::GradMode::is_enabled()))
+    if (!t || t->scalar_type() != at::kBFloat16 || !t->is_cuda() || t->dim() != 2 || !plain(*t))
         return false;
     const int64_t tokens = t->size(0), hidden = t->size(1);
     if (hidden < 1 || (hidden > 1 && t->stride(1) != 1) || (tokens > 1 && t->stride(0) < hidden)) return false;
@@ -129,7 +134,7 @@ PyObject *blocks(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 3) return none();
     const at::Tensor *w = tensor(a[0]), *q = tensor(a[1]), *scales = tensor(a[2]);
     if (!w || w->scalar_type() != at::kBFloat16 || !w->is_cuda() || !(w->dim() == 2 || w->dim() == 3) ||
-        !w->is_contiguous() || (w->requires_grad() && c10::GradMode::is_enabled()))
+        !w->is_contiguous() || !plain(*w))
         return none();
     const int index = w->get_device();
     const int64_t banks = w->dim() == 3 ? w->size(0) : 1, nr = w->size(-2), nc = w->size(-1);

@@ -27,6 +27,7 @@ import weakref
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from lightreason_b200 import build, native
 from lightreason_b200.native import _require
@@ -76,6 +77,8 @@ def _refused(name: str, status) -> None:
 
 
 def _no_grad(*tensors) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the FP8 operators have no forward-mode derivative: a tensor carries a tangent")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the FP8 operators have no gradient: call them under torch.no_grad() or "
                            "torch.inference_mode()")

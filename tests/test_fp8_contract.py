@@ -135,3 +135,14 @@ def test_experts_workspace_does_for_fewer_tokens(so, experts, top_k, hidden, inn
         rc = so.moe_experts_fp8(P, P, P, P, P, P, P, P, t, experts, top_k, hidden, inner, P, P, 0, None, None)
         asked = re.search(rb"workspace of (\d+) bytes", so.moe_last_error())
         assert rc == native.MOE_EINVAL and 0 < int(asked[1]) <= need(t) <= sizes[-1], t
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.ones(4)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+            fp8._no_grad(None, x, dual)
+        fp8._no_grad(None, x, fwd.unpack_dual(dual).primal)

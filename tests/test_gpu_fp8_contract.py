@@ -187,6 +187,28 @@ def test_block_made_in_inference_mode_and_called_outside_it(dev):  # noqa: F811
     assert not torch.equal(first, second) and torch.equal(second, fresh()) and torch.equal(third, second)
 
 
+# ----------------------------------------------------- forward-mode tangents ---
+
+def test_forward_mode_tangents_are_refused(dev):  # noqa: F811
+    """A tensor that carries a tangent is refused instead of losing it."""
+    import torch.autograd.forward_ad as fwd
+
+    x, xs, gu, gus, dn, dns, idx, wt = experts_case(dev, 3, 4, 2, 256, 128)
+    b, w = torch.ones(3, 256, dtype=torch.bfloat16, device=dev), torch.ones(256, dtype=torch.bfloat16, device=dev)
+    with torch.no_grad(), fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t.clone(), torch.ones_like(t))  # noqa: E731
+        for call in (lambda: fp8.quantize_rows(dual(b)), lambda: fp8.quantize_blocks(dual(b)),
+                     lambda: fp8.rmsnorm_quantize(dual(b), w), lambda: fp8.rmsnorm_quantize(b, dual(w)),
+                     lambda: fp8.rmsnorm_quantize(b, w, dual(b)), lambda: fp8.linear(x, dual(xs), gu[0], gus[0]),
+                     lambda: fp8.linear(x, xs, gu[0], dual(gus[0])),
+                     lambda: fp8.experts(x, xs, gu, gus, dn, dns, idx, dual(wt)),
+                     lambda: fp8.experts(x, dual(xs), gu, gus, dn, dns, idx, wt)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        q, s = fp8.quantize_rows(fwd.unpack_dual(dual(b)).primal)  # the values alone are taken
+    assert q.shape == (3, 256) and torch.equal(s, fp8.quantize_rows(b)[1])
+
+
 # --------------------------------------------------- kernels that overlap ---
 
 @pytest.mark.parametrize("tokens", [2, 5, 64, 300])

@@ -16,7 +16,7 @@
 //  * BN = 0, rows as M: tiles of 128 rows against N = 256 weight rows.  An
 //    accumulator lane is one row, so a group's factor is one number per thread,
 //    gate and up of a column meet in one thread, and warps without rows of a
-//    partial tile skip.  A plain product of more than 128 rows runs them on CTA
+//    partial tile skip.  Large plain products run them on CTA
 //    pairs (PAIR): each CTA holds 128 of an item's 256 rows and 128 of its
 //    weight rows, multiplied by tcgen05.mma.cta_group::2 (M = 256), a third less
 //    to load for the same work.  The first CTA issues the products; both CTAs'
@@ -1357,11 +1357,20 @@ LinearFp8Plan plan_linear_fp8(int tokens, int rows, int cols) {
                                          cols / 2048.0 * (0.5 + 0.45 * tokens));
         best.gemv = us < least;
     }
-    // Pairs wherever a pair has more than one tile of rows: the cycles are the
-    // same, the power is not (8192 rows of 2048 against 4096, in a run of
-    // seconds at 1000 W: 90.6 us without, 87.3 with; of 8192 against 8192: 686 and
-    // 659; in short runs 75.6 and 73.4; 300 to 512 rows: alike).
-    best.pair = !best.gemv && best.tile == kBM && best.split == 1 && tokens > kBM && grouped_pair_clusters() > 0;
+    // Pairs where they need no more rounds than single CTAs (an odd number of
+    // row tiles leaves half a pair idle: 1152 rows of 4096 against 4096 are one
+    // round of 144 tiles in 22.1 us, and two of 80 pairs in 37.6; 3456 of 2048 three
+    // in 32.0 and four in 39.9) and each CTA has at least 64 groups to go through.
+    // The cycles of a group are the same, the power and the traffic are not
+    // (8192 rows of 2048 against 4096: 75.6 us single, 72.5 in pairs, 90.6 and 87.3
+    // in a run of seconds at 1000 W; 8192 of 8192 against 8192: 686 and 659), but a
+    // pair takes 0.4 to 0.8 us longer to start and end (512 rows of 512 against
+    // 9216: 7.1 single, 7.9 in pairs; from 64 groups on 0.95 to 1.016 of single).
+    if (!best.gemv && best.tile == kBM && best.split == 1 && tokens > kBM && grouped_pair_clusters() > 0) {
+        const double single = std::ceil(nt * std::ceil(tokens / (1.0 * kBM)) / sm_count());
+        const double paired = std::ceil(nt * std::ceil(tokens / (2.0 * kBM)) / grouped_pair_clusters());
+        best.pair = paired <= single && paired * kbs >= 64;
+    }
     return best;
 }
 

@@ -112,6 +112,53 @@ def test_experts_that_give_up_half_way(dev, tokens, count, top_k, hidden, inner)
     within(fp8.experts(*c), want, bound, "afterwards")
 
 
+@pytest.mark.parametrize("tokens,rows,cols", PAIR_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_pairs(dev, tokens, rows, cols, dtype):  # noqa: F811
+    """Values of CTA pairs; nothing beyond the output; a row with NaN by itself."""
+    x, xs, w, ws = linear_case(dev, tokens, rows, cols)
+    pad = 16
+    store = torch.full((tokens * rows + 2 * pad,), 7.0, dtype=dtype, device=dev)
+    out = store[pad:-pad].view(tokens, rows)
+    fp8.linear(x, xs, w, ws, out=out)
+    want, bound = R.linear(x, xs, w, ws)
+    within(out, want, bound + (R.F32 * want.abs() if dtype is torch.float32 else R.BF * (want.abs() + bound)), "out")
+    assert store[:pad].eq(7).all() and store[-pad:].eq(7).all()
+    xs2 = xs.clone()
+    xs2[tokens - 1, 1] = float("nan")
+    got = fp8.linear(x, xs2, w, ws, out_dtype=dtype)
+    assert got[-1].isnan().all() and torch.equal(got[:-1], out[:-1])
+
+
+def time_of(call, calls=10):
+    """Least device time of a call in microseconds, over replays of a graph of ten."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(calls):
+            call()
+    times = []
+    for _ in range(25):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3 / calls)
+    return min(times)
+
+
+def test_linear_pairs_cost_no_round(dev):  # noqa: F811
+    """Nine tiles of 128 rows take as long as eight where both fit one round
+    of the SMs; as pairs the nine would need two (1.7 times as long)."""
+    times = []
+    for tokens in (1024, 1152):
+        c = linear_case(dev, tokens, 4096, 4096)
+        out = torch.empty(tokens, 4096, dtype=torch.bfloat16, device=dev)
+        times.append(time_of(lambda: fp8.linear(*c, out=out)))  # noqa: B023
+    assert times[1] < 1.35 * times[0], times
+
+
 def test_linear_pairs_back_to_back(dev):  # noqa: F811
     """Pairs right behind other pairs and single CTAs on the same SMs, on both
     dtypes: the same values every time, no wait gives up."""

@@ -48,7 +48,8 @@ def _bind():
     """The module, with the C ABI's addresses in the loaded library."""
     path = str(build.BIND)
     if not build.BIND.exists():
-        raise RuntimeError(f"{path} is missing: build it with `python -m lightreason_b200.build`")
+        raise RuntimeError(f"{path} is missing: build it with `python -m lightreason_b200.build` (it needs a host "
+                           "C++ compiler and the headers of Python and of this torch)")
     spec = importlib.util.spec_from_file_location("_fp8_bind", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)

@@ -146,3 +146,38 @@ def test_tangents_are_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
             fp8._no_grad(None, x, dual)
         fp8._no_grad(None, x, fwd.unpack_dual(dual).primal)
+
+
+# ---------------------------------------------------------------- the build ---
+
+@pytest.fixture
+def scratch(monkeypatch, tmp_path):
+    """A build of one source file into a folder of its own."""
+    monkeypatch.setattr(build, "OUT_DIR", tmp_path)
+    monkeypatch.setattr(build, "LIB", tmp_path / build.LIB.name)
+    monkeypatch.setattr(build, "BIND", tmp_path / build.BIND.name)
+    monkeypatch.setattr(build, "SOURCES", ["host.cu"])
+    return tmp_path
+
+
+@pytest.mark.parametrize("compiler", ["false", "/nowhere/c++"])
+def test_the_library_is_built_where_the_python_module_cannot_be(scratch, monkeypatch, capfd, compiler):
+    """Without a host compiler (or headers), the C library is there and the FP8
+    entry points of Python say what is missing."""
+    monkeypatch.setenv("CXX", compiler)
+    assert build.build() == scratch / "libmoe_b200.so" and build.LIB.exists() and not build.BIND.exists()
+    assert "not built" in capfd.readouterr().err
+    ctypes.CDLL(str(build.LIB)).moe_version()
+    with pytest.raises(RuntimeError, match="missing: build it"):
+        fp8._bind.__wrapped__()
+
+
+def test_the_python_module_belongs_to_one_torch(scratch):
+    """A module built against another torch is not this one's."""
+    assert torch.__version__ in build.BIND.name
+    build.LIB.touch()
+    other = scratch / build.BIND.name.replace(torch.__version__, "1.0.0")
+    other.touch()
+    assert build._bind_stale() and not build._lib_stale()
+    build.BIND.touch()
+    assert not build._bind_stale()

@@ -2,8 +2,6 @@
 // rows), every lane a 16-byte piece of it, FP32 FMA over the e4m3 values
 // (widened to FP16, whose products an FP32 FMA takes exactly).  The rows are the traffic: they are streamed once with all of a
 // row's loads in flight, and the few activations come from L1 and L2.
-#include <algorithm>
-
 #include "fp8_kernels.cuh"
 
 namespace lrb {
@@ -19,7 +17,7 @@ constexpr int kWarps = 8;
 constexpr int kChunk = 32 * 16;  // weight bytes a warp reads per load
 constexpr int kUnroll = 4;       // loads of a row in flight
 
-// A warp per output row, MT tokens at a time.
+// A warp per output row, for up to MT tokens.
 template <int MT>
 __global__ void __launch_bounds__(kWarps * 32) linear_gemv_kernel(LinearFp8 a) {
     const int lane = threadIdx.x & 31;
@@ -34,39 +32,37 @@ __global__ void __launch_bounds__(kWarps * 32) linear_gemv_kernel(LinearFp8 a) {
     grid_dependency_trigger();
     if (!live) return;
     const float *ws = a.w_scales + static_cast<int64_t>(n / kGroup) * gk;
-    for (int m0 = blockIdx.y * MT; m0 < a.tokens; m0 += gridDim.y * MT) {
-        float acc[MT];
+    float acc[MT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = 0.f;
-        for (int c0 = lane * 16; c0 < a.cols; c0 += kUnroll * kChunk) {
-            uint4 v[kUnroll];
+    for (int m = 0; m < MT; ++m) acc[m] = 0.f;
+    for (int c0 = lane * 16; c0 < a.cols; c0 += kUnroll * kChunk) {
+        uint4 v[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int c = c0 + u * kChunk;
-                v[u] = c < a.cols ? ld_again(w + c) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int c = c0 + u * kChunk;
-                if (c >= a.cols) break;
-                const float s = ws[c / kGroup];
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int t = min(m0 + m, a.tokens - 1);
-                    uint16_t x[16];
-                    halves16(ld_again(a.x + static_cast<int64_t>(t) * a.cols + c), x);
-                    acc[m] = fmaf(dot16(v[u], x), s * a.x_scales[static_cast<int64_t>(t) * gk + c / kGroup], acc[m]);
-                }
-            }
+        for (int u = 0; u < kUnroll; ++u) {
+            const int c = c0 + u * kChunk;
+            v[u] = c < a.cols ? ld_again(w + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const float r = warp_sum(acc[m]);
-            if (lane == 0 && m0 + m < a.tokens) {
-                const int64_t at = static_cast<int64_t>(m0 + m) * a.rows + n;
-                if (a.out_f32) static_cast<float *>(a.out)[at] = r;
-                else static_cast<uint16_t *>(a.out)[at] = f2bf(r);
+        for (int u = 0; u < kUnroll; ++u) {
+            const int c = c0 + u * kChunk;
+            if (c >= a.cols) break;
+            const float s = ws[c / kGroup];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int t = min(m, a.tokens - 1);
+                uint16_t x[16];
+                halves16(ld_again(a.x + static_cast<int64_t>(t) * a.cols + c), x);
+                acc[m] = fmaf(dot16(v[u], x), s * a.x_scales[static_cast<int64_t>(t) * gk + c / kGroup], acc[m]);
             }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const float r = warp_sum(acc[m]);
+        if (lane == 0 && m < a.tokens) {
+            const int64_t at = static_cast<int64_t>(m) * a.rows + n;
+            if (a.out_f32) static_cast<float *>(a.out)[at] = r;
+            else static_cast<uint16_t *>(a.out)[at] = f2bf(r);
         }
     }
 }
@@ -229,8 +225,7 @@ __global__ void __launch_bounds__(kWarps * 32) down_gemv_kernel(ExpertsFp8 a, co
 }  // namespace
 
 int launch_linear_fp8_gemv(const LinearFp8 &a, cudaStream_t stream) {
-    const int passes = (a.tokens + kGemvTokens - 1) / kGemvTokens;
-    const dim3 grid((a.rows + kWarps - 1) / kWarps, std::min(passes, 16384)), block(kWarps * 32);
+    const dim3 grid((a.rows + kWarps - 1) / kWarps), block(kWarps * 32);
     if (a.tokens == 1)
         return launch_pdl(linear_gemv_kernel<1>, grid, block, 0, stream, "linear_gemv_kernel", a);
     if (a.tokens == 2)

@@ -29,11 +29,12 @@ struct ExpertsFp8 {
     uint16_t *out;                    // [T, H] BF16
 };
 
-constexpr int kGemvTokens = 4;   // tokens per pass of the linear GEMV
+constexpr int kGemvTokens = 4;   // tokens that the linear GEMV takes
 // Routes up to which the experts take the GEMV kernels, whose weights are read
 // once per route (2048 x 512 experts, top-8, us at 1 / 2 / 3 tokens: GEMV 22.7 /
 // 36.9 / 49.0, tiles 28.7 / 34.7 / 36.9).
 constexpr int kGemvRoutes = 12;
+// up to kGemvTokens tokens
 int launch_linear_fp8_gemv(const LinearFp8 &a, cudaStream_t stream);
 // h: FP32 [T * K, I] scratch
 int launch_experts_fp8_gemv(const ExpertsFp8 &a, float *h, cudaStream_t stream);

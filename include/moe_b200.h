@@ -526,6 +526,8 @@ int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, int cols, ui
 /* out[T, rows] (BF16, or FP32 with out_f32 = 1) = x . w^T on the values that x
  * [T, cols] and w [rows, cols] stand for, products summed in FP32.  cols must
  * be a multiple of 16; x, w and out are 16-byte aligned; no size is above 2^30.
+ * The same call gives the same bits; the order of a row's sums goes by the number
+ * of rows.
  * status (device int32, or NULL) is set to 1 if a bounded wait inside a kernel
  * gave up; out then holds NaN (a linear: in the tiles concerned). */
 int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uint8_t *w, const float *w_scales, int tokens,
@@ -544,7 +546,9 @@ uint64_t moe_fp8_wait_limit(uint64_t ns);
  *   h = silu(gate . x_t) * (up . x_t)  in FP32, brought to e4m3 per 128 values
  *   out[t] += weights[t, k] * (down . h)
  * with FP32 sums and one rounding to BF16 at the end; batches of more than 2048
- * routes keep each route's row as BF16 before the weighted sum.  Ids
+ * routes keep each route's row as BF16 before the weighted sum.  The order of the
+ * sums goes by the batch (as in moe_linear_fp8): a row's last bits may differ
+ * between batches, not between calls.  Ids
  * outside [0, E) contribute nothing (a token with none left is 0).  hidden is
  * a multiple of 16, inner of 128, top_k at most 32, experts at most 1024.
  * status as in moe_linear_fp8.  The workspace of a number of tokens also does for

@@ -296,3 +296,76 @@ def test_each_kernel_reads_what_the_one_before_wrote(dev, tokens):  # noqa: F811
     torch.cuda.synchronize()
     for k, outs in enumerate(got):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(outs, want[k % 5])), k
+
+
+# ------------------------------------------------ across a product's borders ---
+
+def whole_experts_case(dev, tokens, count, top_k, seed=0):  # noqa: F811
+    """Values whose gate and up sums are whole numbers below 2^13 times 2^-5, so
+    that FP32 (and any tensor core's sum) has them exactly; H 256, I 128."""
+    g = gen(seed + tokens, dev)
+    ints = lambda top, *s: torch.randint(-top, top + 1, s, generator=g, device=dev).float()  # noqa: E731
+    x, gu, dn = (v.to(torch.float8_e4m3fn) for v in (ints(2, tokens, 256), ints(3, count, 256, 256), ints(7, count, 256, 128)))
+    xs, gus, dns = (torch.full(s, v, device=dev) for s, v in (((tokens, 2), 1.0), ((count, 2, 2), 2.0 ** -5), ((count, 2, 1), 0.5)))
+    idx = torch.rand(tokens, count, generator=g, device=dev).topk(top_k, -1)[1]
+    return x, xs, gu, gus, dn, dns, idx.contiguous(), torch.softmax(randn(g, tokens, top_k), -1).to(torch.bfloat16)
+
+
+def whole_experts(x, xs, gu, gus, dn, dns, idx, weights):
+    """(exact, bound, sum over the routes of weight times |row|) for such values.
+    gate and up are exact; SiLU is off by 2^-23 (4.5 + 1.2 |gate|) of itself (the
+    documented errors of the fast exponential and quotient, and a rounding), the
+    product and the scale by two more roundings; a value of h that this may carry
+    over a border moves by a step.  The down sums as in fp8_reference, the
+    weighted sum k roundings, BF16 at the end."""
+    out = torch.zeros(x.shape[0], dn.shape[1], dtype=torch.float64, device=x.device)
+    bound, size = torch.zeros_like(out), torch.zeros_like(out)
+    xd = R.widen_rows(x, xs)
+    for e in range(gu.shape[0]):
+        token, slot = torch.nonzero(idx == e, as_tuple=True)
+        p = xd[token] @ R.widen_blocks(gu[e], gus[e]).T
+        gate, up = p[:, :128], p[:, 128:]
+        h = gate * torch.sigmoid(gate) * up
+        off = 2 * R.F32 * (4.5 + 1.2 * gate.abs()) + 2 * R.F32
+        v, q, s = R.rows(h)
+        far = 2 * off.amax(-1, keepdim=True) + 4 * R.F32       # of v: its own error and its group's maximum's
+        near = ((v / R.step(v) - torch.floor(v / R.step(v)) - 0.5).abs() * R.step(v)) <= far * v.abs()
+        qb = torch.where(near, R.step(v), torch.zeros_like(v))
+        wd = R.widen_blocks(dn[e], dns[e])
+        y = (q * s) @ wd.T
+        yb = (qb * s) @ wd.abs().T + (R.chain(128) * R.F32 + far) * ((q * s).abs() @ wd.abs().T)
+        wt = weights[token, slot].double()[:, None]
+        out.index_add_(0, token, y * wt)
+        bound.index_add_(0, token, (yb + idx.shape[1] * R.F32 * y.abs()) * wt)
+        size.index_add_(0, token, y.abs() * wt)
+    return out, bound + R.BF * (out.abs() + bound), size
+
+
+@pytest.mark.parametrize("tokens,count,top_k", [(1, 8, 8), (3, 6, 4), (2, 9, 7), (20, 8, 8), (100, 64, 8), (256, 8, 8), (128, 20, 16)])
+def test_experts_up_to_2048_routes_keep_rows_in_fp32(dev, tokens, count, top_k):  # noqa: F811
+    """GEMV and tiles of every kind up to 2048 routes: one rounding to BF16, at
+    the end (rounding each route's row too would leave the bound)."""
+    c = whole_experts_case(dev, tokens, count, top_k)
+    want, bound, _ = whole_experts(*c)
+    within(fp8.experts(*c), want, bound, "out")
+
+
+def test_experts_above_2048_routes_round_their_rows(dev):  # noqa: F811
+    """The 2049th route brings the rounding of each route's row to BF16, for
+    every token of the batch; without it the values of 2048 routes."""
+    c = whole_experts_case(dev, 257, 8, 8)
+    want, bound, size = whole_experts(*c)
+    within(fp8.experts(*c), want, bound + 1.01 * R.BF * size, "out")
+    first = [t[:256] if t.shape[0] == 257 else t for t in c]
+    within(fp8.experts(*first), want[:256], bound[:256], "256 tokens")
+
+
+def test_linear_rows_in_batches_of_every_size(dev):  # noqa: F811
+    """One row in batches that take other kernels, tiles and splits: its bits may
+    differ, each is within the bound of a sum in FP32."""
+    for rows, cols in ((1024, 2048), (300, 4112), (9216, 512)):
+        x, xs, w, ws = linear_case(dev, 600, rows, cols)
+        want, bound = R.linear(x, xs, w, ws)
+        for tokens in (1, 2, 4, 5, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 600):
+            got = fp8.linear(x[:tokens], xs[:tokens], w, ws, out_dtype=torch.float32)
+            within(got, want[:tokens], (bound + R.F32 * want.abs())[:tokens], f"{tokens} rows of {cols}")

@@ -22,14 +22,15 @@
 //    to load for the same work.  The first CTA issues the products; both CTAs'
 //    loads complete on its barriers, its commits arrive on both CTAs', and all
 //    sixteen epilogue warps hand its buffers back.
-//  * BN = 16, 32 (64 for a plain product), weights as M: the two blocks of 128 weight rows against
-//    N = BN rows.  A lane is one weight row and the tile's few rows are its
-//    columns: at a few rows per expert all eight warps share the epilogue
+//  * BN = 16, 32 (64 for a plain product), weights as M: the two blocks of 128
+//    weight rows against N = BN rows.  A lane is one weight row and the tile's few
+//    rows are its columns: at a few rows per expert all eight warps share the epilogue
 //    instead of one row's pair of warps doing it.
-// A stage is one group: the 256 weight rows (32 KB, two boxes) and the tile's
-// rows (gathered by TMA from the token rows for gate/up; boxes of 16 when the
-// tile is partial).  Three to six stages keep 96 to 192 KB of weights in flight
-// per SM, which is what streams the banks at small and middle widths.
+// A stage is one group: the 256 weight rows (32 KB, two boxes; a pair's CTA 128
+// rows, 16 KB, one box) and the tile's rows (gathered by TMA from the token rows
+// for gate/up; boxes of 16 when the tile is partial).  Three to six stages keep 96
+// to 192 KB of weights in flight per SM, which is what streams the banks at small
+// and middle widths (a pair's four stages 64 KB: there the products bound).
 //
 // The experts are one launch: gate/up items, then down items, fetched in order
 // from a counter.  A down item's weights are requested at once, its rows when
@@ -43,9 +44,11 @@
 // Warps: 0 items and weight tiles, 1 MMA, 2 and 3 row tiles and scales (four
 // groups at a time, up to four such requests in flight), 4-11 epilogue; the
 // first four hand registers to the others (72 and 216, the experts' 104 and
-// 200, a thread of 168 at launch: 64,512 a CTA either way).  Every wait is bounded; a timeout raises
-// *status, drains what is in flight and returns, and leaves NaN: in a linear's
-// tiles of that CTA or pair, in all of an experts call's output.
+// 200, a thread of 168 at launch: 64,512 a CTA either way).  Every wait for loads,
+// products, rows or items is bounded (the barriers of a CTA or cluster are not: all
+// their warps come to them, having given up or not); a timeout raises *status,
+// drains what is in flight and returns, and leaves NaN: in a linear's tiles of that
+// CTA or pair, in all of an experts call's output.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -225,8 +228,11 @@ __device__ __forceinline__ void store_rows64(uint8_t *buf, const uint32_t (&v)[1
     }
 }
 
-// x / (1 + exp(-x)) from the fast exponential and quotient: off by 2^-24 times
-// (4 + 1.2 |x|) of the value at most, below what the FP32 sums behind x leave.
+// x / (1 + exp(-x)) from the fast exponential and quotient: off by 2^-23 times
+// (4.5 + 1.2 |x|) of the value at most (their documented 2 + 1.2 |x| and 2 units in
+// the last place and the sum's rounding), below what the FP32 sums behind x leave;
+// below x = -87.3, where the divisor passes 2^126, it is 0 for a value of 2^-119
+// at most.
 __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 
 // A warp's 32 rows of 256 bytes (128 BF16 columns), one row a lane, staged for

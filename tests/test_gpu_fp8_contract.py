@@ -369,3 +369,40 @@ def test_linear_rows_in_batches_of_every_size(dev):  # noqa: F811
         for tokens in (1, 2, 4, 5, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 600):
             got = fp8.linear(x[:tokens], xs[:tokens], w, ws, out_dtype=torch.float32)
             within(got, want[:tokens], (bound + R.F32 * want.abs())[:tokens], f"{tokens} rows of {cols}")
+
+
+# ----------------------------------------------------------- largest widths ---
+
+@pytest.mark.parametrize("tokens,count,top_k,hidden,inner", [(1, 2, 2, 16, 16384), (40, 2, 1, 16, 16384), (300, 2, 1, 16, 16384),
+                                                             (2, 2, 2, 65536, 128), (40, 2, 1, 65536, 128),
+                                                             (300, 2, 1, 65536, 128)])
+def test_experts_at_the_widest(dev, tokens, count, top_k, hidden, inner):  # noqa: F811
+    c = experts_case(dev, tokens, count, top_k, hidden, inner)
+    want, bound = R.experts(*c)
+    within(fp8.experts(*c), want, bound, "out")
+
+
+@pytest.mark.parametrize("tokens,rows,cols", [(1, 3, 1 << 20), (4, 130, 1 << 19), (5, 3, 1 << 20), (40, 130, 1 << 18),
+                                              (300, 257, 1 << 17)])
+def test_linear_at_long_rows(dev, tokens, rows, cols):  # noqa: F811
+    x, xs, w, ws = linear_case(dev, tokens, rows, cols)
+    want, bound = R.linear(x, xs, w, ws)
+    within(fp8.linear(x, xs, w, ws, out_dtype=torch.float32), want, bound + R.F32 * want.abs(), "f32")
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_rows_at_the_widest(dev, tokens):  # noqa: F811
+    """2^20 values a row: e4m3 exact; the norm within the longest chain of its
+    sum (2^20 / 256 terms a thread, halved by the root, and eight roundings)."""
+    g = gen(tokens, dev)
+    x = randn(g, tokens, 1 << 20).to(torch.bfloat16)
+    q, s = fp8.quantize_rows(x)
+    _, want, scale = R.rows(x.double())
+    assert torch.equal(q.double(), want) and torch.equal(s, scale.float())
+    w = (0.5 * randn(g, 1 << 20)).to(torch.bfloat16)
+    _, s, normed, _ = fp8.rmsnorm_quantize(x, w)
+    xd = x.double()
+    y = xd * torch.rsqrt(xd.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+    rel = (4096 + 16) * R.F32
+    within(normed, y, (R.BF + rel) * y.abs() + 2.0 ** -134, "normed")
+    within(s, R.tops(y) / R.TOP, rel * R.tops(y) / R.TOP, "scales")

@@ -147,8 +147,7 @@ class ExpertPool:
         if banks is not None:
             if banks.holds(layer.gate_up, layer.down, *shared, *extra):
                 return banks
-            if (banks.experts, banks.hidden, banks.inner) == (
-                    layer.module.num_experts, layer.module.hidden_dim, layer.module.intermediate_dim):
+            if banks.takes(layer.gate_up, layer.down, shared, extra):
                 banks.load(layer.gate_up, layer.down, shared=shared, extra=extra)
                 return banks
             self.stats.resident_bytes -= banks.nbytes()  # another module's, gone, under the same id

@@ -258,16 +258,20 @@ class ExpertBanks:
             self.extra = tuple(torch.empty(t.shape, dtype=t.dtype, device=self.device) for t in extra)
         self.load(gate_up, down, shared=shared, extra=extra)
 
+    def takes(self, gate_up: torch.Tensor, down: torch.Tensor, shared=(), extra=()) -> bool:
+        """Whether load() has room for these (a shared expert or none, as when the banks were made)."""
+        count, hidden, inner = self.experts, self.hidden, self.inner
+        return (tuple(gate_up.shape) == (count, 2 * inner, hidden) and tuple(down.shape) == (count, hidden, inner)
+                and self.gate_up.shape[0] == count + bool(shared)
+                and [(t.shape, t.dtype) for t in extra] == [(t.shape, t.dtype) for t in self.extra])
+
     def load(self, gate_up: torch.Tensor, down: torch.Tensor, *, shared=(), extra=()) -> None:
         """Brings these weights into the banks' memory, where captured graphs
         that read it find them too."""
         _require(not (self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()),
                  "FP8 banks cannot be made during a graph capture: call the layer once before it")
         count, hidden, inner = self.experts, self.hidden, self.inner
-        _require(tuple(gate_up.shape) == (count, 2 * inner, hidden) and tuple(down.shape) == (count, hidden, inner)
-                 and self.gate_up.shape[0] == count + bool(shared)
-                 and [t.shape for t in extra] == [t.shape for t in self.extra],
-                 "the weights do not have the banks' shapes")
+        _require(self.takes(gate_up, down, shared, extra), "the weights do not have the banks' shapes")
         _require(not shared or [tuple(t.shape) for t in shared] == [(inner, hidden)] * 2 + [(hidden, inner)],
                  "the shared expert must have the experts' widths")
         self._sources = []  # held only once all of them are there

@@ -148,6 +148,27 @@ def test_tangents_are_refused():
         fp8._no_grad(None, x, fwd.unpack_dual(dual).primal)
 
 
+def test_banks_of_another_kind_under_the_same_key_are_made_anew(quantised):
+    """A key is a module's id, which a later module may get: experts alone where
+    a block was, a block where experts were, another number of experts."""
+    from lightreason_b200 import expert_stream
+
+    pool = expert_stream.ExpertPool("cuda:0")
+    pool.device = torch.device("cpu")
+    gu, dn, shared, router = bank_weights()
+    module = SimpleNamespace(num_experts=20, hidden_dim=64, intermediate_dim=128)
+    layer = lambda a, b: SimpleNamespace(module=module, residency="b200-fp8", gate_up=a, down=b)  # noqa: E731
+    alone = pool._fp8_banks(layer(gu, dn))
+    assert pool._fp8_banks(layer(gu, dn)) is alone and pool.stats.resident_bytes == alone.nbytes()
+    pool.replay_graphs = {(id(module), "b200-fp8", 1, 8): "captured"}
+    block = pool._fp8_banks(layer(gu, dn), shared=tuple(shared), extra=(router,))
+    assert block is not alone and block.holds(gu, dn, *shared, router) and pool.replay_graphs == {}
+    assert pool._fp8_banks(layer(gu * 2, dn), shared=tuple(shared), extra=(router,)) is block
+    module.num_experts = 8
+    fewer = pool._fp8_banks(layer(gu[:8].clone(), dn[:8].clone()))
+    assert fewer.experts == 8 and pool.stats.resident_bytes == fewer.nbytes()
+
+
 # ---------------------------------------------------------------- the build ---
 
 @pytest.fixture

@@ -496,7 +496,7 @@ int moe_ep_p2p_finish(const moe_ep_p2p *p, void *stream);
  *   a = max(max |v_i|, 1e-10),  q_i = e4m3(v_i * 448 / a),  scale = a / 448
  * and read back as q_i * scale.  A group that holds a NaN or an infinity is
  * NaN throughout, and so is what is computed from it; other rows are not
- * touched by it.
+ * touched by it.  Every pointer is aligned to its elements at least.
  *
  * The reference keeps its experts in BF16 (edge35b/expert_stream.py:356); these
  * entry points stand beside the BF16 ones for weights that ship, or are

@@ -9,8 +9,6 @@ namespace {
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
 int check_experts(int tokens, int experts, int top_k, int hidden, int inner) {
     LRB_REQUIRE(tokens >= 0 && experts >= 1 && experts <= 1024, "moe_experts_fp8: bad tokens %d / experts %d", tokens,
                 experts);
@@ -71,8 +69,10 @@ extern "C" int moe_linear_fp8(const uint8_t *x, const float *x_scales, const uin
     LRB_REQUIRE(out_f32 == 0 || out_f32 == 1, "moe_linear_fp8: out_f32 must be 0 or 1");
     if (tokens == 0) return MOE_OK;
     LRB_REQUIRE(x && x_scales && w && w_scales && out, "moe_linear_fp8: null tensor");
-    LRB_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scales, 4) && aligned(w_scales, 4) && aligned(out, 16),
+    LRB_REQUIRE(on_boundary(x, 16) && on_boundary(w, 16) && on_boundary(out, 16),
                 "moe_linear_fp8: x, w and out must be 16-byte aligned");
+    LRB_REQUIRE(on_boundary(x_scales, 4) && on_boundary(w_scales, 4) && on_boundary(status, 4),
+                "moe_linear_fp8: scales and status must be 4-byte aligned");
     if (int rc = require_sm100()) return rc;
     const LinearFp8 a{x, x_scales, w, w_scales, tokens, rows, cols, out, out_f32};
     if (plan_linear_fp8(tokens, rows, cols).gemv) return launch_linear_fp8_gemv(a, as_stream(stream));
@@ -98,11 +98,13 @@ extern "C" int moe_experts_fp8(const uint8_t *x, const float *x_scales, const ui
     if (tokens == 0) return MOE_OK;
     LRB_REQUIRE(x && x_scales && gate_up && gate_up_scales && down && down_scales && idx && weights && out,
                 "moe_experts_fp8: null tensor");
-    LRB_REQUIRE(aligned(x, 16) && aligned(gate_up, 16) && aligned(down, 16) && aligned(x_scales, 4) &&
-                    aligned(gate_up_scales, 4) && aligned(down_scales, 4) && aligned(out, 16),
+    LRB_REQUIRE(on_boundary(x, 16) && on_boundary(gate_up, 16) && on_boundary(down, 16) && on_boundary(out, 16),
                 "moe_experts_fp8: x, the banks and out must be 16-byte aligned");
+    LRB_REQUIRE(on_boundary(x_scales, 4) && on_boundary(gate_up_scales, 4) && on_boundary(down_scales, 4) && on_boundary(idx, 8) &&
+                    on_boundary(weights, 2) && on_boundary(status, 4),
+                "moe_experts_fp8: scales, idx, weights and status must be aligned to their elements");
     const Layout l = layout(tokens, experts, top_k, hidden, inner);
-    LRB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes,
+    LRB_REQUIRE(workspace && on_boundary(workspace, 256) && workspace_bytes >= l.bytes,
                 "moe_experts_fp8: workspace of %zu bytes (256-byte aligned) required", l.bytes);
     if (int rc = require_sm100()) return rc;
     const ExpertsFp8 a{x, x_scales, gate_up, down, gate_up_scales, down_scales, idx, weights, tokens, experts, top_k,

@@ -6,6 +6,9 @@
 
 namespace lrb {
 
+// p on a boundary of `a` bytes (a power of two)
+inline bool on_boundary(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
 // out[m, n] = sum over 128-column groups of xs[m, g] * ws[n / 128, g] * (x . w over the group)
 struct LinearFp8 {
     const uint8_t *x;        // [tokens, cols] e4m3

@@ -6,8 +6,7 @@
 // (transformers modeling_qwen3_5_moe.py): r = bf16(x + residual),
 // y = r * rsqrt(mean(r^2) + eps) * (offset + weight), the sum of squares in
 // FP32; q and the scales are those of y before it is rounded to BF16.
-#include "fp8.cuh"
-#include "kernels.cuh"
+#include "fp8_kernels.cuh"
 
 namespace lrb {
 namespace {
@@ -204,7 +203,7 @@ int launch_rows(const RowArgs &a, cudaStream_t stream) {
                       "row_kernel", a);
 }
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned16(const void *p) { return on_boundary(p, 16); }
 
 template <bool NORM>
 int rows_for(const RowArgs &a, cudaStream_t stream) {
@@ -309,6 +308,9 @@ extern "C" int moe_rmsnorm_fp8(const uint16_t *x, int64_t x_stride, const uint16
     LRB_REQUIRE(tokens <= 1 || (x_stride >= hidden && (!residual || residual_stride >= hidden)),
                 "moe_rmsnorm_fp8: row strides below hidden");
     LRB_REQUIRE(tokens == 0 || (x && q && scales), "moe_rmsnorm_fp8: null tensor");
+    LRB_REQUIRE(lrb::on_boundary(x, 2) && lrb::on_boundary(residual, 2) && lrb::on_boundary(weight, 2) &&
+                    lrb::on_boundary(normed, 2) && lrb::on_boundary(residual_out, 2) && lrb::on_boundary(scales, 4),
+                "moe_rmsnorm_fp8: tensors must be aligned to their elements");
     LRB_REQUIRE(!weight || (eps >= 0.f && eps < 1.f), "moe_rmsnorm_fp8: eps outside [0, 1)");
     if (tokens == 0) return MOE_OK;
     if (int rc = lrb::require_sm100()) return rc;
@@ -324,6 +326,8 @@ extern "C" int moe_quantize_fp8_blocks(const uint16_t *w, int banks, int rows, i
     const int64_t blocks = static_cast<int64_t>(banks) * lrb::fp8::groups(rows) * lrb::fp8::groups(cols);
     LRB_REQUIRE(blocks < (1ll << 31), "moe_quantize_fp8_blocks: too many blocks");
     LRB_REQUIRE(banks == 0 || (w && q && scales), "moe_quantize_fp8_blocks: null tensor");
+    LRB_REQUIRE(lrb::on_boundary(w, 2) && lrb::on_boundary(scales, 4),
+                "moe_quantize_fp8_blocks: tensors must be aligned to their elements");
     if (banks == 0) return MOE_OK;
     if (int rc = lrb::require_sm100()) return rc;
     const bool vec = cols % 8 == 0 && lrb::aligned16(w) && (reinterpret_cast<uintptr_t>(q) & 7) == 0;

@@ -169,6 +169,31 @@ def test_banks_of_another_kind_under_the_same_key_are_made_anew(quantised):
     assert fewer.experts == 8 and pool.stats.resident_bytes == fewer.nbytes()
 
 
+def test_pointers_off_their_elements_are_refused(so):
+    """An address that the kernels' loads and stores cannot take is an argument
+    error, not a fault on the device."""
+    P = ctypes.c_void_p
+    ok, odd, half, four = P(1 << 20), P((1 << 20) + 1), P((1 << 20) + 2), P((1 << 20) + 4)
+
+    def refused(rc):
+        assert rc == native.MOE_EINVAL and b"aligned" in so.moe_last_error(), so.moe_last_error()
+
+    rows = dict(x=ok, res=ok, w=ok, q=ok, s=ok, normed=ok, total=ok)
+    for name, bad in (("x", odd), ("res", odd), ("w", odd), ("s", half), ("normed", odd), ("total", odd)):
+        a = {**rows, name: bad}
+        refused(so.moe_rmsnorm_fp8(a["x"], 64, a["res"], 64, a["w"], 1.0, 1e-6, 2, 64, a["q"], a["s"], a["normed"],
+                                   a["total"], None))
+    refused(so.moe_quantize_fp8_blocks(odd, 1, 4, 4, ok, ok, None))
+    refused(so.moe_quantize_fp8_blocks(ok, 1, 4, 4, ok, half, None))
+    for bad in (dict(xs=half), dict(ws=half), dict(status=half)):
+        a = {"xs": ok, "ws": ok, "status": None, **bad}
+        refused(so.moe_linear_fp8(ok, a["xs"], ok, a["ws"], 2, 64, 64, ok, 0, a["status"], None))
+    for bad in (dict(xs=half), dict(gus=half), dict(dns=half), dict(idx=four), dict(wt=odd), dict(status=half)):
+        a = {"xs": ok, "gus": ok, "dns": ok, "idx": ok, "wt": ok, "status": None, **bad}
+        refused(so.moe_experts_fp8(ok, a["xs"], ok, a["gus"], ok, a["dns"], a["idx"], a["wt"], 2, 4, 2, 64, 128, ok, ok,
+                                   1 << 24, a["status"], None))
+
+
 # ---------------------------------------------------------------- the build ---
 
 @pytest.fixture

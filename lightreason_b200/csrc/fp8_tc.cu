@@ -1428,7 +1428,10 @@ int experts_fp8_tile(int routes, int experts) {
 
 // FP32 rows cost nothing beside the weights on small batches; above 2048 routes
 // they are rounded to BF16, half the traffic of what then takes a tenth of the
-// time.
+// time (256 experts of 2048 x 512, top-8, at 300 / 1024 / 4096 / 8192 tokens: 135 /
+// 156 / 294 / 538 us, with FP32 rows 145 / 167 / 344 / 644).  The output's error
+// against 64 bits is then 0.0024 of its size instead of the 0.0017 of its own
+// rounding to BF16; the BF16 layer rounds the same rows.
 bool experts_fp8_wide_rows(int routes) { return routes <= kWideRoutes; }
 
 int launch_experts_fp8_tiles(const ExpertsFp8 &a, const ExpertsFp8Scratch &s, int32_t *status, cudaStream_t stream) {

@@ -150,7 +150,9 @@ class ExpertPool:
             if banks.takes(layer.gate_up, layer.down, shared, extra):
                 banks.load(layer.gate_up, layer.down, shared=shared, extra=extra)
                 return banks
-            self.stats.resident_bytes -= banks.nbytes()  # another module's, gone, under the same id
+            # another module's, gone, under the same id: its memory is free for the new ones
+            banks = None
+            self.stats.resident_bytes -= self._layers.pop(key).nbytes()
         # calls captured on other banks under this key go with those
         graphs = getattr(self, "replay_graphs", {})
         for old in [k for k in graphs if k[:2] == key[:2]]:

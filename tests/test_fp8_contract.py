@@ -169,6 +169,25 @@ def test_banks_of_another_kind_under_the_same_key_are_made_anew(quantised):
     assert fewer.experts == 8 and pool.stats.resident_bytes == fewer.nbytes()
 
 
+def test_resident_bytes_when_new_banks_fail(quantised):
+    """Banks that had to go are counted out once, however often making the new ones fails."""
+    from lightreason_b200 import expert_stream
+
+    pool = expert_stream.ExpertPool("cuda:0")
+    pool.device = torch.device("cpu")
+    gu, dn, shared, router = bank_weights()
+    module = SimpleNamespace(num_experts=20, hidden_dim=64, intermediate_dim=128)
+    layer = SimpleNamespace(module=module, residency="b200-fp8", gate_up=gu, down=dn)
+    pool._fp8_banks(layer)
+    quantised.fail_at = len(quantised.shapes)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="out of memory"):
+            pool._fp8_banks(layer, shared=tuple(shared), extra=(router,))
+        assert pool.stats.resident_bytes == 0
+    quantised.fail_at = None
+    assert pool._fp8_banks(layer).nbytes() == pool.stats.resident_bytes
+
+
 def test_pointers_off_their_elements_are_refused(so):
     """An address that the kernels' loads and stores cannot take is an argument
     error, not a fault on the device."""

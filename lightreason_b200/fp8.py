@@ -33,6 +33,7 @@ from lightreason_b200 import build, native
 from lightreason_b200.native import _require
 
 GROUP = 128
+MAX_ROUTES = 32  # of a token, in experts
 E4M3 = torch.float8_e4m3fn
 _BF16, _F32 = torch.bfloat16, torch.float32
 

@@ -39,6 +39,9 @@ class _Block:
             if block.shared_expert.gate_proj.weight.shape[0] != block.experts.intermediate_dim:
                 raise ValueError(f"{name}: FP8 blocks need a shared expert of the experts' width")
             fp8.check_widths(block.experts.hidden_dim, block.experts.intermediate_dim, block.experts.num_experts + 1)
+            if self.top_k + 1 > fp8.MAX_ROUTES:
+                raise ValueError(f"{name}: FP8 blocks take {fp8.MAX_ROUTES - 1} routes a token beside the shared expert, "
+                                 f"got {self.top_k}")
 
     def _extra(self):
         dev = self.pool.device

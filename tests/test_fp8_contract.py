@@ -169,6 +169,26 @@ def test_banks_of_another_kind_under_the_same_key_are_made_anew(quantised):
     assert fewer.experts == 8 and pool.stats.resident_bytes == fewer.nbytes()
 
 
+def test_block_patch_refuses_more_routes_than_the_experts_take():
+    """The shared expert is one route more: 32 routes a token are refused when
+    the block is patched, not at each call."""
+    from lightreason_b200 import expert_stream, moe_block
+    from transformers.models.qwen3_5_moe.configuration_qwen3_5_moe import Qwen3_5MoeTextConfig
+    from transformers.models.qwen3_5_moe.modeling_qwen3_5_moe import Qwen3_5MoeSparseMoeBlock
+
+    def block(top_k):
+        config = Qwen3_5MoeTextConfig(hidden_size=64, moe_intermediate_size=128, shared_expert_intermediate_size=128,
+                                      num_experts=40, num_experts_per_tok=top_k)
+        config._experts_implementation = "eager"
+        return Qwen3_5MoeSparseMoeBlock(config).to(torch.bfloat16).eval().requires_grad_(False)
+
+    pool = expert_stream.ExpertPool("cuda:0")
+    assert moe_block._Block("b", block(31), pool, "b200-fp8").top_k == 31
+    with pytest.raises(ValueError, match="31 routes a token"):
+        moe_block._Block("b", block(32), pool, "b200-fp8")
+    assert moe_block._Block("b", block(32), pool, "b200").top_k == 32
+
+
 def test_resident_bytes_when_new_banks_fail(quantised):
     """Banks that had to go are counted out once, however often making the new ones fails."""
     from lightreason_b200 import expert_stream
